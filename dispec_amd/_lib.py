@@ -11,6 +11,7 @@ does every kernel wrapper built on it.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
@@ -73,6 +74,17 @@ SIGNATURES: dict[str, tuple] = {
         c_int, [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, _P, c_int64, c_int32,
                 _P, _P, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_int32,
                 c_int32, _P, c_size_t, _P, c_int64, c_int64, c_int32, _P, _P]),
+    "dsp_tree_mask": (c_int, [_P, _P, c_int64, c_int32, c_int32, c_int32, _P, _P]),
+    "dsp_paged_tree_workspace_bytes": (c_size_t, [c_int32] * 6),
+    "dsp_paged_tree_attention": (c_int, [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64,
+        _P, c_int64, c_int32, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
+        c_int32, c_int32, _P, c_size_t, _P, c_int64, c_int64, c_int32, _P, _P]),
+    "dsp_verify_workspace_bytes": (c_size_t, [c_int32, c_int64]),
+    "dsp_verify_draft": (c_int, [_P, _P, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, _P,
+        c_int32, c_int32, c_int64, c_int32, _P, c_size_t, _P, _P, _P, _P, _P]),
+    "dsp_match_draft": (c_int, [_P, _P, _P, _P, c_int64, c_int32, c_int32, _P, _P, _P, _P]),
+    "dsp_kv_commit_path": (c_int, [_P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int32,
+        _P, c_int64, c_int32, _P, _P, _P, c_int64, c_int32, _P, c_int32, _P, _P]),
     "dsp_kv_map_gemm": (c_int, [_P, _I64P, c_int32, c_int64, c_int64, _P, c_int64, _P, c_int64,
                                 c_int64, c_int64, c_int64, c_int32, c_int64, c_int64, _P, c_int32,
                                 c_int32, c_int32, c_int32, _P]),
@@ -94,12 +106,13 @@ SIGNATURES: dict[str, tuple] = {
 _LIB: ctypes.CDLL | None = None
 _CALLS = None
 
-# Entry points a decode step calls once per layer: dispec_amd._fastcall (csrc/fastcall.c)
+# Entry points a decode step calls once per layer, or a speculative one once: dispec_amd._fastcall (csrc/fastcall.c)
 # binds them with METH_FASTCALL functions that take the same arguments as the ctypes
 # functions and skip ctypes' per-argument conversion (~4-5 us a call).
 FAST_CALLS = ("dsp_paged_decode", "dsp_kv_append", "dsp_paged_mq_attention",
               "dsp_paged_mq_attention_ragged", "dsp_paged_mq_attention_shared_prefix",
-              "dsp_qk_norm_rope_append")
+              "dsp_qk_norm_rope_append", "dsp_paged_tree_attention", "dsp_verify_draft",
+              "dsp_match_draft", "dsp_kv_commit_path")
 
 
 class HipLibraryError(RuntimeError):
@@ -209,6 +222,24 @@ def stream_of(t) -> int:
     if raw is not None:  # the handle itself, without building a torch Stream object
         return raw(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def on_device(t):
+    """A context in which t's device is the current one: a launch on a stream of another device
+    than the current fails.  (The device is nearly always the current one: no context then.)"""
+    import torch
+    index = t.get_device()
+    return _SAME if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+_SAME = contextlib.nullcontext()
+
+
+def same_device(t, *others) -> None:
+    """ValueError unless the tensors (or None) are on t's device."""
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError(f"tensors on {t.device} and {o.device}: one call takes one device")
 
 
 def require_gpu(*tensors) -> None:

@@ -121,3 +121,17 @@ __device__ __forceinline__ float dsp_shfl_xor(float x, int mask) {
 }
 
 __device__ __forceinline__ float dsp_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Which of the 32 keys from one on a tree's query sees (bit i: key i): all before the tree, and of
+// the tree's n nodes those of its mask, `words` 32-bit words at `row`.  a: the first key's node
+// (negative: so many keys before the tree).  Bits past the mask or the tree are 0.
+__device__ __forceinline__ uint32_t dsp_tree_window(const uint32_t* __restrict__ row, int words,
+                                                    int n, int a) {
+  if (a <= -32) return ~0u;
+  const int p = a > 0 ? a : 0, w = p >> 5, left = n - p;
+  if (left <= 0) return 0u;
+  const uint32_t lo = w < words ? row[w] : 0u, hi = w + 1 < words ? row[w + 1] : 0u;
+  uint32_t v = __builtin_amdgcn_alignbit(hi, lo, p & 31);
+  if (left < 32) v &= (1u << left) - 1u;
+  return a < 0 ? (v << -a) | ((1u << -a) - 1u) : v;
+}

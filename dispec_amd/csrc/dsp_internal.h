@@ -108,7 +108,8 @@ int prefill_ragged(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h,
 // dsp_paged_mq_attention.  log2_bs < 0 reads `table` as a per-token slot table.  Partial
 // results need generic_workspace_bytes(B, Hq, D, max_q_len, max_ctx, P) bytes of `workspace`
 // (none for a single partition).  Grid limits: B * max_q_len <= 2^26, ceil(max_ctx / P) <=
-// 65535 (else DSP_EUNSUPPORTED).
+// 65535 (else DSP_EUNSUPPORTED).  tree: not null: the masks of dsp_paged_tree_attention, `words`
+// words a query, with cu_q and by block table.
 bool generic_head_dim(int32_t D);
 size_t generic_workspace_bytes(int32_t B, int32_t Hq, int32_t D, int32_t max_q_len,
                                int32_t max_ctx, int32_t P);
@@ -119,6 +120,6 @@ int generic_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
                       int32_t Hq, int32_t KVH, int32_t D, float scale, int32_t max_q_len,
                       int32_t max_ctx, int32_t P, void* workspace, void* out,
                       int64_t o_stride_t, int64_t o_stride_h, int32_t dtype, int32_t* err_count,
-                      hipStream_t s);
+                      hipStream_t s, const uint32_t* tree = nullptr, int32_t words = 0);
 
 }  // namespace dsp_detail

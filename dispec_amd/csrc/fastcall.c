@@ -1,4 +1,5 @@
-/* CPython bindings of the C-ABI entry points that a decode step calls once per layer.
+/* CPython bindings of the C-ABI entry points that a decode step calls once per layer (and a
+ * speculative one once).
  *
  * ctypes converts each of a call's ~30 arguments through its argtypes before calling,
  * about 4-5 us per call, which is most of a small decode launch's host time.  These
@@ -81,6 +82,18 @@ typedef int (*prologue_fn)(void*, int64_t, int64_t, void*, int64_t, int64_t, voi
                            int64_t, void*, void*, float, void*, void*, int64_t, void*, int64_t,
                            int32_t, int32_t, int32_t, void*, int64_t, int64_t, void*, void*,
                            int64_t, int64_t, int64_t, int32_t, void*, void*);
+typedef int (*tree_fn)(void*, int64_t, int64_t, void*, void*, int64_t, int64_t, int64_t,
+                       void*, int64_t, int32_t, void*, void*, void*, int32_t, int32_t,
+                       int32_t, int32_t, int32_t, float, int32_t, int32_t, void*, size_t,
+                       void*, int64_t, int64_t, int32_t, void*, void*);
+typedef int (*verify_fn)(void*, void*, void*, int64_t, int64_t, void*, int64_t, int64_t,
+                         void*, void*, void*, int32_t, int32_t, int64_t, int32_t, void*,
+                         size_t, void*, void*, void*, void*, void*);
+typedef int (*match_fn)(void*, void*, void*, void*, int64_t, int32_t, int32_t, void*, void*,
+                        void*, void*);
+typedef int (*commit_fn)(void*, void*, int64_t, int64_t, int64_t, int64_t, int64_t, int32_t,
+                         void*, int64_t, int32_t, void*, void*, void*, int64_t, int32_t,
+                         void*, int32_t, void*, void*);
 
 static decode_fn p_decode;
 static append_fn p_append;
@@ -88,6 +101,10 @@ static mq_fn p_mq;
 static mq_ragged_fn p_mq_ragged;
 static mq_sp_fn p_mq_sp;
 static prologue_fn p_prologue;
+static tree_fn p_tree;
+static verify_fn p_verify;
+static match_fn p_match;
+static commit_fn p_commit;
 
 #define UNBOUND(ptr, name)                                                        \
   if (!(ptr)) {                                                                   \
@@ -186,6 +203,62 @@ static PyObject* w_prologue(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(st);
 }
 
+static const char kTreeSig[] = "PqqPPqqqPqiPPPiiiiifiiPzPqqiPP";
+static PyObject* w_tree(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  arg_t v[32];
+  UNBOUND(p_tree, "dsp_paged_tree_attention");
+  if (!convert("dsp_paged_tree_attention", kTreeSig, a, n, v)) return NULL;
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = p_tree(v[0].p, v[1].q, v[2].q, v[3].p, v[4].p, v[5].q, v[6].q, v[7].q, v[8].p,
+              v[9].q, v[10].i, v[11].p, v[12].p, v[13].p, v[14].i, v[15].i, v[16].i,
+              v[17].i, v[18].i, v[19].f, v[20].i, v[21].i, v[22].p, v[23].z, v[24].p,
+              v[25].q, v[26].q, v[27].i, v[28].p, v[29].p);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
+static const char kVerifySig[] = "PPPqqPqqPPPiiqiPzPPPPP";
+static PyObject* w_verify(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  arg_t v[32];
+  UNBOUND(p_verify, "dsp_verify_draft");
+  if (!convert("dsp_verify_draft", kVerifySig, a, n, v)) return NULL;
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = p_verify(v[0].p, v[1].p, v[2].p, v[3].q, v[4].q, v[5].p, v[6].q, v[7].q, v[8].p,
+                v[9].p, v[10].p, v[11].i, v[12].i, v[13].q, v[14].i, v[15].p, v[16].z,
+                v[17].p, v[18].p, v[19].p, v[20].p, v[21].p);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
+static const char kMatchSig[] = "PPPPqiiPPPP";
+static PyObject* w_match(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  arg_t v[32];
+  UNBOUND(p_match, "dsp_match_draft");
+  if (!convert("dsp_match_draft", kMatchSig, a, n, v)) return NULL;
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = p_match(v[0].p, v[1].p, v[2].p, v[3].p, v[4].q, v[5].i, v[6].i, v[7].p, v[8].p,
+               v[9].p, v[10].p);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
+static const char kCommitSig[] = "PPqqqqqiPqiPPPqiPiPP";
+static PyObject* w_commit(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  arg_t v[32];
+  UNBOUND(p_commit, "dsp_kv_commit_path");
+  if (!convert("dsp_kv_commit_path", kCommitSig, a, n, v)) return NULL;
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = p_commit(v[0].p, v[1].p, v[2].q, v[3].q, v[4].q, v[5].q, v[6].q, v[7].i, v[8].p,
+                v[9].q, v[10].i, v[11].p, v[12].p, v[13].p, v[14].q, v[15].i, v[16].p,
+                v[17].i, v[18].p, v[19].p);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
 /* bind(name, address): the entry point `name` of the loaded library is at `address`. */
 static PyObject* w_bind(PyObject* self, PyObject* args) {
   const char* name;
@@ -198,6 +271,10 @@ static PyObject* w_bind(PyObject* self, PyObject* args) {
   else if (!strcmp(name, "dsp_paged_mq_attention_ragged")) p_mq_ragged = (mq_ragged_fn)p;
   else if (!strcmp(name, "dsp_paged_mq_attention_shared_prefix")) p_mq_sp = (mq_sp_fn)p;
   else if (!strcmp(name, "dsp_qk_norm_rope_append")) p_prologue = (prologue_fn)p;
+  else if (!strcmp(name, "dsp_paged_tree_attention")) p_tree = (tree_fn)p;
+  else if (!strcmp(name, "dsp_verify_draft")) p_verify = (verify_fn)p;
+  else if (!strcmp(name, "dsp_match_draft")) p_match = (match_fn)p;
+  else if (!strcmp(name, "dsp_kv_commit_path")) p_commit = (commit_fn)p;
   else {
     PyErr_Format(PyExc_KeyError, "no fast binding for %s", name);
     return NULL;
@@ -215,6 +292,10 @@ static PyMethodDef kMethods[] = {
     {"dsp_paged_mq_attention_shared_prefix", (PyCFunction)(void (*)(void))w_mq_sp,
      METH_FASTCALL, NULL},
     {"dsp_qk_norm_rope_append", (PyCFunction)(void (*)(void))w_prologue, METH_FASTCALL, NULL},
+    {"dsp_paged_tree_attention", (PyCFunction)(void (*)(void))w_tree, METH_FASTCALL, NULL},
+    {"dsp_verify_draft", (PyCFunction)(void (*)(void))w_verify, METH_FASTCALL, NULL},
+    {"dsp_match_draft", (PyCFunction)(void (*)(void))w_match, METH_FASTCALL, NULL},
+    {"dsp_kv_commit_path", (PyCFunction)(void (*)(void))w_commit, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fastcall", NULL, -1, kMethods};
@@ -231,7 +312,11 @@ PyMODINIT_FUNC PyInit__fastcall(void) {
                {"dsp_paged_mq_attention", kMqSig},
                {"dsp_paged_mq_attention_ragged", kMqRaggedSig},
                {"dsp_paged_mq_attention_shared_prefix", kMqSpSig},
-               {"dsp_qk_norm_rope_append", kPrologueSig}};
+               {"dsp_qk_norm_rope_append", kPrologueSig},
+               {"dsp_paged_tree_attention", kTreeSig},
+               {"dsp_verify_draft", kVerifySig},
+               {"dsp_match_draft", kMatchSig},
+               {"dsp_kv_commit_path", kCommitSig}};
   PyObject* m = PyModule_Create(&kModule);
   if (!m) return NULL;
   PyObject* sigs = PyDict_New();

@@ -64,12 +64,16 @@ struct RowInfo {
   int vis;       // visible keys; 0 writes zeros
   bool live;     // false: slot beyond the sequence's q_len (nothing to write)
   bool counted;  // this slot reports the sequence's bad lengths (one slot per sequence)
+  int qlen;      // the sequence's queries
 };
 
+// (kTree: a row's keys end with the context, its mask says which of the tree's it sees)
+template <bool kTree>
 __device__ __forceinline__ RowInfo row_info(const int32_t* __restrict__ cu_q,
                                             const int32_t* __restrict__ ctx_lens,
                                             int max_q_len, int max_ctx, int z) {
   RowInfo r;
+  r.qlen = 1;
   r.b = z / max_q_len;
   const int i = z - r.b * max_q_len;
   const int ctx = ctx_lens[r.b];
@@ -85,8 +89,9 @@ __device__ __forceinline__ RowInfo row_info(const int32_t* __restrict__ cu_q,
   r.tok = int64_t(c0) + i;
   r.live = i < qlen;
   const bool bad = qlen < 0 || ctx < qlen || ctx > max_ctx;
-  r.vis = bad ? 0 : ctx - qlen + i + 1;
+  r.vis = bad ? 0 : kTree ? ctx : ctx - qlen + i + 1;
   r.counted = bad && i == 0;
+  r.qlen = qlen;
   return r;
 }
 
@@ -97,7 +102,7 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v + dsp_shfl_xor(v, 32);
 }
 
-template <typename Tag, int D>
+template <typename Tag, int D, bool kTree>
 __global__ __launch_bounds__(64) void generic_attn_kernel(
     const typename Tag::store* __restrict__ q, int64_t qst, int64_t qsh,
     const typename Tag::store* __restrict__ kc, const typename Tag::store* __restrict__ vc,
@@ -106,12 +111,12 @@ __global__ __launch_bounds__(64) void generic_attn_kernel(
     const int32_t* __restrict__ ctx_lens, int32_t G, int32_t max_ctx, int32_t max_q_len,
     float scale_log2, int32_t P, int32_t num_parts, float* __restrict__ ws_acc,
     float* __restrict__ ws_ml, typename Tag::store* __restrict__ out, int64_t ost, int64_t osh,
-    int32_t* __restrict__ err_count) {
+    int32_t* __restrict__ err_count, const uint32_t* __restrict__ tree, int32_t words) {
   constexpr int NV = D > 64 ? D / 64 : 1;  // dims per lane
   const int z = blockIdx.x, h = blockIdx.y, part = blockIdx.z, Hq = gridDim.y;
   const int lane = threadIdx.x;
   const bool act = lane < D;
-  const RowInfo r = row_info(cu_q, ctx_lens, max_q_len, max_ctx, z);
+  const RowInfo r = row_info<kTree>(cu_q, ctx_lens, max_q_len, max_ctx, z);
   if (!r.live) return;
   if (r.counted && part == 0 && h == 0 && lane == 0 && err_count) atomicAdd(err_count, 1);
   const int vis = r.vis;
@@ -138,6 +143,9 @@ __global__ __launch_bounds__(64) void generic_attn_kernel(
   float m = -INFINITY, l = 0.f;
   bool bad_slot = false;
   for (int k0 = kbeg; k0 < kend; k0 += kKeysPerStep) {
+    uint32_t seen = ~0u;
+    if constexpr (kTree)
+      seen = dsp_tree_window(tree + r.tok * words, words, r.qlen, k0 - (vis - r.qlen));
     float kv[kKeysPerStep][NV], vv[kKeysPerStep][NV], s[kKeysPerStep];
     bool ok[kKeysPerStep];
 #pragma unroll
@@ -151,6 +159,7 @@ __global__ __launch_bounds__(64) void generic_attn_kernel(
       }
       ok[u] = key < kend && sl >= 0 && sl < num_slots;
       bad_slot |= key < kend && !ok[u];
+      if constexpr (kTree) ok[u] = ok[u] && ((seen >> u) & 1u);
       const int64_t e = (ok[u] ? sl : 0) * kvs_slot + head_off;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -244,7 +253,7 @@ __device__ __forceinline__ void load_f32(const float* __restrict__ p, bool ok, f
 
 constexpr int kTileWaves = 4;
 
-template <int D>
+template <int D, bool kTree>
 __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2))) void f32_tile_kernel(
     const float* __restrict__ q, int64_t qst, int64_t qsh, const float* __restrict__ kc,
     const float* __restrict__ vc, int64_t num_slots, int64_t kvs_slot, int64_t kvs_head,
@@ -252,7 +261,8 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ ctx_lens, int32_t G,
     int32_t max_ctx, int32_t max_q_len, float scale_log2, int32_t P, int32_t num_parts,
     float* __restrict__ ws_acc, float* __restrict__ ws_ml, float* __restrict__ out, int64_t ost,
-    int64_t osh, int32_t* __restrict__ err_count) {
+    int64_t osh, int32_t* __restrict__ err_count, const uint32_t* __restrict__ tree,
+    int32_t words) {
   constexpr int KE = D >= 16 ? 4 : 2;          // floats per K load
   constexpr int KJ = D / (4 * KE);             // K loads per row and lane
   constexpr int VE = D >= 64 ? 4 : (D >= 32 ? 2 : 1);  // floats per V load
@@ -274,8 +284,12 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
     atomicAdd(err_count, 1);
   if (dec) ctx = ctx < 0 ? 0 : (ctx > max_ctx ? max_ctx : ctx);
   // keys visible to row r: its query's position + 1 (none for bad lengths or no context)
-  auto visible = [&](int r) { return !dec && bad_len ? 0 : ctx - qlen + r / G + 1; };
-  const int kend = visible(min(r0 + 15, rows - 1)), vis0 = visible(r0);
+  // (kTree: ctx, of which a row's mask says which of the tree's it sees)
+  auto visible = [&](int r) {
+    return !dec && bad_len ? 0 : kTree ? ctx : ctx - qlen + r / G + 1;
+  };
+  const int base = ctx - qlen;  // kTree: the tree's first key
+  const int kend = visible(min(r0 + 15, rows - 1)), vis0 = kTree ? base : visible(r0);
   const int kbeg = part * P, kfin = min(kbeg + P, kend);
   if (kbeg >= kend && part > 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -336,10 +350,19 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
             __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], qf[j][e], sc[(j * KE + e) % CH], 0, 0, 0);
 #pragma unroll
     for (int c = 1; c < CH; ++c) sc[0] += sc[c];
+    // which of this lane's keys its row sees: by their index, or (kTree) by the row's mask
+    uint32_t bits = 0;
+    if constexpr (kTree)
+      if (row_ok)
+        bits = dsp_tree_window(tree + int64_t(q0 + r / G) * words, words, qlen, t0 - base) >>
+               (4 * grp);
+    auto sees = [&](int j) {
+      return kTree ? ((bits >> j) & 1u) != 0 : t0 + 4 * grp + j < vis;
+    };
     float p[4], mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      p[j] = ok[j] && t0 + 4 * grp + j < vis ? sc[0][j] * scale_log2 : -INFINITY;
+      p[j] = ok[j] && sees(j) ? sc[0][j] * scale_log2 : -INFINITY;
       mx = fmaxf(mx, p[j]);
     }
     mx = fmaxf(mx, dsp_shfl_xor(mx, 16));
@@ -371,7 +394,7 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
         constexpr float kHuge = 0x1p127f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float seen = t0 + 4 * grp + j < vis ? kHuge : 0.f;
+          const float seen = sees(j) ? kHuge : 0.f;
 #pragma unroll
           for (int h = 0; h < VH; ++h)
 #pragma unroll
@@ -455,7 +478,7 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
 // Merge of a row's partitions: one wave per (row slot, head), four heads per workgroup (most row
 // slots of a ragged batch are empty: a quarter of the workgroups to start and end); lane d
 // folds dims d, d+64, ...
-template <typename Tag, int D>
+template <typename Tag, int D, bool kTree>
 __global__ __launch_bounds__(256) void generic_merge_kernel(
     const float* __restrict__ ws_acc, const float* __restrict__ ws_ml,
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ ctx_lens, int32_t max_ctx,
@@ -465,7 +488,7 @@ __global__ __launch_bounds__(256) void generic_merge_kernel(
   const int z = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (h >= Hq) return;
-  const RowInfo r = row_info(cu_q, ctx_lens, max_q_len, max_ctx, z);
+  const RowInfo r = row_info<kTree>(cu_q, ctx_lens, max_q_len, max_ctx, z);
   if (!r.live || r.vis <= P) return;  // one partition at most: written by the attention kernel
   const int nparts = (r.vis + P - 1) / P;
   const int64_t row0 = (int64_t(z) * Hq + h) * num_parts;
@@ -529,40 +552,55 @@ struct GenericArgs {
   void* out;
   int64_t ost, osh;
   int32_t* err_count;
+  const uint32_t* tree;  // tree masks of `words` words a row, or null
+  int32_t words;
 };
 
-template <typename Tag, int D>
+template <typename Tag, int D, bool kTree>
 int launch_generic_d(const GenericArgs& a, dim3 grid, dim3 mgrid, hipStream_t s) {
   using S = typename Tag::store;
   if constexpr (std::is_same<Tag, GF32>::value)
-    f32_tile_kernel<D><<<grid, 64 * kTileWaves, 0, s>>>(
+    f32_tile_kernel<D, kTree><<<grid, 64 * kTileWaves, 0, s>>>(
         static_cast<const S*>(a.q), a.qst, a.qsh, static_cast<const S*>(a.kc),
         static_cast<const S*>(a.vc), a.num_slots, a.kvs_slot, a.kvs_head, a.table, a.table_stride,
         a.log2_bs, a.cu_q, a.ctx_lens, a.G, a.max_ctx, a.max_q_len, a.scale_log2, a.P,
-        a.num_parts, a.ws_acc, a.ws_ml, static_cast<S*>(a.out), a.ost, a.osh, a.err_count);
+        a.num_parts, a.ws_acc, a.ws_ml, static_cast<S*>(a.out), a.ost, a.osh, a.err_count, a.tree,
+        a.words);
   else
-    generic_attn_kernel<Tag, D><<<grid, 64, 0, s>>>(
+    generic_attn_kernel<Tag, D, kTree><<<grid, 64, 0, s>>>(
         static_cast<const S*>(a.q), a.qst, a.qsh, static_cast<const S*>(a.kc),
         static_cast<const S*>(a.vc), a.num_slots, a.kvs_slot, a.kvs_head, a.table, a.table_stride,
         a.log2_bs, a.cu_q, a.ctx_lens, a.G, a.max_ctx, a.max_q_len, a.scale_log2, a.P,
-        a.num_parts, a.ws_acc, a.ws_ml, static_cast<S*>(a.out), a.ost, a.osh, a.err_count);
+        a.num_parts, a.ws_acc, a.ws_ml, static_cast<S*>(a.out), a.ost, a.osh, a.err_count, a.tree,
+        a.words);
   const int st = dsp_launch_status();
   if (st != DSP_OK || a.num_parts <= 1) return st;
-  generic_merge_kernel<Tag, D><<<mgrid, 256, 0, s>>>(a.ws_acc, a.ws_ml, a.cu_q, a.ctx_lens,
+  generic_merge_kernel<Tag, D, kTree><<<mgrid, 256, 0, s>>>(a.ws_acc, a.ws_ml, a.cu_q, a.ctx_lens,
                                                      a.max_ctx, a.max_q_len, a.P, a.num_parts,
                                                      a.Hq, static_cast<S*>(a.out), a.ost, a.osh);
   return dsp_launch_status();
 }
 
-template <typename Tag>
+template <typename Tag, bool kTree>
 int launch_generic(int D, const GenericArgs& a, dim3 grid, dim3 mgrid, hipStream_t s) {
   switch (D) {
-    case 8: return launch_generic_d<Tag, 8>(a, grid, mgrid, s);
-    case 16: return launch_generic_d<Tag, 16>(a, grid, mgrid, s);
-    case 32: return launch_generic_d<Tag, 32>(a, grid, mgrid, s);
-    case 64: return launch_generic_d<Tag, 64>(a, grid, mgrid, s);
-    case 128: return launch_generic_d<Tag, 128>(a, grid, mgrid, s);
-    case 256: return launch_generic_d<Tag, 256>(a, grid, mgrid, s);
+    case 8: return launch_generic_d<Tag, 8, kTree>(a, grid, mgrid, s);
+    case 16: return launch_generic_d<Tag, 16, kTree>(a, grid, mgrid, s);
+    case 32: return launch_generic_d<Tag, 32, kTree>(a, grid, mgrid, s);
+    case 64: return launch_generic_d<Tag, 64, kTree>(a, grid, mgrid, s);
+    case 128: return launch_generic_d<Tag, 128, kTree>(a, grid, mgrid, s);
+    case 256: return launch_generic_d<Tag, 256, kTree>(a, grid, mgrid, s);
+    default: return DSP_EUNSUPPORTED;
+  }
+}
+
+template <bool kTree>
+int launch_generic_type(int32_t dtype, int D, const GenericArgs& a, dim3 grid, dim3 mgrid,
+                        hipStream_t s) {
+  switch (dtype) {
+    case DSP_BF16: return launch_generic<GBf16, kTree>(D, a, grid, mgrid, s);
+    case DSP_F16: return launch_generic<GF16, kTree>(D, a, grid, mgrid, s);
+    case DSP_F32: return launch_generic<GF32, kTree>(D, a, grid, mgrid, s);
     default: return DSP_EUNSUPPORTED;
   }
 }
@@ -590,7 +628,7 @@ int generic_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
                       int32_t Hq, int32_t KVH, int32_t D, float scale, int32_t max_q_len,
                       int32_t max_ctx, int32_t P, void* workspace, void* out,
                       int64_t o_stride_t, int64_t o_stride_h, int32_t dtype, int32_t* err_count,
-                      hipStream_t s) {
+                      hipStream_t s, const uint32_t* tree, int32_t words) {
   if (B == 0 || max_q_len == 0) return DSP_OK;
   const int32_t num_parts = max_ctx > 0 ? (max_ctx + P - 1) / P : 1;
   const int64_t rows = int64_t(B) * max_q_len;
@@ -602,7 +640,7 @@ int generic_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
                 kv_stride_head, table, table_stride, log2_bs, cu_q, ctx_lens, Hq / KVH, Hq,
                 max_ctx, max_q_len, scale * 1.4426950408889634f, P, num_parts, ws_acc,
                 num_parts > 1 ? ws_acc + rows * Hq * num_parts * D : nullptr, out, o_stride_t,
-                o_stride_h, err_count};
+                o_stride_h, err_count, tree, words};
   dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(Hq),
             static_cast<unsigned>(num_parts));
   dim3 mgrid(static_cast<unsigned>(rows), static_cast<unsigned>((Hq + 3) / 4));
@@ -614,12 +652,8 @@ int generic_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
     grid = dim3(static_cast<unsigned>(tiles * num_parts), static_cast<unsigned>(KVH),
                 static_cast<unsigned>(B));
   }
-  switch (dtype) {
-    case DSP_BF16: return launch_generic<GBf16>(D, a, grid, mgrid, s);
-    case DSP_F16: return launch_generic<GF16>(D, a, grid, mgrid, s);
-    case DSP_F32: return launch_generic<GF32>(D, a, grid, mgrid, s);
-    default: return DSP_EUNSUPPORTED;
-  }
+  return tree ? launch_generic_type<true>(dtype, D, a, grid, mgrid, s)
+              : launch_generic_type<false>(dtype, D, a, grid, mgrid, s);
 }
 
 }  // namespace dsp_detail

@@ -356,3 +356,128 @@ def _ragged(q, k_cache, v_cache, block_table, cu_q, ctx_lens, block_size, scale,
         return False
     _lib.check(st, "dsp_paged_mq_attention_ragged")
     return True
+
+
+# ---- drafted trees: the last tokens of a context are the nodes of a tree
+@functools.lru_cache(maxsize=256)
+def _tree_ws_bytes(B, Hq, KVH, D, max_q_len, max_ctx) -> int:
+    return _lib.lib().dsp_paged_tree_workspace_bytes(B, Hq, KVH, D, max_q_len, max_ctx)
+
+
+def tree_mask(parents, cu_q, max_q_len=None, num_tokens=None):
+    """The masks of `paged_tree_attention` for trees given by their parents: (T, words) int32, bit
+    a % 32 of word a // 32 of a node's row set where node a is the node itself or an ancestor.
+
+    parents:    (T,) int32, the parent of each node within its sequence, before the node; a node
+                whose parent is not an earlier one (-1) is a root.  None: chains (causal masks).
+    cu_q:       (B+1,) int32 node offsets
+    max_q_len:  bound of the nodes of a sequence (computed from cu_q if omitted, which costs a
+                device->host copy)
+    num_tokens: T, for chains
+    """
+    _lib.require_gpu(parents, cu_q)
+    _lib.same_device(cu_q, parents)
+    if cu_q.dim() != 1 or not cu_q.numel():
+        raise ValueError(f"cu_q has shape {tuple(cu_q.shape)}: expected (B + 1,)")
+    if parents is None and num_tokens is None:
+        raise ValueError("num_tokens is needed where no parents are given")
+    if parents is not None:
+        if parents.dim() != 1 or num_tokens not in (None, parents.numel()):
+            raise ValueError(f"parents has shape {tuple(parents.shape)} for {num_tokens} nodes")
+        parents, num_tokens = _i32(parents), parents.numel()
+    cu_q = _i32(cu_q)
+    B = cu_q.numel() - 1
+    if max_q_len is None:
+        max_q_len = int((cu_q[1:] - cu_q[:-1]).max().item()) if B else 0
+    max_q_len = int(max_q_len)
+    words = max(1, -(-max_q_len // 32))
+    mask = torch.zeros((num_tokens, words), dtype=torch.int32, device=cu_q.device)
+    with _lib.on_device(cu_q):
+        _lib.check(_lib.calls().dsp_tree_mask(
+            _lib.ptr(parents), cu_q.data_ptr(), num_tokens, B, max_q_len, words, mask.data_ptr(),
+            _lib.stream_of(cu_q)), "dsp_tree_mask")
+    return mask
+
+
+def tree_workspace(batch, num_heads, num_kv_heads, head_dim, max_q_len, max_ctx, device):
+    """A float32 workspace for every `paged_tree_attention` launch of this shape, or None when it
+    needs none.  One buffer serves all layers of a forward: the launches run in stream order."""
+    need = _tree_ws_bytes(batch, num_heads, num_kv_heads, head_dim, max_q_len, max_ctx)
+    return torch.empty(need // 4 + 1, dtype=torch.float32, device=device) if need else None
+
+
+def paged_tree_attention(q, k_cache, v_cache, block_table, cu_q, ctx_lens, tree_mask, kv_groups,
+                         block_size=16, scale=None, max_q_len=None, max_ctx=None, out=None,
+                         err=None, workspace=None):
+    """Attention of drafted trees over the paged cache (dsp_paged_tree_attention).
+
+    Per sequence b, rows q[cu_q[b]:cu_q[b+1]] are the last tokens of a ctx_b-token context already
+    in the cache: the nodes of a tree.  A node sees every token before the tree and, of the tree,
+    the nodes of its mask; a node that sees nothing gives zeros.  A single-token sequence and a
+    prompt chunk (chain masks) may be in the same batch.
+
+    q:           (sum q_len, num_heads, head_dim), packed by sequence
+    block_table: (B, max_blocks) int32
+    cu_q:        (B+1,) int32 node offsets;  ctx_lens: (B,) int32 context lengths
+    tree_mask:   (sum q_len, words) int32, bit a % 32 of word a // 32: the row sees node a of its
+                 sequence (`tree_mask` makes it from parents); words >= max_q_len / 32
+    max_q_len, max_ctx: host-side bounds (computed from cu_q / the table if omitted, the former at
+                 the cost of a device->host copy)
+    workspace:   optional preallocated buffer (`tree_workspace`), for one stream at a time
+    err:         optional int32 device counter of bad lengths and block ids
+    returns:     (sum q_len, num_heads, head_dim) in q's dtype
+    """
+    _lib.require_gpu(q, k_cache, v_cache, block_table, cu_q, ctx_lens, tree_mask, out, err, workspace)
+    _lib.same_device(q, k_cache, v_cache, block_table, cu_q, ctx_lens, tree_mask, out, err,
+                     workspace)
+    if q.dim() != 3 or k_cache.dim() != 3 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"expected q (T, Hq, D) and caches (S, KVH, D); got {tuple(q.shape)}, "
+                         f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    T, Hq, D = q.shape
+    S, KVH, Dk = k_cache.shape
+    if Dk != D or Hq != KVH * kv_groups:
+        raise ValueError(f"q has {Hq} heads of {D}, cache {KVH} heads of {Dk}, kv_groups {kv_groups}")
+    if q.dtype not in _DTYPES or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError(f"q/k/v dtypes {q.dtype}/{k_cache.dtype}/{v_cache.dtype}: "
+                         "the HIP kernels take bf16, fp16 or fp32, all the same")
+    if k_cache.stride() != v_cache.stride() or k_cache.stride(2) != 1:
+        raise ValueError("k_cache and v_cache need the same strides with head_dim contiguous")
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    cu_q, ctx_lens, block_table = _i32(cu_q), _i32(ctx_lens), _i32(block_table)
+    B = ctx_lens.numel()
+    if cu_q.numel() != B + 1 or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"cu_q has {cu_q.numel()} entries, block_table shape "
+                         f"{tuple(block_table.shape)} for {B} sequences")
+    if max_q_len is None:
+        max_q_len = int((cu_q[1:] - cu_q[:-1]).max().item()) if B else 0
+    if max_ctx is None:
+        max_ctx = block_table.shape[1] * block_size
+    max_q_len, max_ctx = int(max_q_len), int(max_ctx)
+    if max_ctx > block_table.shape[1] * block_size:
+        raise ValueError(f"max_ctx {max_ctx} exceeds the table's {block_table.shape[1]} blocks")
+    if (tree_mask.dim() != 2 or tree_mask.dtype != torch.int32 or tree_mask.shape[0] != T
+            or tree_mask.shape[1] * 32 < max_q_len):
+        raise ValueError(f"tree_mask must be (T, words) int32 with a bit for each of {max_q_len} "
+                         f"nodes; got {tuple(tree_mask.shape)} {tree_mask.dtype} for {T} rows")
+    tree_mask = tree_mask.contiguous()
+    scale = D ** -0.5 if scale is None else scale
+    out = torch.empty_like(q) if out is None else out
+    if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("out must have q's shape and dtype with head_dim contiguous")
+    if not T:
+        return out
+    need = _tree_ws_bytes(B, Hq, KVH, D, max_q_len, max_ctx)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        # (of a size with the chip, not the batch: from torch's stream-ordered allocator per call)
+        workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+    with _lib.on_device(q):
+        _lib.check(_lib.calls().dsp_paged_tree_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), S,
+            k_cache.stride(0), k_cache.stride(1), block_table.data_ptr(), block_table.stride(0),
+            block_size, cu_q.data_ptr(), ctx_lens.data_ptr(), tree_mask.data_ptr(),
+            tree_mask.shape[1], B, Hq, KVH, D, float(scale), max_q_len, max_ctx,
+            _lib.ptr(workspace), need, out.data_ptr(), out.stride(0), out.stride(1),
+            _lib.dtype_code(q.dtype), _lib.ptr(err), _lib.stream_of(q)),
+            "dsp_paged_tree_attention")
+    return out

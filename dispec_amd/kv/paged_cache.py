@@ -14,6 +14,7 @@ working.  What changes is who moves the bytes:
   import_contiguous  -> dsp_kv_scatter_ordered (:92-96)
   copy_blocks        -> dsp_kv_copy_blocks   (new: the data move behind copy-on-write
                                               fork and prefix-cache spill)
+  commit_path        -> dsp_kv_commit_path   (new: the kept path of a drafted tree)
 
 Kernels never read or write out of the pool: an out-of-range slot or block id is
 skipped and counted in a device counter; `check_errors()` (or DISPEC_HIP_CHECK=1, which
@@ -57,6 +58,54 @@ def check_prefix_coverage(covered: int, prompt_len: int) -> None:
     if not 0 < covered < prompt_len:
         raise ValueError(f"prefix_kv covers {covered} tokens of a {prompt_len}-token "
                          "prompt; it must cover at least one and fewer than all of them")
+
+
+def commit_path(key, value, block_table, cu_q, ctx_lens, path, num_accepted, block_size=16,
+                err=None) -> None:
+    """Move the K and V rows of each sequence's kept path right behind its context, in place and
+    over all layers (dsp_kv_commit_path): of sequence b, whose last cu_q[b+1] - cu_q[b] tokens are
+    the nodes of a drafted tree that starts at position `base`, the rows of node path[b, j] go from
+    position base + path[b, j] to base + j, j = 1 .. num_accepted[b].
+
+    key, value:   (num_layers, num_slots, num_kv_heads, head_dim), the pool's layout
+    block_table:  (B, max_blocks) int32; the blocks of the trees belong to one sequence each
+    cu_q:         (B+1,) int32;  ctx_lens: (B,) int32, the trees included
+    path:         (B, width) int32, rising from path[b, 0] = 0 (`DraftVerdict.path`)
+    num_accepted: (B,) int32 (`DraftVerdict.num_accepted`)
+    err:          optional int32 device counter of slots outside the pool and of paths that do not
+                  go down a tree (from there on nothing is moved)
+    """
+    _lib.require_gpu(key, value, block_table, cu_q, ctx_lens, path, num_accepted, err)
+    _lib.same_device(key, value, block_table, cu_q, ctx_lens, path, num_accepted, err)
+    if key.dim() != 4 or key.shape != value.shape or key.dtype != value.dtype:
+        raise ValueError(f"expected pools (L, slots, KVH, D) of one shape and dtype; got "
+                         f"{tuple(key.shape)} {key.dtype}, {tuple(value.shape)} {value.dtype}")
+    L, S, KVH, D = key.shape
+    if key.stride() != value.stride() or key.stride(3) != 1 or key.stride(2) != D:
+        raise ValueError("key and value need the same strides with contiguous rows")
+    B = ctx_lens.numel()
+    if (block_table.dim() != 2 or block_table.shape[0] != B or cu_q.numel() != B + 1
+            or path.dim() != 2 or path.shape[0] != B or num_accepted.numel() != B):
+        raise ValueError(f"block_table {tuple(block_table.shape)}, cu_q {tuple(cu_q.shape)}, path "
+                         f"{tuple(path.shape)}, num_accepted {tuple(num_accepted.shape)} for {B} "
+                         "sequences")
+    for t, name in ((block_table, "block_table"), (cu_q, "cu_q"), (ctx_lens, "ctx_lens"),
+                    (path, "path"), (num_accepted, "num_accepted")):
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} must be int32, got {t.dtype}")
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        block_table = block_table.contiguous()
+    if path.stride(1) != 1 and path.shape[1] > 1:
+        path = path.contiguous()
+    cu_q, ctx_lens, num_accepted = (t.contiguous() for t in (cu_q, ctx_lens, num_accepted))
+    es = key.element_size()
+    with _lib.on_device(key):
+        _lib.check(_lib.calls().dsp_kv_commit_path(
+            key.data_ptr(), value.data_ptr(), L, key.stride(0) * es, key.stride(1) * es, S,
+            KVH * D * es, block_size, block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(), path.data_ptr(),
+            path.stride(0), path.shape[1], num_accepted.data_ptr(), B, _lib.ptr(err),
+            _lib.stream_of(key)), "dsp_kv_commit_path")
 
 
 class PagedKVCache:
@@ -348,6 +397,14 @@ class PagedKVCache:
             self.key.data_ptr(), self.value.data_ptr(), self.layer_bytes, self.num_blocks,
             self.num_layers, self.block_bytes, int(src_block), dst_ids.data_ptr(),
             dst_ids.numel(), self._err.data_ptr(), self._stream()), "dsp_kv_copy_block_fanout")
+
+    def commit_path(self, block_table: torch.Tensor, cu_q: torch.Tensor, ctx_lens: torch.Tensor,
+                    path: torch.Tensor, num_accepted: torch.Tensor) -> None:
+        """Every layer's rows of the kept paths of drafted trees move right behind their contexts
+        (see `commit_path`); int32 tensors on the GPU."""
+        commit_path(self.key, self.value, block_table, cu_q, ctx_lens, path, num_accepted,
+                    block_size=self.block_size, err=self._err)
+        self._after()
 
     # -- block copies (copy-on-write, prefix-cache spill) ----------------------------------
     def copy_blocks_from(self, src: "PagedKVCache", src_ids: list[int], dst_ids: list[int]) -> None:

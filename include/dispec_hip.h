@@ -365,6 +365,110 @@ int dsp_paged_mq_attention_shared_prefix(
     void* workspace, size_t workspace_bytes, void* out, int64_t o_stride_t, int64_t o_stride_h,
     int32_t dtype, int32_t* err_count, dsp_stream_t stream);
 
+/* ------------------------------------------------------------------- drafted trees
+ * Speculative decoding with a tree of drafted tokens instead of a chain (the reference drafts
+ * and verifies chains: dispec/spec/speculative.py:71-157, dispec/spec/rejection.py:25-54).  The
+ * last q_len_b = cu_q[b+1] - cu_q[b] context tokens of sequence b are the nodes of a tree; node 0
+ * is the last token that was kept, and a node comes after its parent.
+ *
+ * The masks of dsp_paged_tree_attention for trees given by their parents: bit a (word a / 32, bit
+ * a % 32) of node i's row is set where a is i or an ancestor of i.
+ *   parents   : int32 [num_rows], a node's parent within its sequence; a node whose parent is not
+ *               an earlier one (-1) is a root.  NULL: chains, whose masks are causal.
+ *   cu_q      : int32 [B+1]; of a sequence the first max_q_len nodes are written, none at or past
+ *               num_rows.
+ *   mask      : int32 [num_rows, mask_words], mask_words >= ceil(max_q_len / 32). */
+int dsp_tree_mask(const int32_t* parents, const int32_t* cu_q, int64_t num_rows, int32_t B,
+                  int32_t max_q_len, int32_t mask_words, int32_t* mask, dsp_stream_t stream);
+
+/* Attention of drafted trees over the paged cache: dsp_paged_mq_attention's arguments and layout
+ * with a mask among the last tokens instead of the causal one.  With base_b = ctx_lens[b] -
+ * q_len_b, query i of sequence b sees the keys j < base_b and, of the tree, the keys base_b + a
+ * whose bit a of mask row cu_q[b] + i is set (bits at or past q_len_b count for nothing):
+ *     out[i, h] = softmax_j(scale * q[i, h] . K[j, h / G]) . V[j, h / G]
+ * A row that sees no key is zeros.  The nodes' K/V must already be in the cache.
+ *   tree_mask : int32 [sum q_len, mask_words], rows contiguous, mask_words >= max_q_len / 32.
+ *   max_q_len : bound of q_len_b; of a longer sequence the first max_q_len rows are computed.
+ *   workspace : dsp_paged_tree_workspace_bytes bytes for the same arguments on the same device
+ *               (16-byte aligned; none where that is 0).
+ * dtype DSP_BF16, DSP_F16 or DSP_F32, D a power of two from 8 to 256, any G.  A sequence with
+ * q_len > ctx or ctx > max_ctx is counted in err_count and its rows written as zeros; keys of
+ * block ids outside the cache are counted and skipped.  Infinities and NaN of a key's V reach the
+ * rows that see the key. */
+size_t dsp_paged_tree_workspace_bytes(int32_t B, int32_t Hq, int32_t KVH, int32_t D,
+                                      int32_t max_q_len, int32_t max_ctx);
+int dsp_paged_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                             const void* k_cache, const void* v_cache, int64_t num_slots,
+                             int64_t kv_stride_slot, int64_t kv_stride_head,
+                             const int32_t* block_table, int64_t bt_stride, int32_t block_size,
+                             const int32_t* cu_q, const int32_t* ctx_lens,
+                             const int32_t* tree_mask, int32_t mask_words, int32_t B, int32_t Hq,
+                             int32_t KVH, int32_t D, float scale, int32_t max_q_len,
+                             int32_t max_ctx, void* workspace, size_t workspace_bytes, void* out,
+                             int64_t o_stride_t, int64_t o_stride_h, int32_t dtype,
+                             int32_t* err_count, dsp_stream_t stream);
+
+/* Which path of each tree the target keeps, and the token after it, from given random numbers
+ * (the reference decides chains: dispec/spec/rejection.py:25-54).  p_i, row cu_q[b] + i of
+ * target_probs, is the target's distribution after node i; u_i the uniform of that row.
+ *   draft_probs given: a chain (parents NULL) whose tokens were drawn from them.  Node i's
+ *     successor, of token x, is kept where u_i q_i(x) < p_i(x); after the last node i that is
+ *     kept the next token is drawn from max(p_i - q_i, 0), after the chain's end from p_i.  A
+ *     sequence of n nodes has n - 1 rows q_0 .. q_{n-2}, an empty one none, packed.
+ *   draft_probs NULL: a tree (parents NULL: a chain) of proposed tokens.  Of node i's children, in
+ *     order, the first is kept for which u_i < p_i(x_1) + ... + p_i(x) (a token that an earlier
+ *     one holds counts once); after the last node that is kept the next token is drawn from p_i
+ *     without its children's tokens.
+ * Drawn is the least v with r_0 + ... + r_v > u' S, u' = final_uniforms[b], S the sum of the row r;
+ * where r is zero throughout, from p_i.  Products, sums and comparisons are in 64 bits.
+ *   draft_tokens : int64 [num_rows] (a root's is not read).  A token outside [0, V) is never kept
+ *                  and counted; a node whose parent is not an earlier node is never reached.
+ *   target_probs : [num_rows, V], draft_probs [num_draft_rows, V], rows at a stride, of `dtype`,
+ *                  not negative; V < 2^31.  Of a row that has no positive, finite sum no token is
+ *                  drawn (-1), and it is counted.  Of NaN and negative entries none is drawn.
+ *   uniforms     : fp32 [num_rows], final_uniforms fp32 [B], in [0, 1).
+ *   cu_q         : int32 [B+1]; of a sequence the first max_q_len nodes count (<= 1024).
+ *   num_accepted : int32 [B], the kept nodes besides the root.
+ *   path         : int32 [B, max_q_len], the kept nodes from the root (0) on, then -1.
+ *   tokens       : int64 [B, max_q_len], their tokens without the root's, the drawn token, then -1.
+ *                  (An empty sequence has 0, and -1 throughout.)
+ *   workspace    : dsp_verify_workspace_bytes(B, V) bytes, 8-byte aligned. */
+size_t dsp_verify_workspace_bytes(int32_t B, int64_t V);
+int dsp_verify_draft(const int64_t* draft_tokens, const int32_t* parents,
+                     const void* target_probs, int64_t target_stride, int64_t num_rows,
+                     const void* draft_probs, int64_t draft_stride, int64_t num_draft_rows,
+                     const float* uniforms, const float* final_uniforms, const int32_t* cu_q,
+                     int32_t B, int32_t max_q_len, int64_t V, int32_t dtype, void* workspace,
+                     size_t workspace_bytes, int32_t* num_accepted, int32_t* path,
+                     int64_t* tokens, int32_t* err_count, dsp_stream_t stream);
+
+/* The same verdict where the target's token after each node is known (greedy decoding, or sampled
+ * already): target_tokens int64 [num_rows].  A child is kept where its token is the target's after
+ * its parent (the first of several); the token after the path is the target's. */
+int dsp_match_draft(const int64_t* draft_tokens, const int64_t* target_tokens,
+                    const int32_t* parents, const int32_t* cu_q, int64_t num_rows, int32_t B,
+                    int32_t max_q_len, int32_t* num_accepted, int32_t* path, int64_t* tokens,
+                    dsp_stream_t stream);
+
+/* Commit of the kept paths: of every layer, the K and V rows of node path[b, j] (position base_b +
+ * path[b, j], base_b = ctx_lens[b] - q_len_b) move to position base_b + j, j = 1 .. num_accepted[b],
+ * in place (what follows is BlockManager.truncate, dispec/kv/block_manager.py:128-141).  Bit-exact.
+ *   k_pool, v_pool : all layers, rows of row_bytes at pool_slot_stride_bytes, layers at
+ *                    pool_layer_stride_bytes.
+ *   block_table    : int32 [B, bt_cols] rows at bt_stride; blocks that hold trees belong to one
+ *                    sequence.
+ *   path           : int32 [B, path_cols] rows at path_stride (<= 1024 columns), path[b, 0] = 0,
+ *                    rising.  From an entry on that does not rise or is no node nothing is moved,
+ *                    and the sequence is counted; so is a row whose slot lies outside the pool,
+ *                    which is left alone.  num_accepted is clamped to path_cols - 1. */
+int dsp_kv_commit_path(void* k_pool, void* v_pool, int64_t num_layers,
+                       int64_t pool_layer_stride_bytes, int64_t pool_slot_stride_bytes,
+                       int64_t num_slots, int64_t row_bytes, int32_t block_size,
+                       const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
+                       const int32_t* cu_q, const int32_t* ctx_lens, const int32_t* path,
+                       int64_t path_stride, int32_t path_cols, const int32_t* num_accepted,
+                       int32_t B, int32_t* err_count, dsp_stream_t stream);
+
 /* ------------------------------------------------------------------------------ J5b
  * The cross-model map GEMM: C[M, N] = epilogue(A[M, K] . Bt[N, K]^T), bf16 operands,
  * fp32 accumulation (MFMA).  Replaces the matmuls of LayerMap.apply
