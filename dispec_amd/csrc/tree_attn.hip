@@ -9,17 +9,20 @@
 // that hold nodes only, the last one to few.
 //
 // Tile (16-bit caches): NW waves of 32 packed rows each (row r: query r / G of head kvh G + r % G)
-// share 64-key chunks of K and V that the LDS DMA brings in, double-buffered; S^T = K Q^T and O^T =
-// V^T P^T on v_mfma_f32_32x32x16, with P in registers (dsp_tile32.h), a running maximum that moves
-// when it is exceeded by 2^8, sums and accumulators in fp32.  The probabilities enter P V as one
-// 16-bit operand (rounded to nearest; the sum takes the unrounded ones): half a step of the type,
-// as much as the output's own rounding.
-//  * 4 waves (128 rows) for up to 128 rows a KV head, 8 waves (256 rows, a chunk loaded once for
-//    twice the rows) above.
+// share 64-key chunks of K and V that the LDS DMA brings in; S^T = K Q^T and O^T = V^T P^T on
+// v_mfma_f32_32x32x16, with P in registers (dsp_tile32.h), a running maximum that moves when it is
+// exceeded by 2^8, sums and accumulators in fp32.  The probabilities enter P V as one 16-bit operand
+// (rounded to nearest; the sum takes the unrounded ones): half a step of the type, as much as the
+// output's own rounding.
+//  * Two workgroups of 4 waves (128 rows) to a CU for up to 128 rows a KV head, one of 8 waves (256
+//    rows, a chunk loaded once for twice the rows) above.
 //  * The list of (sequence, KV head, tile, chunk) units is cut into as many equal runs as there are
 //    workgroups resident on the chip, computed on the device from the lengths.  A run's end within
 //    kSnap chunks of a tile's end moves onto it.  A tile inside a run is written; a tile that runs
 //    cut leaves its rows' maximum, sum and accumulator per piece, and the second launch merges them.
+//  * What bounds it, heads of 128 in bf16: 32 trees of 16 nodes (G 2, 500 to 4000 tokens, 321 MB) 81
+//    us, where the loads alone take 79; 4 trees of 64 (G 4, 32768 tokens) 205 us, 670 TFLOP/s: two
+//    waves a SIMD issue for 74 % of the time, what they compute runs on the matrix cores for 38 %.
 // Everything else (fp32 caches, other head dims, blocks of fewer than 16 tokens, rows off 16 bytes,
 // a scale that is not positive) runs on the kernels of generic_attn.hip with the same masks.
 #include <float.h>
@@ -38,6 +41,8 @@ using namespace dsp_mfma;
 constexpr int kChunk = 64;     // keys per chunk
 constexpr int kMinChunks = 2;  // a workgroup gets at least this many chunks
 constexpr int kSnap = 2;
+constexpr int kBlocks = 2048;  // block ids of a piece held in LDS
+constexpr int kDesc = 8;       // ints that describe a run's merge: pieces, q0, rows, KV head, tile
 constexpr int kMaskThreads = 256;
 
 // One thread a node: its mask row is its own bit and its ancestors'.  Parents come before their
@@ -66,6 +71,22 @@ __global__ __launch_bounds__(kMaskThreads) void tree_mask_kernel(
     bits = 0;
   }
 }
+
+// a / b for 0 <= a < 2^24, 0 < b < 2^24: a reciprocal (to 24 bits, so that a times it is off by
+// less than 1) and one correction, where the compiler's division is tens of instructions (a
+// workgroup runs a chain of them before its first load).
+struct Div {
+  int b;
+  float inv;
+  __device__ __forceinline__ explicit Div(int d) : b(d) {
+    const float f = float(d), x = __builtin_amdgcn_rcpf(f);
+    inv = fmaf(fmaf(-f, x, 1.f), x, x);
+  }
+  __device__ __forceinline__ int operator()(int a) const {
+    const int q = int(float(a) * inv), r = a - q * b;
+    return r < 0 ? q - 1 : (r >= b ? q + 1 : q);
+  }
+};
 
 // One sequence: `tiles` of TR packed rows (its first max_q_len nodes'), each of `chunks` units (one
 // unit a tile where the tiles stay whole).
@@ -110,19 +131,61 @@ __device__ __forceinline__ int wave_incl_scan(int v) {
   return v;
 }
 
-template <typename Tag, int D, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(
-    D > 128 ? 1 : D > 64 ? 2 : NW > 4 ? 4 : 3))) void tree_tile_kernel(
+// The shape of a tile: kNW waves of 32 rows, and buffers of a chunk's K and V: 128 KiB of them on a CU,
+// for kPerCU workgroups.
+template <int kNW, int kPerCU>
+struct Shape {
+  static constexpr int NW = kNW, TR = 32 * kNW;
+  static constexpr int bufs(int D) { return 128 * 1024 / (4 * kChunk * D) / kPerCU; }
+};
+
+// Waits until at most n chunks' loads (kLoads each) of this wave are out, n <= kMost.
+template <int kMost, int kLoads>
+__device__ __forceinline__ void wait_chunks(int n) {
+  if constexpr (kMost > 0) {
+    if (n >= kMost) {
+      __builtin_amdgcn_s_waitcnt(dsp_waitcnt_vm<kMost * kLoads>());
+      return;
+    }
+    wait_chunks<kMost - 1, kLoads>(n);
+  } else {
+    __builtin_amdgcn_s_waitcnt(dsp_waitcnt_vm<0>());
+  }
+}
+
+template <typename Tag>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  if constexpr (std::is_same<Tag, Bf16Tag>::value)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+
+template <typename Tag>
+__device__ __forceinline__ float low(uint32_t two) {
+  return std::is_same<Tag, Bf16Tag>::value ? dsp_bf16lo(two) : dsp_f16lo(two);
+}
+template <typename Tag>
+__device__ __forceinline__ float high(uint32_t two) {
+  return std::is_same<Tag, Bf16Tag>::value ? dsp_bf16hi(two) : dsp_f16hi(two);
+}
+
+template <typename Tag, int D, typename S>
+__global__ __launch_bounds__(64 * S::NW) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2))) void
+tree_tile_kernel(
     const uint16_t* __restrict__ q, int64_t qst, int64_t qsh, const uint16_t* __restrict__ kc,
-    const uint16_t* __restrict__ vc, int64_t num_slots, int64_t kvs_slot, int64_t kvs_head,
+    const uint16_t* __restrict__ vc, uint32_t num_blocks, int32_t kvs_slot, int64_t kvs_head,
     const int32_t* __restrict__ bt, int64_t bt_stride, int32_t log2_bs,
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ ctx_lens,
     const uint32_t* __restrict__ mask, int32_t words, int32_t B, int32_t KVH, int32_t G,
-    int32_t max_q_len, int32_t max_ctx, float scale_log2, int32_t whole,
-    float* __restrict__ ws_acc, float* __restrict__ ws_ml, int32_t* __restrict__ ws_desc,
-    uint16_t* __restrict__ out, int64_t ost, int64_t osh, int32_t vec_out,
-    int32_t* __restrict__ err_count) {
-  constexpr int TR = 32 * NW;                    // packed rows per tile
+    int32_t max_q_len, int32_t max_ctx, float scale_log2, int32_t whole, int32_t least,
+    int32_t tiles_max, float* __restrict__ ws_acc, float* __restrict__ ws_ml,
+    int32_t* __restrict__ ws_desc, uint16_t* __restrict__ out, int64_t ost, int64_t osh,
+    int32_t vec_out, int32_t* __restrict__ err_count) {
+  constexpr int NW = S::NW, TR = S::TR, NB = S::bufs(D);
   constexpr int NKS = D / 16, NDT = D / 32;      // 16-dim steps of K Q^T, 32-dim tiles of V^T P^T
   constexpr int CPR = D / 8, ROWB = 2 * D;       // 16-byte pieces and bytes of a K or V row
   constexpr int SLAB = kChunk * ROWB;            // a chunk of K (or V)
@@ -130,8 +193,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(
   constexpr int LPW = SLAB / 1024 / NW;          // loads per wave and slab
   constexpr int RPW = kChunk / NW;               // rows per wave: one block's
   static_assert(LPW >= 1 && LPW * RPI == RPW && RPW <= 16, "a wave's rows lie in one block");
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][SLAB];  // [buffer][K | V]
-  __shared__ int32_t s_flag[2][NW];              // of each wave's rows: 1 bad block, 2 odd values
+  // Stage c of a piece is V of its chunk c and K of chunk c + 1, what one turn of the loop needs.
+  // [buffer][K | V]
+  __shared__ __attribute__((aligned(1024))) char lds[NB][2][SLAB];
+  // of each wave's rows: bit 2 wave: K's block id is bad, 2 wave + 1: odd values in V
+  __shared__ __attribute__((aligned(16))) int32_t s_flag[NB][NW];
+  __shared__ int32_t s_blk[kBlocks + 16];        // block ids of a piece (16: read ahead, not used)
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -153,12 +220,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(
   for (int f = 0; f < B; f += 64) {
     look(f);
     total += __builtin_amdgcn_readlane(incl, 63);
-    // bad lengths: counted once, the rows written as zeros, one sequence per workgroup
-    for (int b = lin; b < B; b += gridDim.x) {
-      if (b < f || b >= f + 64) continue;
-      const TreeSeq s = lane_seq(mine, b - f);
-      if (!tree_bad(s.n, s.ctx, max_ctx)) continue;
+    // bad lengths (rare): counted once, the rows written as zeros, one sequence per workgroup
+    uint64_t bad = __ballot(f + lane < B && tree_bad(mine.n, mine.ctx, max_ctx));
+    for (; bad; bad &= bad - 1) {
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(bad)) - 1);
+      if ((f + l) % int(gridDim.x) != lin) continue;
       if (threadIdx.x == 0 && err_count) atomicAdd(err_count, 1);
+      const TreeSeq s = lane_seq(mine, l);
       const int row = KVH * G * D, n = min(s.n, max_q_len);
       for (int i = 0; i < n; ++i)
         for (int e = threadIdx.x; e < row; e += 64 * NW)
@@ -166,17 +234,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(
     }
   }
   const int C = total * KVH;
-  const int least = whole ? 1 : kMinChunks;
-  const int W = min((C + least - 1) / least, int(gridDim.x));
+  const int W = min(Div(least)(C + least - 1), int(gridDim.x));
   if (lin >= W) {
-    if (!whole && threadIdx.x == 0) ws_desc[4 * lin + 3] = 0;
+    if (!whole && tiles_max == 0 && threadIdx.x == 0) ws_desc[kDesc * lin] = 0;
     return;
   }
   // workgroup lin runs on XCD lin % 8: each XCD takes a contiguous part of the list, so that the
   // tiles and pieces of one (sequence, KV head) share an L2
   const int q8 = W / 8, r8 = W % 8, xcd = lin % 8, pos = lin / 8;
   const int w = xcd < r8 ? xcd * (q8 + 1) + pos : r8 * (q8 + 1) + (xcd - r8) * q8 + pos;
-  const int share = C / W, extra = C - share * W;
+  const Div by_w(W);
+  const int share = by_w(C), extra = C - share * W;
   int b = 0, kvh = 0, tile = 0, c0 = 0;  // where the run stands
   int base = 0;                          // units (of all KV heads) before sequence b
   TreeSeq sq;
@@ -196,15 +264,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(
       pre += __builtin_amdgcn_readlane(incl, 63);
     }
     int rest = u - base;
-    kvh = rest / sq.units;
+    kvh = __builtin_amdgcn_readfirstlane(Div(sq.units)(rest));
     rest -= kvh * sq.units;
-    if (whole) {
-      tile = rest;
-      c0 = 0;
-    } else {
-      tile = rest / sq.chunks;
-      c0 = rest - tile * sq.chunks;
-    }
+    tile = whole ? rest : __builtin_amdgcn_readfirstlane(Div(sq.chunks)(rest));
+    c0 = whole ? 0 : rest - tile * sq.chunks;
   };
   // the tile after this one (there is one)
   auto next_tile = [&]() {
@@ -221,7 +284,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(
   };
   // Run w begins at unit floor(w C / W), moved onto a tile's end where that is within kSnap chunks
   // (in the same way by both its neighbours).
-  auto begin_of = [&](int v) { return v * share + int(int64_t(v) * extra / W); };
+  auto begin_of = [&](int v) {
+    return __builtin_amdgcn_readfirstlane(v * share + by_w(v * extra));
+  };
   int end = C;
   if (w + 1 < W) {
     end = begin_of(w + 1);
@@ -248,37 +313,32 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(
   auto kswz = [](int row) { return row & (CPR - 1); };
   auto vswz = [](int row) { return D >= 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); };
   const int bmask = (1 << log2_bs) - 1;
+  const uint32_t slot_bytes = uint32_t(kvs_slot) * 2, blk_bytes = slot_bytes << log2_bs;
   uint32_t koff[LPW], voff[LPW];
 #pragma unroll
   for (int j = 0; j < LPW; ++j) {
     const int rw = j * RPI + lane / CPR, row = RPW * wave + rw, sl = lane % CPR;
-    koff[j] = uint32_t(rw * kvs_slot * 2 + 16 * (sl ^ kswz(row)));
-    voff[j] = uint32_t(rw * kvs_slot * 2 + 16 * (sl ^ vswz(row)));
+    koff[j] = uint32_t(rw) * slot_bytes + 16 * (sl ^ kswz(row));
+    voff[j] = uint32_t(rw) * slot_bytes + 16 * (sl ^ vswz(row));
   }
   const uint32_t lds_base = uint32_t(reinterpret_cast<uintptr_t>((lds_void_t*)&lds[0][0][0]));
-  int32_t d_b = 0, d_kvh = 0, d_tile = 0, d_np = 0;
+  int32_t d_np = 0, d_q0 = 0, d_rows = 0, d_kvh = 0, d_tile = 0;
   bool any_bad = false;
   for (bool again = false; left > 0; again = true) {
     const int nch = sq.chunks, c1 = whole ? nch : min(nch, c0 + left);
     const int kbeg = c0 * kChunk, kfin = min(c1 * kChunk, sq.ctx), tree0 = sq.ctx - sq.n;
-    const int r0 = tile * TR;
+    const int r0 = tile * TR + 32 * wave;   // this wave's first row
     const int64_t bt_row = int64_t(b) * bt_stride;
-    auto load_blk = [&](int t0) {
-      return bt[bt_row + (min(t0 + RPW * wave, kfin - 1) >> log2_bs)];
-    };
-    int32_t blk = load_blk(kbeg);
-    const int32_t blk_second = load_blk(kbeg + kChunk);
-    const int r = r0 + 32 * wave + col;
+    const bool wave_has_rows = r0 < sq.rows;
+    const int r = r0 + col;
     const bool row_ok = r < sq.rows;
-    const bool wave_has_rows = r0 + 32 * wave < sq.rows;
-    const int qi = row_ok ? r / G : 0;
-    const int h = kvh * G + (row_ok ? r - qi * G : 0);
-    const uint32_t* const mrow = mask + int64_t(sq.q0 + qi) * words;
+    const int qi = row_ok ? r / G : 0, tok = sq.q0 + qi;
+    const int head = kvh * G + (row_ok ? r - qi * G : 0);
     dsp_u32x4 qop[NKS];
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks)
-      qop[ks] = row_ok ? *reinterpret_cast<const dsp_u32x4*>(q + int64_t(sq.q0 + qi) * qst +
-                                                             int64_t(h) * qsh + 16 * ks + 8 * hl)
+      qop[ks] = row_ok ? *reinterpret_cast<const dsp_u32x4*>(q + int64_t(tok) * qst +
+                                                             int64_t(head) * qsh + 16 * ks + 8 * hl)
                        : dsp_u32x4{0u, 0u, 0u, 0u};
     float m = -INFINITY, lpart = 0.f;
     f32x16 acc[NDT];
@@ -286,210 +346,347 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[dt][j] = 0.f;
-    const int64_t head_off = int64_t(kvh) * kvs_head;
-    bool bad_rows = false;  // the rows this wave loaded last are those of a bad block id (uniform)
-    // K and V of the chunk at t0 into buffer buf: this wave's RPW rows, those past kfin as the last
-    // key's (a stale row may hold anything), of a bad block slots 0 ..
-    auto issue = [&](int buf, int t0, int32_t blk_v) {
-      const int32_t id = __builtin_amdgcn_readfirstlane(blk_v);
-      const int from = min(t0 + RPW * wave, kfin - 1);
-      int64_t slot0 = int64_t(id) * (bmask + 1) + (from & bmask);
-      bad_rows = id < 0 || (int64_t(id) + 1) * (bmask + 1) > num_slots;
-      if (bad_rows) {
-        slot0 = 0;
-        any_bad |= t0 + RPW * wave < kfin;
-      }
-      const int64_t e = slot0 * kvs_slot + head_off;
-      const char* kb = reinterpret_cast<const char*>(kc + e);
-      const char* vb = reinterpret_cast<const char*>(vc + e);
-      const uint32_t m0 = lds_base + uint32_t(buf * 2 * SLAB + wave * LPW * 1024);
-      if (t0 + kChunk > kfin) {
+    int blk0 = 0;                   // the first block id in s_blk
+    // the block ids from the one that holds key t0 on, as many as fit; every wave is done with the
+    // buffers and the ids
+    auto stage_ids = [&](int t0) {
+      blk0 = t0 >> log2_bs;
+      const int n = min(kBlocks, ((kfin - 1) >> log2_bs) - blk0 + 1);
+      for (int i = threadIdx.x; i < n; i += 64 * NW) s_blk[i] = bt[bt_row + blk0 + i];
+      __syncthreads();
+    };
+    // This wave's RPW rows of a chunk lie in one block.  A chunk's K is sent for one stage ahead of its
+    // V: the rows' offset is kept in between, the next chunk's id read from LDS a stage ahead.  (All
+    // uniform.)
+    const char* const kbase = reinterpret_cast<const char*>(kc + int64_t(kvh) * kvs_head);
+    const char* const vbase = reinterpret_cast<const char*>(vc + int64_t(kvh) * kvs_head);
+    uint64_t rows_off = 0;          // of the chunk whose K was sent for last; its id is bad
+    bool rows_bad = false;
+    uint32_t bad_k = 0, bad_v = 0;  // buffers whose rows of this wave have a bad block id
+    int32_t id_next = 0;
+    auto first_key = [&](int c) { return min(kbeg + c * kChunk + RPW * wave, kfin - 1); };
+    auto read_id = [&](int c) { id_next = s_blk[(first_key(c) >> log2_bs) - blk0]; };
+    // rows from `off` into a slab; those past kfin as the last key's (a stale row may hold anything)
+    auto fetch = [&](const char* rows, int c, uint32_t m0, bool is_v) {
+      if (kbeg + (c + 1) * kChunk > kfin) {
+        const int room = kfin - 1 - first_key(c);
 #pragma unroll
         for (int j = 0; j < LPW; ++j) {
           const int rw = j * RPI + lane / CPR, row = RPW * wave + rw, sl = lane % CPR;
-          const uint32_t ro = uint32_t(min(rw, kfin - 1 - from) * kvs_slot * 2);
-          dma16<false>(kb, ro + 16 * (sl ^ kswz(row)), m0 + j * 1024);
-          dma16<false>(vb, ro + 16 * (sl ^ vswz(row)), m0 + SLAB + j * 1024);
+          dma16<false>(rows, uint32_t(min(rw, room)) * slot_bytes +
+                                 16 * (sl ^ (is_v ? vswz(row) : kswz(row))), m0 + j * 1024);
         }
         return;
       }
 #pragma unroll
-      for (int j = 0; j < LPW; ++j) {
-        dma16<false>(kb, koff[j], m0 + j * 1024);
-        dma16<false>(vb, voff[j], m0 + SLAB + j * 1024);
-      }
+      for (int j = 0; j < LPW; ++j) dma16<false>(rows, is_v ? voff[j] : koff[j], m0 + j * 1024);
     };
-    if (again) __syncthreads();  // every wave is done with the previous piece's buffers
-    issue(0, kbeg, blk);
-    blk = blk_second;
+    auto slab_of = [&](int buf, int plane) {
+      return lds_base + uint32_t((2 * buf + plane) * SLAB + wave * LPW * 1024);
+    };
+    auto send_k = [&](int c, int buf) {
+      const uint32_t id = __builtin_amdgcn_readfirstlane(id_next);
+      rows_bad = id >= num_blocks;   // (its rows: slots 0 ..)
+      rows_off = rows_bad ? 0 : uint64_t(id) * blk_bytes +
+                                    uint32_t(first_key(c) & bmask) * uint64_t(slot_bytes);
+      any_bad |= rows_bad && kbeg + c * kChunk + RPW * wave < kfin;
+      bad_k = (bad_k & ~(1u << buf)) | uint32_t(rows_bad) << buf;
+      fetch(kbase + rows_off, c, slab_of(buf, 0), false);
+      read_id(c + 1);
+    };
+    auto send_stage = [&](int c) {
+      const int buf = c & (NB - 1);
+      bad_v = (bad_v & ~(1u << buf)) | uint32_t(rows_bad) << buf;
+      fetch(vbase + rows_off, c, slab_of(buf, 1), true);
+      send_k(c + 1, buf);
+    };
+    if (again) __syncthreads();  // every wave is done with the previous piece's buffers and ids
+    stage_ids(kbeg);
+    // the wait for the ids was one for the q rows too (issued before them): none is left to the
+    // loop, whose loads the compiler cannot count
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) asm volatile("" : "+v"(qop[ks]));
     const int nc = c1 - c0;
-    for (int c = 0; c < nc; ++c) {
-      const int t0 = kbeg + c * kChunk, buf = c & 1;
-      // this wave's DMAs of chunk c (and the block ids of chunk c + 1) are in; after the barrier
-      // every wave's are, and every wave is done with chunk c - 1, whose buffer the next overwrites
+    // stages whose ids are held: for those past them the ids are staged once the loads are done
+    const int fit = int(min(int64_t(nc) + 1, (int64_t(kBlocks - 1) << log2_bs) / kChunk));
+    int held = fit > nc ? nc : fit - 1;
+    int sent = 0;           // stages sent for
+    read_id(0);
+    send_k(0, NB - 1);
+    for (; sent < min(held, NB - 1); ++sent) send_stage(sent);
+    __builtin_amdgcn_sched_barrier(0);
+    wait_chunks<NB - 1, 2 * LPW>(sent);
+    s_flag[NB - 1][wave] = int(((bad_k >> (NB - 1)) & 1u) << 2 * wave);
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int kBadK = 0x5555, kOddV = 0xaaaa;
+    auto flags_of = [&](int buf) {
+      int f = 0;
+#pragma unroll
+      for (int x = 0; x < NW; x += 4) {
+        const dsp_u32x4 four = *reinterpret_cast<const dsp_u32x4*>(&s_flag[buf][x]);
+        f |= int(four[0] | four[1] | four[2] | four[3]);
+      }
+      return f;
+    };
+    // Stage c is in LDS, for every wave: its loads are waited for, its flags (of every wave's rows)
+    // returned; the stage NB - 1 further on is sent for into the buffer of stage c - 1, which every
+    // wave is done with.
+    auto arrive = [&](int c) -> int {
+      const int buf = c & (NB - 1);
+      if (c == sent) {  // (a piece longer than the ids held)
+        __syncthreads();
+        stage_ids(kbeg + c * kChunk);
+        held = nc - c < fit ? nc : c + fit - 1;
+        read_id(c + 1);
+        for (; sent < min(held, c + NB - 1); ++sent) send_stage(sent);
+      }
       __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt(dsp_waitcnt_vm<0>());
+      wait_chunks<NB - 2, 2 * LPW>(sent - c - 1);
       char* const my_v = &lds[buf][1][wave * LPW * 1024];  // the V rows this wave loaded
-      const bool edge = t0 + kChunk > tree0;               // (uniform) some row may not see all of it
-      if (bad_rows) zero_rows<CPR, LPW>(my_v, 0);
-      int flag = bad_rows ? 1 : 0;
-      if (edge) {
+      int flag = (bad_k >> buf) & 1u;
+      if ((bad_v >> buf) & 1u) zero_rows<CPR, LPW>(my_v, 0);
+      if (kbeg + (c + 1) * kChunk > tree0) {
         __builtin_amdgcn_sched_barrier(0);
         flag |= any_nonfinite<Tag, LPW>(my_v) ? 2 : 0;
       }
-      s_flag[buf][wave] = flag;
+      s_flag[buf][wave] = flag << 2 * wave;
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
-      int flags = 0;
+      const int flags = flags_of(buf);
+      if (sent < min(held, c + NB)) send_stage(sent++);
+      return flags;
+    };
+    // ---- operands from LDS.  K: row 32*x + col of buffer buf, 16-byte piece 2*ks + hl, which lies at
+    // piece (2*ks + hl) ^ kswz(row): the bits that ks sets are XORed into the address.  V^T: as in
+    // load_vt, the bits of dt XORed likewise; 16-key steps and halves of them by whole rows.
+    typedef __attribute__((address_space(3))) const dsp_u32x4 lds_u32x4_t;
+    const uint32_t k_lane = lds_base + uint32_t(col * ROWB + 16 * (hl ^ kswz(col)));
+    const uint32_t v_lane = lds_base + uint32_t(
+        SLAB + (4 * hl + ((lane & 15) >> 2)) * ROWB +
+        16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vswz((lane & 15) >> 2)) + 8 * (lane & 1));
+    auto read_k = [&](uint32_t at, int x, int ks) {
+      return *reinterpret_cast<lds_u32x4_t*>(((k_lane + at) ^ uint32_t(32 * ks)) +
+                                             uint32_t(32 * x * ROWB));
+    };
+    auto read_v = [&](uint32_t at, int x, int ps, int dt) {
+      v4i16 vh[2];
 #pragma unroll
-      for (int x = 0; x < NW; ++x) flags |= s_flag[buf][x];
-      flags = __builtin_amdgcn_readfirstlane(flags);
-      const bool odd = (flags & 2) != 0;
-      auto clear_odd = [&] {
-        __syncthreads();  // every wave has taken the chunk's infinities and NaN
-        clear_nonfinite<Tag, LPW>(my_v);
-        __syncthreads();
-      };
-      if (c + 1 < nc) {
-        issue(buf ^ 1, t0 + kChunk, blk);
-        if (c + 2 < nc) blk = load_blk(t0 + 2 * kChunk);
-      }
-      if (!wave_has_rows) {  // it only loads
-        if (odd) clear_odd();
-        continue;
-      }
-      const char* ks_lds = &lds[buf][0][0];
-      const char* vs_lds = &lds[buf][1][0];
-      // ---- scores S^T (keys x rows): two 32-key halves.  sc[mt][j] is key 32*mt + 8*(j/4) + 4*hl
-      // + j%4 of this lane's row.
-      f32x16 sc[2];
+      for (int inst = 0; inst < 2; ++inst)
+        vh[inst] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(
+            ((v_lane + at) ^ uint32_t(64 * dt)) + uint32_t((32 * x + 16 * ps + 8 * inst) * ROWB)));
+      return __builtin_bit_cast(dsp_u32x4, vh);
+    };
+    static_assert(D >= 64, "row strides of 128 bytes or more: the XORed bits lie inside a row");
+    // Scores S^T (keys x rows) of half x of the chunk in buffer buf: sc[j] is key 32*x + 8*(j/4) +
+    // 4*hl + j%4 of row col.
+    auto scores = [&](int buf, int x, f32x16& sc) {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
+      for (int j = 0; j < 16; ++j) sc[j] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sc[mt][j] = 0.f;
-        const int krow = 32 * mt + col;
+      for (int ks = 0; ks < NKS; ++ks)
+        sc = mfma32x32<Tag>(read_k(buf * 2 * SLAB, x, ks), qop[ks], sc);
+    };
+    // O^T += V^T . P^T over half x of the chunk in buffer buf.
+    auto add_pv = [&](int buf, int x, const dsp_u32x4 (&pop)[2]) {
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
-          const dsp_u32x4 kop = *reinterpret_cast<const dsp_u32x4*>(
-              ks_lds + krow * ROWB + 16 * ((2 * ks + hl) ^ kswz(krow)));
-          sc[mt] = mfma32x32<Tag>(kop, qop[ks], sc[mt]);
-        }
-      }
-      // ---- which keys the row sees, in the chunks that hold nodes (bit i: key t0 + 32 mt + 4 hl + i)
-      uint32_t seen[2] = {~0u, ~0u};
-      if (edge) {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          seen[mt] = dsp_tree_window(mrow, words, sq.n, t0 + 32 * mt - tree0) >> (4 * hl);
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            sc[mt][j] = (seen[mt] >> (8 * (j >> 2) + (j & 3))) & 1u ? sc[mt][j] : -INFINITY;
-        }
-      }
-      if (flags & 1) {
-        // sc[mt][j] lies in the chunk's 16-key group 2*mt + j/8
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          if (__builtin_amdgcn_readfirstlane(s_flag[buf][g * (NW / 4)]) & 1) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sc[g >> 1][8 * (g & 1) + j] = -INFINITY;
-          }
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[mt][j]);
-      mx = fmaxf(mx, dsp_shfl_xor(mx, 32)) * scale_log2;  // base 2; -inf stays -inf
-      // the maximum moves when some row's exceeds it by 8 (p <= 2^8): the sum and the accumulators
-      // share it, so the result is the same
-      if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
-        const float m_new = fmaxf(m, mx);
-        const float alpha = m_new == -INFINITY ? 1.f : dsp_exp2(m - m_new);
-        m = m_new;
-        lpart *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
-      }
-      const float neg_m = m == -INFINITY ? 0.f : -m;
-      // P^T operands of the four 16-key steps: step ps = 2*mt + half takes registers j = 8*half ..
-      // 8*half + 7, i.e. keys 16*ps + 4*hl + {0..3, 8..11}
-      dsp_u32x4 pop[4];
-#pragma unroll
-      for (int ps = 0; ps < 4; ++ps) {
-        float p8[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p8[i] = dsp_exp2(fmaf(sc[ps >> 1][8 * (ps & 1) + i], scale_log2, neg_m));
-          lpart += p8[i];
-        }
-        pop[ps] = dsp_u32x4{pack2(narrow<Tag>(p8[0]), narrow<Tag>(p8[1])),
-                            pack2(narrow<Tag>(p8[2]), narrow<Tag>(p8[3])),
-                            pack2(narrow<Tag>(p8[4]), narrow<Tag>(p8[5])),
-                            pack2(narrow<Tag>(p8[6]), narrow<Tag>(p8[7]))};
-      }
-      // (rare) infinities and NaN of V to the rows that see them
-      if (odd) {
-#pragma unroll 1
-        for (int ps = 0; ps < 4; ++ps) {
-          const uint32_t bits = (ps < 2 ? seen[0] : seen[1]) >> (16 * (ps & 1));
-          dsp_u32x4 huge;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t two = bits >> (8 * (i >> 1) + 2 * (i & 1));
-            huge[i] = (two & 1u ? kHuge : 0u) | (two & 2u ? kHuge << 16 : 0u);
-          }
-#pragma unroll
-          for (int dt = 0; dt < NDT; ++dt) {
-            __builtin_amdgcn_sched_barrier(0);  // one tile's operands at a time: registers
-            const dsp_u32x4 v = load_vt<D>(vs_lds, ps, dt);
-            acc[dt] = mfma32x32<Bf16Tag>(odd_operand<Tag>(v, false), huge, acc[dt]);
-            acc[dt] = mfma32x32<Bf16Tag>(odd_operand<Tag>(v, true), huge, acc[dt]);
-          }
-        }
-        clear_odd();
-      }
-      // ---- O^T += V^T . P^T
-#pragma unroll
-      for (int ps = 0; ps < 4; ++ps)
+      for (int ps = 0; ps < 2; ++ps)
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
-          v4i16 vh[2];
-#pragma unroll
-          for (int inst = 0; inst < 2; ++inst) {  // (load_vt written out: paged_prefill.hip)
-            const int kr = 16 * ps + 8 * inst + 4 * hl + ((lane & 15) >> 2);
-            const int dim0 = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            vh[inst] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(
-                vs_lds + kr * ROWB + 16 * ((dim0 >> 3) ^ vswz(kr)) + 2 * (dim0 & 7)));
-          }
-          acc[dt] = mfma32x32<Tag>(__builtin_bit_cast(dsp_u32x4, vh), pop[ps], acc[dt]);
+          __builtin_amdgcn_sched_barrier(0);  // (registers)
+          acc[dt] = mfma32x32<Tag>(read_v(buf * 2 * SLAB, x, ps, dt), pop[ps], acc[dt]);
         }
+    };
+    // Which keys of half x of chunk c the row sees, in a chunk that holds nodes (bit i: key 32*x +
+    // 4*hl + i of it).
+    auto window = [&](int c, int x) {
+      return dsp_tree_window(mask + int64_t(tok) * words, words, sq.n,
+                             kbeg + c * kChunk + 32 * x - tree0) >> (4 * hl);
+    };
+    // Half x of chunk c: keys that count for nothing (kflags: the flags that came with its K), and
+    // whether a row's maximum exceeds the running one by more than 2^8; mx: the half's, base 2.
+    float mx = 0.f;
+    auto settle = [&](int c, int x, int kflags, f32x16& sc) -> bool {
+      if (kbeg + (c + 1) * kChunk > tree0) {
+        const uint32_t seen = window(c, x);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          sc[j] = (seen >> (8 * (j >> 2) + (j & 3))) & 1u ? sc[j] : -INFINITY;
+      }
+      if (const uint32_t bad = __builtin_amdgcn_readfirstlane(kflags) & kBadK; bad != 0) {
+        // sc[j] lies in the chunk's 16-key group 2*x + j/8, whose id the wave that loaded it found
+        // bad
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if ((bad >> (2 * (((2 * x + g) * NW) / 4))) & 1u) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sc[8 * g + j] = -INFINITY;
+          }
+      }
+      mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[j]);
+      mx = fmaxf(mx, dsp_shfl_xor(mx, 32)) * scale_log2;  // -inf stays -inf
+      return __builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0;
+    };
+    // The running maximum moves only then (p <= 2^8 otherwise): the sum and the accumulators share
+    // it, so the result is the same.
+    auto rescale = [&]() -> float {
+      const float m_new = fmaxf(m, mx);
+      const float alpha = m_new == -INFINITY ? 1.f : dsp_exp2(m - m_new);
+      m = m_new;
+      lpart *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
+      return alpha;
+    };
+    // One probability of a half, and the operands they make (P^T of two 16-key steps: step ps takes
+    // registers j = 8*ps .. 8*ps + 7, i.e. keys 16*ps + 4*hl + {0..3, 8..11}).
+    auto prob = [&](const f32x16& sc, int j, float neg_m) {
+      const float p = dsp_exp2(fmaf(sc[j], scale_log2, neg_m));
+      lpart += p;
+      return p;
+    };
+    auto probs = [&](const f32x16& sc, dsp_u32x4 (&pop)[2]) {
+      const float neg_m = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        const float p0 = prob(sc, j, neg_m), p1 = prob(sc, j + 1, neg_m);
+        pop[j >> 3][(j >> 1) & 3] = narrow2<Tag>(p0, p1);
+      }
+    };
+    // (rare) infinities and NaN of V of chunk c, in buffer buf, to the rows that see them; then they
+    // are cleared
+    auto take_odd = [&](int c, int buf) {
+      if (wave_has_rows)
+#pragma unroll 1
+        for (int y = 0; y < 4; ++y) {
+          const int x = y >> 1, ps = y & 1;
+          const uint32_t seen = window(c, x);
+          {
+            dsp_u32x4 huge;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t two = seen >> (16 * ps + 8 * (i >> 1) + 2 * (i & 1));
+              huge[i] = (two & 1u ? kHuge : 0u) | (two & 2u ? kHuge << 16 : 0u);
+            }
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+              __builtin_amdgcn_sched_barrier(0);  // one tile's operands at a time: registers
+              const dsp_u32x4 v = read_v(buf * 2 * SLAB, x, ps, dt);
+              acc[dt] = mfma32x32<Bf16Tag>(odd_operand<Tag>(v, false), huge, acc[dt]);
+              acc[dt] = mfma32x32<Bf16Tag>(odd_operand<Tag>(v, true), huge, acc[dt]);
+            }
+          }
+        }
+      __syncthreads();  // every wave has taken them
+      clear_nonfinite<Tag, LPW>(&lds[buf][1][wave * LPW * 1024]);
+      __syncthreads();
+    };
+    constexpr int kFirst = NB - 1;  // the buffer of K of chunk 0
+    constexpr int kAhead = NDT < 3 ? NDT : 3;  // operands read ahead of their MFMAs
+    // A half's exponentials, 1 / NKS of them at a time (step i).
+    static_assert(NKS <= 16 && NKS == 2 * NDT, "a step has one exponential or more");
+    auto take_probs = [&](f32x16& sc, int i, float neg_m, dsp_u32x4 (&pop)[2]) {
+      constexpr int PER = 16 / NKS;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int j = PER * i + e;
+        sc[j] = prob(sc, j, neg_m);
+        if (j & 1) pop[j >> 3][(j >> 1) & 3] = narrow2<Tag>(sc[j - 1], sc[j]);
+      }
+    };
+    int kflags = flags_of(kFirst);  // (in a vector register until it is looked at)
+    // Half by half, a pipeline in which the MFMAs of one half's scores and of another's P V have
+    // the exponentials of a third beside them, instruction by instruction (a wave issues in order:
+    // MFMAs in a row, each after the wait for its operands, left the chip 67 % idle).  half(x): the
+    // probabilities of cur; of half x of a stage, next = the scores and acc += P V with the
+    // probabilities before (pop).
+    f32x16 s0, s1;
+    dsp_u32x4 pop[2];
+    auto half = [&](auto xc, int c, int cx, int buf, int kfl, f32x16& cur, f32x16& next) {
+      constexpr int x = decltype(xc)::value;
+      const uint32_t at = uint32_t(buf * 2 * SLAB);
+      dsp_u32x4 kop[NKS], vop[2 * NDT];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        kop[i] = read_k(at, x, i);
+        vop[i] = read_v(at, x, i / NDT, i % NDT);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (settle(c, cx, kfl, cur)) {
+        // the probabilities that still wait for their P V move along, rounded once more
+        const float alpha = rescale();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t two = pop[i >> 2][i & 3];
+          pop[i >> 2][i & 3] = narrow2<Tag>(low<Tag>(two) * alpha, high<Tag>(two) * alpha);
+        }
+      }
+      const float neg_m = m == -INFINITY ? 0.f : -m;
+      dsp_u32x4 fresh[2];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) next[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NKS; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + kAhead < NKS) {
+          kop[i + kAhead] = read_k(at, x, i + kAhead);
+          vop[i + kAhead] = read_v(at, x, (i + kAhead) / NDT, (i + kAhead) % NDT);
+        }
+        next = mfma32x32<Tag>(kop[i], qop[i], next);
+        take_probs(cur, i, neg_m, fresh);
+        __builtin_amdgcn_sched_barrier(0);
+        acc[i % NDT] = mfma32x32<Tag>(vop[i], pop[i / NDT], acc[i % NDT]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      pop[0] = fresh[0];
+      pop[1] = fresh[1];
+    };
+    if (wave_has_rows) {
+      scores(kFirst, 0, s0);
+      if (settle(0, 0, kflags, s0)) rescale();
+      probs(s0, pop);
+      scores(kFirst, 1, s1);
     }
+    for (int c = 0; c < nc; ++c) {
+      const int buf = c & (NB - 1);
+      const int flags = arrive(c);
+      if (kbeg + (c + 1) * kChunk > tree0 && (__builtin_amdgcn_readfirstlane(flags) & kOddV))
+        take_odd(c, buf);
+      if (wave_has_rows) {
+        half(std::integral_constant<int, 0>{}, c, 1, buf, kflags, s1, s0);
+        if (c + 1 < nc) half(std::integral_constant<int, 1>{}, c + 1, 0, buf, flags, s0, s1);
+      }
+      kflags = flags;
+    }
+    if (wave_has_rows) add_pv((nc - 1) & (NB - 1), 1, pop);
     // ---- the piece's rows: acc[dt][j] = O[row col][dim 32*dt + 8*(j/4) + 4*hl + j%4]
     lpart += dsp_shfl_xor(lpart, 32);
-    if (c0 == 0 && c1 == nch) {
-      const float inv = lpart == 0.f ? 0.f : 1.f / lpart;  // (0: the row sees no key; NaN stays)
-      if (row_ok) {
-        uint16_t* o = out + int64_t(sq.q0 + qi) * ost + int64_t(h) * osh;
+    const bool complete = c0 == 0 && c1 == nch;
+    if (row_ok) {
+      if (complete) {
+        const float inv = lpart == 0.f ? 0.f : 1.f / lpart;  // (0: the row sees no key; NaN stays)
+        uint16_t* o = out + int64_t(tok) * ost + int64_t(head) * osh;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
           for (int j4 = 0; j4 < 4; ++j4) {
-            uint16_t x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = narrow<Tag>(acc[dt][4 * j4 + j] * inv);
+            const f32x16& a = acc[dt];
+            const uint32_t lo = narrow2<Tag>(a[4 * j4] * inv, a[4 * j4 + 1] * inv);
+            const uint32_t hi = narrow2<Tag>(a[4 * j4 + 2] * inv, a[4 * j4 + 3] * inv);
             uint16_t* const at = o + 32 * dt + 8 * j4 + 4 * hl;
             if (vec_out) {
-              *reinterpret_cast<dsp_u32x2*>(at) = dsp_u32x2{pack2(x[0], x[1]), pack2(x[2], x[3])};
+              *reinterpret_cast<dsp_u32x2*>(at) = dsp_u32x2{lo, hi};
             } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) at[j] = x[j];
+              at[0] = uint16_t(lo);
+              at[1] = uint16_t(lo >> 16);
+              at[2] = uint16_t(hi);
+              at[3] = uint16_t(hi >> 16);
             }
           }
-      }
-    } else {
-      const int64_t wrow = int64_t(2 * w + (c0 == 0 ? 1 : 0)) * TR + 32 * wave + col;
-      if (row_ok) {
+      } else {
+        const int64_t wrow = int64_t(2 * w + (c0 == 0 ? 1 : 0)) * TR + 32 * wave + col;
         float* dst = ws_acc + wrow * D;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
@@ -503,117 +700,194 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(
           ws_ml[2 * wrow + 1] = lpart;
         }
       }
-      if (c0 == 0) {  // this run began the tile: its merge is described here
-        const int tile_end = base + (kvh * sq.tiles + tile + 1) * nch;
-        d_b = b;
+    }
+    if (c0 == 0 && !whole) {
+      // this run began the tile: its merge is described here.  Pieces: up to the last run that
+      // begins before the tile's end (those within kSnap moved onto it).
+      int np = 0;
+      if (!complete) {
+        const int upto = base + (kvh * sq.tiles + tile + 1) * nch - kSnap;
+        int v = min(W - 1, int(float(upto) * float(W) / float(C)));
+        while (begin_of(v) >= upto) --v;
+        while (v + 1 < W && begin_of(v + 1) < upto) ++v;
+        np = v - w + 1;
+        d_np = np;
+        d_q0 = sq.q0;
+        d_rows = sq.rows;
         d_kvh = kvh;
         d_tile = tile;
-        // up to the last run that begins before the tile's end (those within kSnap moved onto it)
-        d_np = int32_t((int64_t(tile_end - kSnap) * W - 1) / C) - w + 1;
+      }
+      if (tiles_max > 0 && threadIdx.x == 0) {
+        int32_t* d = ws_desc + kDesc * ((int64_t(b) * KVH + kvh) * tiles_max + tile);
+        d[0] = np;
+        d[1] = w;
       }
     }
     left -= whole ? 1 : c1 - c0;
     if (left > 0) next_tile();
   }
   if (err_count && any_bad && lane == 0) atomicAdd(err_count, 1);  // once per wave
-  if (!whole && threadIdx.x == 0) {
-    int32_t* d = ws_desc + 4 * w;
-    d[0] = d_b;
-    d[1] = d_kvh;
-    d[2] = d_tile;
-    d[3] = d_np;
+  if (!whole && tiles_max == 0 && threadIdx.x == 0) {
+    int32_t* d = ws_desc + kDesc * w;
+    d[0] = d_np;
+    d[1] = d_q0;
+    d[2] = d_rows;
+    d[3] = d_kvh;
+    d[4] = d_tile;
   }
 }
 
-// Grid (workgroups of the first launch, row groups): R rows of the tile that run x began and did
-// not finish, one thread per (row, 4 dims); its pieces are loaded 16 at a time before they are
-// folded.
-constexpr int tree_merge_rows(int D) { return 1024 / D; }
+// The merge of the tiles that runs cut.  One workgroup per (item, R rows); an item is a tile of the
+// batch (tiles_max > 0: of the grid of tiles_max for each sequence and KV head) or, where there
+// are fewer runs than tiles, the tile that a run began.  One thread per (row, 4 dims, every kSplit-th
+// piece), its pieces loaded 8 at a time; the kSplit threads' results meet in LDS.  Neighbours in
+// the grid are the row groups of one item; the runs that begin a tile often lie a multiple of 8
+// apart, so the groups of every next 8 items start one XCD further (all of one XCD's: 47 us instead
+// of 15 at 32 tiles of 256 rows in 8 pieces).
+constexpr int tree_merge_rows(int D, int split) { return 1024 / D / split; }
 
-template <typename Tag, int D>
+template <typename Tag, int D, int kSplit>
 __global__ __launch_bounds__(256) void tree_merge_kernel(
     const float* __restrict__ ws_acc, const float* __restrict__ ws_ml,
-    const int32_t* __restrict__ ws_desc, const int32_t* __restrict__ cu_q, int32_t G,
-    int32_t max_q_len, int32_t tile_rows, uint16_t* __restrict__ out, int64_t ost, int64_t osh) {
-  constexpr int TPR = D / 4, R = tree_merge_rows(D), kBatch = 16;
-  const int64_t w = blockIdx.x;
-  const int32_t* desc = ws_desc + 4 * w;
-  const int b = desc[0], kvh = desc[1], tile = desc[2], np = desc[3];
-  if (np <= 0) return;
-  const int q0 = cu_q[b], rows = min(cu_q[b + 1] - q0, max_q_len) * G;
-  const int lr = blockIdx.y * R + threadIdx.x / TPR, d = 4 * (threadIdx.x % TPR);
+    const int32_t* __restrict__ ws_desc, const int32_t* __restrict__ cu_q,
+    const int32_t* __restrict__ ctx_lens, int32_t items, int32_t groups, int32_t KVH, int32_t G,
+    int32_t max_q_len, int32_t max_ctx, int32_t tiles_max, int32_t tile_rows,
+    uint16_t* __restrict__ out, int64_t ost, int64_t osh) {
+  constexpr int TPR = D / 4, R = tree_merge_rows(D, kSplit), kBatch = 8;
+  __shared__ float s_acc[kSplit][R][D];
+  __shared__ float s_ml[kSplit][R][2];
+  const Div by_groups(groups);
+  const int turn = blockIdx.x / 8;
+  const int idx = 8 * turn + ((int(blockIdx.x % 8) - by_groups(turn)) & 7);
+  const int item = by_groups(idx), group = idx - item * groups;
+  if (item >= items) return;
+  const int32_t* desc = ws_desc + int64_t(kDesc) * item;
+  int np = desc[0], q0, rows, kvh, tile;
+  int64_t w;
+  if (tiles_max > 0) {
+    const Div by_tiles(tiles_max), by_heads(KVH);
+    const int head = by_tiles(item), b = by_heads(head);
+    tile = item - head * tiles_max;
+    kvh = head - b * KVH;
+    w = desc[1];
+    q0 = cu_q[b];
+    const int n = cu_q[b + 1] - q0;
+    // (a tile that the sequence does not have has no description)
+    rows = n <= 0 || tree_bad(n, ctx_lens[b], max_ctx) ? 0 : min(n, max_q_len) * G;
+  } else {
+    w = item;
+    q0 = desc[1];
+    rows = desc[2];
+    kvh = desc[3];
+    tile = desc[4];
+    if (np <= 0) return;
+  }
+  const int lr = group * R + threadIdx.x / TPR % R, d = 4 * (threadIdx.x % TPR);
+  const int split = threadIdx.x / (TPR * R);
   const int r = tile * tile_rows + lr;
-  if (lr >= tile_rows || r >= rows) return;
+  if (tile * tile_rows + group * R >= rows || np <= 0) return;  // (uniform)
+  const bool live = lr < tile_rows && r < rows;
   float M = -INFINITY, L = 0.f;
   f32x4 A = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int p0 = 0; p0 < np; p0 += kBatch) {
-    const int n = min(np - p0, kBatch);
-    f32x4 va[kBatch];
-    float vm[kBatch], vl[kBatch];
+  if (live)
+    for (int p0 = split; p0 < np; p0 += kSplit * kBatch) {
+      f32x4 va[kBatch];
+      float vm[kBatch], vl[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      if (i < n) {
-        const int p = p0 + i;
+      for (int i = 0; i < kBatch; ++i) {
+        const int p = min(p0 + kSplit * i, np - 1);  // (past the last: again, for nothing)
         const int64_t row = (p == 0 ? 2 * w + 1 : 2 * (w + p)) * tile_rows + lr;
         va[i] = *reinterpret_cast<const f32x4*>(ws_acc + row * D + d);
         vm[i] = ws_ml[2 * row];
         vl[i] = ws_ml[2 * row + 1];
       }
+      float bm = M;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) bm = fmaxf(bm, vm[i]);
+      const float Mu = bm == -INFINITY ? 0.f : bm;
+      const float keep = dsp_exp2(M - Mu);
+      L *= keep;
+      A *= keep;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float x = p0 + kSplit * i < np ? dsp_exp2(vm[i] - Mu) : 0.f;
+        const bool in = p0 + kSplit * i < np;
+        L = fmaf(in ? vl[i] : 0.f, x, L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) A[e] = fmaf(in ? va[i][e] : 0.f, x, A[e]);
+      }
+      M = bm;
+    }
+  if constexpr (kSplit > 1) {
+    const int at = lr - group * R;
+    *reinterpret_cast<f32x4*>(&s_acc[split][at][d]) = A;
+    if (d == 0) {
+      s_ml[split][at][0] = M;
+      s_ml[split][at][1] = L;
+    }
+    __syncthreads();
+    if (split > 0) return;
     float bm = M;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) bm = i < n ? fmaxf(bm, vm[i]) : bm;
-    const float Mu = bm == -INFINITY ? 0.f : bm;
-    const float keep = dsp_exp2(M - Mu);
+    for (int i = 1; i < kSplit; ++i) bm = fmaxf(bm, s_ml[i][at][0]);
+    const float Mu = bm == -INFINITY ? 0.f : bm, keep = dsp_exp2(M - Mu);
     L *= keep;
     A *= keep;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const float x = i < n ? dsp_exp2(vm[i] - Mu) : 0.f;
-      L = fmaf(i < n ? vl[i] : 0.f, x, L);
+    for (int i = 1; i < kSplit; ++i) {
+      const float x = dsp_exp2(s_ml[i][at][0] - Mu);
+      const f32x4 o = *reinterpret_cast<const f32x4*>(&s_acc[i][at][d]);
+      L = fmaf(s_ml[i][at][1], x, L);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) A[e] = fmaf(i < n ? va[i][e] : 0.f, x, A[e]);
+      for (int e = 0; e < 4; ++e) A[e] = fmaf(o[e], x, A[e]);
     }
-    M = bm;
   }
+  if (!live) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  uint16_t* o = out + int64_t(q0 + r / G) * ost + int64_t(kvh * G + r % G) * osh + d;
+  const int qi = r / G;
+  uint16_t* o = out + int64_t(q0 + qi) * ost + int64_t(kvh * G + r - qi * G) * osh + d;
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] = narrow<Tag>(A[e] * inv);
 }
 
 // ---- which launch a shape takes
 struct TreePlan {
-  bool tile;       // the tile kernel (else generic)
-  bool whole;      // its tiles stay whole: no second launch
-  int waves;       // of a workgroup
-  int workers;     // workgroups
+  bool tile;        // the tile kernel (else generic)
+  bool whole;       // its tiles stay whole: no second launch
+  int rows;         // of a tile
+  int workers;      // workgroups, each with a run of the list
+  int least;        // units that a run has at least
+  int tiles_max;    // tiles of a sequence and KV head, where the merge goes by them (else 0: by runs)
+  int items;        // of the merge
 };
-
-bool tree_tile_shape(int32_t D) { return D == 64 || D == 128 || D == 256; }
-
-int tree_waves(int32_t D, int64_t rows) { return rows > 128 && D <= 128 ? 8 : 4; }
 
 TreePlan tree_plan(int32_t B, int32_t KVH, int32_t G, int32_t D, int32_t max_q_len,
                    int32_t max_ctx) {
   TreePlan p{};
-  if (!tree_tile_shape(D) || B < 1 || max_q_len < 1 || max_ctx < 1) return p;
+  if (!(D == 64 || D == 128 || D == 256) || B < 1 || max_q_len < 1 || max_ctx < 1) return p;
   const int64_t rows = int64_t(max_q_len) * G;
-  p.waves = tree_waves(D, rows);
-  const int64_t tiles = (rows + 32 * p.waves - 1) / (32 * p.waves) * B * KVH;
+  // 256 rows take one workgroup of 8 waves to a CU, 128 rows two of 4 (D 256: one, for the buffers).
+  // 32 sequences of 500 to 4000 tokens, 8 KV heads, D 128, bf16: 128 rows a head 110 us with two of
+  // 4 (124 with one of 8); 192, 256 and 512 rows 160, 175 and 300 us with one of 8 (169, 186 and 311
+  // with two of 4, which load a chunk for 128 rows each).
+  p.rows = D > 128 || rows <= 128 ? 128 : 256;
+  const int64_t per_head = (rows + p.rows - 1) / p.rows, tiles = per_head * B * KVH;
   const int64_t chunks = (int64_t(max_ctx) + kChunk - 1) / kChunk;
-  p.tile = rows < (int64_t(1) << 30) && tiles * chunks < (int64_t(1) << 31) &&
-           max_ctx < (1 << 30);
+  // (the numbers that Div divides)
+  p.tile = max_ctx < (1 << 24) && rows < (1 << 24) && tiles * chunks < (1 << 24) && B < (1 << 16);
+  if (!p.tile) return p;
   p.whole = chunks <= 8;
-  // workgroups that fit the chip at once (LDS and registers)
-  const int per_cu = D > 128 ? 1 : D > 64 ? (p.waves > 4 ? 1 : 2) : (p.waves > 4 ? 2 : 3);
-  const int64_t slots = int64_t(per_cu) * dsp_detail::device_cus();
-  p.workers = int(p.whole ? std::min(tiles, slots)
-                          : std::min((tiles * chunks + kMinChunks - 1) / kMinChunks, slots));
+  p.least = p.whole ? 1 : kMinChunks;
+  // workgroups that fit the chip at once (LDS)
+  const int64_t slots = int64_t(dsp_detail::device_cus()) * (p.rows == 128 && D <= 128 ? 2 : 1);
+  p.workers = int(std::min((p.whole ? tiles : (tiles * chunks + p.least - 1) / p.least), slots));
+  p.tiles_max = tiles <= p.workers ? int(per_head) : 0;
+  p.items = tiles <= p.workers ? int(tiles) : p.workers;
   return p;
 }
 
 size_t tree_tile_bytes(const TreePlan& p, int32_t D) {
-  return p.whole ? 0 : size_t(p.workers) * (size_t(2) * 32 * p.waves * (D + 2) + 4) * sizeof(float);
+  return p.whole ? 0 : size_t(p.workers) * (size_t(2) * p.rows * (D + 2) + kDesc) * sizeof(float);
 }
 
 template <typename Tag, int D>
@@ -624,28 +898,36 @@ int launch_tree(const TreePlan& p, const uint16_t* q, int64_t qst, int64_t qsh, 
                 int32_t KVH, int32_t G, int32_t max_q_len, int32_t max_ctx, float scale_log2,
                 float* ws, uint16_t* out, int64_t ost, int64_t osh, int32_t* err_count,
                 hipStream_t s) {
-  const int tr = 32 * p.waves;
-  float* ws_ml = ws + int64_t(2) * p.workers * tr * D;
-  int32_t* ws_desc = reinterpret_cast<int32_t*>(ws_ml + int64_t(4) * p.workers * tr);
+  float* ws_ml = ws + int64_t(2) * p.workers * p.rows * D;
+  int32_t* ws_desc = reinterpret_cast<int32_t*>(ws_ml + int64_t(4) * p.workers * p.rows);
   const int vec_out = ost % 4 == 0 && osh % 4 == 0 && dsp_aligned(out, 8);
-  auto launch = [&](auto kernel) {
-    kernel<<<p.workers, 64 * p.waves, 0, s>>>(
-        q, qst, qsh, kc, vc, num_slots, kvs_slot, kvs_head, bt, bt_stride, log2_bs, cu_q, ctx_lens,
-        mask, words, B, KVH, G, max_q_len, max_ctx, scale_log2, p.whole, ws, ws_ml, ws_desc, out,
-        ost, osh, vec_out, err_count);
+  auto launch = [&](auto shape) {
+    using S = decltype(shape);
+    tree_tile_kernel<Tag, D, S><<<p.workers, 64 * S::NW, 0, s>>>(
+        q, qst, qsh, kc, vc, uint32_t(num_slots >> log2_bs), int32_t(kvs_slot), kvs_head, bt,
+        bt_stride, log2_bs, cu_q, ctx_lens, mask, words, B, KVH, G, max_q_len, max_ctx, scale_log2,
+        p.whole, p.least, p.tiles_max, ws, ws_ml, ws_desc, out, ost, osh, vec_out, err_count);
   };
   if constexpr (D <= 128) {
-    if (p.waves == 8) launch(tree_tile_kernel<Tag, D, 8>);
-    else launch(tree_tile_kernel<Tag, D, 4>);
+    if (p.rows == 256) launch(Shape<8, 1>{});
+    else launch(Shape<4, 2>{});
   } else {
-    launch(tree_tile_kernel<Tag, D, 4>);
+    launch(Shape<4, 1>{});
   }
   const int st = dsp_launch_status();
   if (st != DSP_OK || p.whole) return st;
-  const int64_t rows = std::min(int64_t(max_q_len) * G, int64_t(tr));
-  const dim3 grid(unsigned(p.workers), unsigned((rows + tree_merge_rows(D) - 1) / tree_merge_rows(D)));
-  tree_merge_kernel<Tag, D><<<grid, 256, 0, s>>>(ws, ws_ml, ws_desc, cu_q, G, max_q_len, tr, out,
-                                                 ost, osh);
+  const int64_t rows = std::min(int64_t(max_q_len) * G, int64_t(p.rows));
+  auto merge = [&](auto split) {
+    constexpr int kSplit = decltype(split)::value;
+    constexpr int R = tree_merge_rows(D, kSplit);
+    const int groups = int((rows + R - 1) / R);
+    tree_merge_kernel<Tag, D, kSplit>
+        <<<unsigned((int64_t(p.items) * groups + 7) / 8 * 8), 256, 0, s>>>(
+            ws, ws_ml, ws_desc, cu_q, ctx_lens, p.items, groups, KVH, G, max_q_len, max_ctx,
+            p.tiles_max, p.rows, out, ost, osh);
+  };
+  if (p.workers > 4 * p.items) merge(std::integral_constant<int, 4>{});
+  else merge(std::integral_constant<int, 1>{});
   return dsp_launch_status();
 }
 
@@ -708,7 +990,9 @@ extern "C" int dsp_paged_tree_attention(
   const uint32_t* mask = reinterpret_cast<const uint32_t*>(tree_mask);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool tile = p.tile && dtype != DSP_F32 && block_size >= 16 && num_slots >= 16 &&
-                    num_slots % block_size == 0 && kv_stride_slot < (int64_t(1) << 25) &&
+                    num_slots % block_size == 0 && num_slots / block_size < (int64_t(1) << 31) &&
+                    kv_stride_slot >= 0 && kv_stride_slot < (int64_t(1) << 25) &&
+                    kv_stride_slot * block_size < (int64_t(1) << 31) &&
                     scale > 0.f && scale < FLT_MAX && q_stride_t % 8 == 0 && q_stride_h % 8 == 0 &&
                     kv_stride_slot % 8 == 0 && kv_stride_head % 8 == 0 && dsp_aligned(q, 16) &&
                     dsp_aligned(k_cache, 16) && dsp_aligned(v_cache, 16);
