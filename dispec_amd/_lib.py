@@ -237,8 +237,9 @@ _SAME = contextlib.nullcontext()
 
 def same_device(t, *others) -> None:
     """ValueError unless the tensors (or None) are on t's device."""
+    index = t.get_device()
     for o in others:
-        if o is not None and o.device != t.device:
+        if o is not None and o.get_device() != index:
             raise ValueError(f"tensors on {t.device} and {o.device}: one call takes one device")
 
 

@@ -30,7 +30,6 @@ constexpr int kThreads = 256;
 constexpr int kSlice = 4096;      // tokens of a row per workgroup
 constexpr int kPerThread = kSlice / kThreads;
 constexpr int kMaxNodes = 1024;   // nodes of one tree (their tokens and probabilities sit in LDS)
-constexpr int kInfo = 4;          // ints a sequence: its last kept node (-1: none), tokens kept
 
 struct VBf16 { using store = uint16_t; };
 struct VF16 { using store = uint16_t; };
@@ -45,6 +44,13 @@ __device__ __forceinline__ float value(typename Tag::store x) {
   else
     return x;
 }
+
+// What the first launch leaves for the second: the last kept node (-1: no nodes) and its row, the
+// tokens kept before it, and the row of the draft's probabilities after it (-1: none was drafted).
+struct Info {
+  int32_t end, row, len, draft_row;
+};
+static_assert(sizeof(Info) == 16, "one load");
 
 // One sequence's nodes: those of its first max_q_len that lie inside the rows.
 struct Tree {
@@ -112,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
     const typename Tag::store* __restrict__ draft, int64_t ds, int64_t draft_rows,
     const float* __restrict__ u, const int32_t* __restrict__ cu_q, int32_t max_q_len, int64_t V,
     int32_t slices,
-    double* __restrict__ sums, int32_t* __restrict__ info, int32_t* __restrict__ num,
+    double* __restrict__ sums, Info* __restrict__ info, int32_t* __restrict__ num,
     int32_t* __restrict__ path, int64_t* __restrict__ out_tokens,
     int32_t* __restrict__ err_count) {
   __shared__ int32_t s_par[kMaxNodes], s_tok[kMaxNodes], s_path[kMaxNodes];
@@ -203,11 +209,12 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
       // (the token after the path is the second launch's)
       out_tokens[o] = i < len ? int64_t(s_tok[s_path[i + 1]]) : -1;
     }
-    if (tid == 0) {
-      num[b] = max(len, 0);
-      info[kInfo * b] = end;
-      info[kInfo * b + 1] = len;
-    }
+  }
+  // (nothing was drafted after a chain's last node)
+  const bool with_q = kChain && end + 1 < t.n && dr >= 0 && dr + end < draft_rows;
+  if (slice == 0 && tid == 0) {
+    num[b] = max(len, 0);
+    info[b] = Info{end, t.at + end, len, with_q ? int32_t(dr + end) : -1};
   }
   if (len < 0) return;
   const int64_t v0 = int64_t(slice) * kSlice;
@@ -221,8 +228,6 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
     __syncthreads();
   }
   const bool kids = !kChain && s_any != 0;
-  // (nothing was drafted after a chain's last node)
-  const bool with_q = kChain && end + 1 < t.n && dr >= 0 && dr + end < draft_rows;
   const auto* p = target + (int64_t(t.at) + end) * ts + v0;
   const auto* q = with_q ? draft + (dr + end) * ds + v0 : p;
   using V16 = typename Vec<Tag>::type;
@@ -260,64 +265,64 @@ __global__ __launch_bounds__(kThreads) void verify_walk_kernel(
   }
 }
 
-// Inclusive sums over the workgroup's threads, in thread order; the last one is the total.
-__device__ __forceinline__ double block_scan(double v, double* s_wave, double& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Inclusive sums over a wave's lanes, in their order.
+__device__ __forceinline__ double wave_scan(double v) {
+  const int lane = __lane_id();
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const double o = __shfl_up(v, d);
     if (lane >= d) v += o;
   }
-  __syncthreads();
-  if (lane == 63) s_wave[wave] = v;
-  __syncthreads();
-  double before = 0.0;
-  total = 0.0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < wave) before += s_wave[w];
-    total += s_wave[w];
-  }
-  return before + v;
+  return v;
 }
 
+// One workgroup a sequence.  It is a chain of loads, each of which names the next (what the walk
+// left, the slices' sums, the slice's tokens), so the first are sent for together, every wave scans
+// the sums by itself (64 slices at a time: one step for 262144 tokens) and the workgroup meets
+// twice.
 template <typename Tag, bool kChain>
 __global__ __launch_bounds__(kThreads) void verify_pick_kernel(
     const int64_t* __restrict__ tokens, const int32_t* __restrict__ parents,
     const typename Tag::store* __restrict__ target, int64_t ts, int64_t rows,
-    const typename Tag::store* __restrict__ draft, int64_t ds, int64_t draft_rows,
-    const float* __restrict__ u_last, const int32_t* __restrict__ cu_q, int32_t max_q_len,
-    int64_t V, int32_t slices, double* __restrict__ sums, const int32_t* __restrict__ info,
-    int64_t* __restrict__ out_tokens, int32_t* __restrict__ err_count) {
-  __shared__ double s_wave[kThreads / 64];
+    const typename Tag::store* __restrict__ draft, int64_t ds, const float* __restrict__ u_last,
+    const int32_t* __restrict__ cu_q, int32_t max_q_len, int64_t V, int32_t slices,
+    double* __restrict__ sums, const Info* __restrict__ info, int64_t* __restrict__ out_tokens,
+    int32_t* __restrict__ err_count) {
+  constexpr int kWaves = kThreads / 64;
+  __shared__ double s_wave[kWaves];
+  __shared__ int32_t s_first[kWaves], s_last[kWaves];
   __shared__ uint32_t s_kids[kSlice / 32];
-  __shared__ int32_t s_first, s_last;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const int end = info[kInfo * b], len = info[kInfo * b + 1];
-  if (len < 0) return;
-  const Tree t = tree_of(cu_q, b, max_q_len, rows);
-  const int64_t dr = kChain ? first_draft_row(cu_q, b) : 0;
-  const auto* prow = target + (int64_t(t.at) + end) * ts;
-  const bool with_q = kChain && end + 1 < t.n && dr >= 0 && dr + end < draft_rows;
-  const auto* qrow = with_q ? draft + (dr + end) * ds : prow;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   double* mine = sums + int64_t(b) * slices;
+  auto sum_of = [&](int s) { return s < slices ? mine[s] : 0.0; };
+  double v0 = sum_of(lane);   // the first 64 slices' sums
+  const Info seq = info[b];
+  const double u = u_last[b];
+  const Tree t = kChain ? Tree{0, 0} : tree_of(cu_q, b, max_q_len, rows);
+  if (seq.len < 0) return;
+  // the last node's children: this thread's nodes
+  constexpr int kNodes = kMaxNodes / kThreads;
+  int32_t kid[kNodes];
+  if constexpr (!kChain) {
+#pragma unroll
+    for (int i = 0; i < kNodes; ++i) {
+      const int at = tid + i * kThreads;
+      kid[i] = -1;
+      if (at < t.n && parent_of(parents, t.at, at) == seq.end) {
+        const int64_t x = tokens[t.at + at];
+        kid[i] = x >= 0 && x < V ? int32_t(x) : -1;
+      }
+    }
+    for (int i = tid; i < kSlice / 32; i += kThreads) s_kids[i] = 0u;
+  }
+  const bool with_q = kChain && seq.draft_row >= 0;
+  const auto* prow = target + int64_t(seq.row) * ts;
+  const auto* qrow = with_q ? draft + int64_t(seq.draft_row) * ds : prow;
   // this thread's tokens of a slice: kPerThread in a row
   double r[kPerThread];
   auto load = [&](int slice, bool whole) {
-    const int64_t v0 = int64_t(slice) * kSlice;
-    const int nv = int(min(int64_t(kSlice), V - v0));
-    if constexpr (!kChain) {
-      __syncthreads();
-      for (int i = tid; i < kSlice / 32; i += kThreads) s_kids[i] = 0u;
-      __syncthreads();
-      if (!whole)
-        for (int i = tid; i < t.n; i += kThreads)
-          if (parent_of(parents, t.at, i) == end) {
-            const int64_t x = tokens[t.at + i] - v0;
-            if (x >= 0 && x < nv) atomicOr(&s_kids[x >> 5], 1u << (x & 31));
-          }
-      __syncthreads();
-    }
+    const int64_t first = int64_t(slice) * kSlice;
+    const int nv = int(min(int64_t(kSlice), V - first));
     const bool sub = with_q && !whole;
     float pf[kPerThread], qf[kPerThread];
     const int v1 = tid * kPerThread;
@@ -326,9 +331,9 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(
       constexpr int N = Vec<Tag>::N;
 #pragma unroll
       for (int j = 0; j < kPerThread / N; ++j) {
-        const V16 pv = *reinterpret_cast<const V16*>(prow + v0 + v1 + j * N);
+        const V16 pv = *reinterpret_cast<const V16*>(prow + first + v1 + j * N);
         V16 qv = pv;
-        if (sub) qv = *reinterpret_cast<const V16*>(qrow + v0 + v1 + j * N);
+        if (sub) qv = *reinterpret_cast<const V16*>(qrow + first + v1 + j * N);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           pf[j * N + i] = at<Tag>(pv, i);
@@ -339,96 +344,133 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(
 #pragma unroll
       for (int i = 0; i < kPerThread; ++i) {
         const bool in = v1 + i < nv;
-        pf[i] = in ? value<Tag>(prow[v0 + v1 + i]) : 0.f;
-        qf[i] = in && sub ? value<Tag>(qrow[v0 + v1 + i]) : 0.f;
+        pf[i] = in ? value<Tag>(prow[first + v1 + i]) : 0.f;
+        qf[i] = in && sub ? value<Tag>(qrow[first + v1 + i]) : 0.f;
       }
     }
-    const uint32_t kids = kChain ? 0u : s_kids[v1 >> 5] >> (v1 & 31);
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) r[i] = (kids >> i) & 1u ? 0.0 : rest(pf[i], qf[i]);
+    for (int i = 0; i < kPerThread; ++i) r[i] = rest(pf[i], qf[i]);
   };
-  static_assert(kPerThread == 16, "a thread's tokens lie in one word of s_kids");
   auto slice_sum = [&]() {
     double s = 0.0;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) s += r[i];
     return s;
   };
+  // the first 64 slices' running sums and the total of all
+  double upto0, all;
   auto total_of = [&]() {
-    double all = 0.0, part;
-    for (int s0 = 0; s0 < slices; s0 += kThreads) {
-      block_scan(s0 + tid < slices ? mine[s0 + tid] : 0.0, s_wave, part);
-      all += part;
-    }
-    return all;
+    upto0 = wave_scan(v0);
+    all = __shfl(upto0, 63);
+    for (int s0 = 64; s0 < slices; s0 += 64) all += wave_sum(sum_of(s0 + lane));
   };
-  double all = total_of();
+  total_of();
   bool whole = false;
   if (!(all > 0.0)) {
     // nothing is left over (the rows are equal, or the children hold all of it): from the whole
     // row of p
     whole = true;
+    __syncthreads();  // every wave has read the sums
     for (int s = 0; s < slices; ++s) {
       load(s, true);
-      double part;
-      block_scan(slice_sum(), s_wave, part);
-      if (tid == 0) mine[s] = part;
-    }
-    __syncthreads();
-    all = total_of();
-  }
-  int64_t token = -1;
-  if (all > 0.0 && all <= DBL_MAX) {
-    const double goal = double(u_last[b]) * all;
-    // the first slice whose sums pass the goal, and the sum before it; where rounding or a u of 1
-    // leaves none, the last slice that holds anything
-    if (tid == 0) {
-      s_first = INT32_MAX;
-      s_last = -1;
-    }
-    double before = 0.0, part;
-    for (int s0 = 0; s0 < slices; s0 += kThreads) {
-      const double v = s0 + tid < slices ? mine[s0 + tid] : 0.0;
-      const double upto = before + block_scan(v, s_wave, part);
-      if (v > 0.0) {
-        if (upto > goal) atomicMin(&s_first, s0 + tid);
-        atomicMax(&s_last, s0 + tid);
-      }
-      before += part;
-    }
-    __syncthreads();
-    const bool found = s_first != INT32_MAX;
-    const int slice = found ? s_first : s_last;
-    before = 0.0;
-    for (int s0 = 0; s0 < slices; s0 += kThreads) {
-      block_scan(s0 + tid < slice ? mine[s0 + tid] : 0.0, s_wave, part);
-      before += part;
-    }
-    load(slice, whole);
-    __syncthreads();
-    if (tid == 0) {
-      s_first = INT32_MAX;
-      s_last = -1;
-    }
-    const double own = slice_sum();
-    double run = before + (block_scan(own, s_wave, part) - own);
-    int first = INT32_MAX, last = -1;
+      const double part = wave_sum(slice_sum());
+      if (lane == 0) s_wave[wave] = part;
+      __syncthreads();
+      if (tid == 0) {
+        double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      run += r[i];
-      if (r[i] > 0.0) {
-        if (first == INT32_MAX && run > goal) first = tid * kPerThread + i;
-        last = tid * kPerThread + i;
+        for (int w = 0; w < kWaves; ++w) sum += s_wave[w];
+        mine[s] = sum;
       }
+      __syncthreads();
     }
-    if (found && first != INT32_MAX) atomicMin(&s_first, first);
-    if (last >= 0) atomicMax(&s_last, last);
-    __syncthreads();
-    token = int64_t(slice) * kSlice + (s_first != INT32_MAX ? s_first : s_last);
-  } else if (tid == 0 && err_count) {
-    atomicAdd(err_count, 1);  // a row without a positive, finite sum: no token
+    v0 = sum_of(lane);
+    total_of();
   }
-  if (tid == 0) out_tokens[int64_t(b) * max_q_len + len] = token;
+  if (!(all > 0.0 && all <= DBL_MAX)) {
+    // a row without a positive, finite sum: no token
+    if (tid == 0) {
+      if (err_count) atomicAdd(err_count, 1);
+      out_tokens[int64_t(b) * max_q_len + seq.len] = -1;
+    }
+    return;
+  }
+  const double goal = u * all;
+  // the first slice whose sums pass the goal, and the sum before it; where rounding or a u of 1
+  // leaves none, the last slice that holds anything
+  int slice = -1;
+  bool found = false;
+  double before = 0.0, upto = upto0, v = v0, ahead = 0.0;
+  for (int s0 = 0; !found; ) {
+    const uint64_t some = __ballot(v > 0.0), hit = __ballot(v > 0.0 && upto > goal);
+    found = hit != 0;
+    const int l = found ? __ffsll(static_cast<unsigned long long>(hit)) - 1
+                        : (some ? 63 - __clzll(static_cast<long long>(some)) : -1);
+    if (l >= 0) {
+      slice = s0 + l;
+      before = l > 0 ? __shfl(upto, l - 1) : ahead;
+    }
+    ahead = __shfl(upto, 63);
+    s0 += 64;
+    if (s0 >= slices) break;
+    if (!found) {
+      v = sum_of(s0 + lane);
+      upto = ahead + wave_scan(v);
+    }
+  }
+  load(slice, whole);
+  if constexpr (!kChain) {
+    if (!whole) {
+      // tokens that the children hold count for nothing
+      __syncthreads();  // s_kids is clear
+      const int64_t first = int64_t(slice) * kSlice;
+#pragma unroll
+      for (int i = 0; i < kNodes; ++i)
+        if (kid[i] >= first && kid[i] < first + kSlice)
+          atomicOr(&s_kids[(kid[i] - first) >> 5], 1u << ((kid[i] - first) & 31));
+      __syncthreads();
+      static_assert(kPerThread == 16, "a thread's tokens lie in one word of s_kids");
+      const uint32_t kids = s_kids[(tid * kPerThread) >> 5] >> (tid * kPerThread & 31);
+#pragma unroll
+      for (int i = 0; i < kPerThread; ++i)
+        if ((kids >> i) & 1u) r[i] = 0.0;
+    }
+  }
+  const double own = slice_sum(), upto_own = wave_scan(own);
+  if (lane == 63) s_wave[wave] = upto_own;
+  __syncthreads();
+  double run = before;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) run += w < wave ? s_wave[w] : 0.0;
+  run += upto_own - own;
+  int first = -1, last = -1;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    run += r[i];
+    if (r[i] > 0.0) {
+      if (first < 0 && run > goal) first = tid * kPerThread + i;
+      last = tid * kPerThread + i;
+    }
+  }
+  const uint64_t firsts = __ballot(found && first >= 0), lasts = __ballot(last >= 0);
+  first = firsts ? __shfl(first, __ffsll(static_cast<unsigned long long>(firsts)) - 1) : -1;
+  last = lasts ? __shfl(last, 63 - __clzll(static_cast<long long>(lasts))) : -1;
+  if (lane == 0) {
+    s_first[wave] = first;
+    s_last[wave] = last;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    first = -1;
+    last = -1;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (first < 0) first = s_first[w];
+      if (s_last[w] >= 0) last = s_last[w];
+    }
+    out_tokens[int64_t(b) * max_q_len + seq.len] =
+        int64_t(slice) * kSlice + (first >= 0 ? first : last);
+  }
 }
 
 // The tokens that the target chose after each node are known: a node is kept where its token is
@@ -480,8 +522,8 @@ int launch_verify(const int64_t* tokens, const int32_t* parents, const void* tar
                   hipStream_t s) {
   using S = typename Tag::store;
   const int slices = int(slices_of(V));
-  double* sums = static_cast<double*>(workspace);
-  int32_t* info = reinterpret_cast<int32_t*>(sums + int64_t(B) * slices);
+  Info* info = reinterpret_cast<Info*>(workspace);
+  double* sums = reinterpret_cast<double*>(info + B);
   verify_walk_kernel<Tag, kChain>
       <<<dim3(unsigned(slices), unsigned(B)), kThreads, 0, s>>>(
           tokens, parents, static_cast<const S*>(target), ts, rows, static_cast<const S*>(draft),
@@ -490,7 +532,7 @@ int launch_verify(const int64_t* tokens, const int32_t* parents, const void* tar
   if (st != DSP_OK) return st;
   verify_pick_kernel<Tag, kChain><<<unsigned(B), kThreads, 0, s>>>(
       tokens, parents, static_cast<const S*>(target), ts, rows, static_cast<const S*>(draft), ds,
-      draft_rows, u_last, cu_q, max_q_len, V, slices, sums, info, out_tokens, err_count);
+      u_last, cu_q, max_q_len, V, slices, sums, info, out_tokens, err_count);
   return dsp_launch_status();
 }
 
@@ -507,7 +549,7 @@ int launch_verify_type(int32_t dtype, A... args) {
 
 extern "C" size_t dsp_verify_workspace_bytes(int32_t B, int64_t V) {
   if (B <= 0 || V <= 0) return 0;
-  return size_t(B) * (size_t(slices_of(V)) * sizeof(double) + kInfo * sizeof(int32_t));
+  return size_t(B) * (size_t(slices_of(V)) * sizeof(double) + sizeof(Info));
 }
 
 extern "C" int dsp_verify_draft(const int64_t* draft_tokens, const int32_t* parents,
@@ -533,7 +575,7 @@ extern "C" int dsp_verify_draft(const int64_t* draft_tokens, const int32_t* pare
                  DSP_EALIGN);
   DSP_HOST_CHECK(workspace && workspace_bytes >= dsp_verify_workspace_bytes(B, V),
                  DSP_EWORKSPACE);
-  DSP_HOST_CHECK(dsp_aligned(workspace, 8), DSP_EALIGN);
+  DSP_HOST_CHECK(dsp_aligned(workspace, 16), DSP_EALIGN);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (draft_probs)
     return launch_verify_type<true>(dtype, draft_tokens, parents, target_probs, target_stride,

@@ -18,6 +18,7 @@ import torch
 from dispec_amd import _lib
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_INTS = (torch.int64, torch.int32)
 
 
 class DraftVerdict(NamedTuple):
@@ -38,22 +39,21 @@ def _as(t, dtype):
 
 
 def _ints(t, name, n):
-    if t.dim() != 1 or t.numel() != n or t.dtype not in (torch.int32, torch.int64):
+    if t.shape != (n,) or t.dtype not in _INTS:
         raise ValueError(f"{name} must be ({n},) int32 or int64; got {tuple(t.shape)} {t.dtype}")
     return _as(t, torch.int64)
 
 
 def _layout(draft_tokens, cu_q, parents, max_q_len):
     """(tokens int64, cu_q int32, parents int32 or None, T, B, max_q_len) of a draft."""
+    T, B = draft_tokens.numel(), cu_q.numel() - 1
     if draft_tokens.dim() != 1:
         raise ValueError(f"draft_tokens has shape {tuple(draft_tokens.shape)}: expected (T,)")
-    T = draft_tokens.numel()
-    if cu_q.dim() != 1 or not cu_q.numel():
+    if cu_q.dim() != 1 or B < 0:
         raise ValueError(f"cu_q has shape {tuple(cu_q.shape)}: expected (B + 1,)")
-    if parents is not None and tuple(parents.shape) != (T,):
+    if parents is not None and parents.shape != (T,):
         raise ValueError(f"parents has shape {tuple(parents.shape)} for {T} nodes")
     cu_q = _as(cu_q, torch.int32)
-    B = cu_q.numel() - 1
     if max_q_len is None:
         max_q_len = int((cu_q[1:] - cu_q[:-1]).max().item()) if B else 0
     return (_ints(draft_tokens, "draft_tokens", T), cu_q,
@@ -61,13 +61,15 @@ def _layout(draft_tokens, cu_q, parents, max_q_len):
 
 
 def _outputs(B, width, device):
-    return DraftVerdict(torch.empty(B, dtype=torch.int32, device=device),
-                        torch.empty((B, width), dtype=torch.int32, device=device),
-                        torch.empty((B, width), dtype=torch.int64, device=device))
+    empty = torch.empty
+    return DraftVerdict(empty(B, dtype=torch.int32, device=device),
+                        empty((B, width), dtype=torch.int32, device=device),
+                        empty((B, width), dtype=torch.int64, device=device))
 
 
 def _rows(probs, name, dtype, vocab):
-    if probs.dim() != 2 or probs.shape[1] != vocab or probs.dtype != dtype:
+    shape = probs.shape
+    if len(shape) != 2 or shape[1] != vocab or probs.dtype != dtype:
         raise ValueError(f"{name} must be (rows, {vocab}) of {dtype}; got {tuple(probs.shape)} "
                          f"{probs.dtype}")
     return probs if probs.stride(1) == 1 or vocab == 1 else probs.contiguous()
@@ -122,7 +124,7 @@ def verify_draft(draft_tokens, target_probs, uniforms, final_uniforms, cu_q, par
             raise ValueError(f"draft_probs has {draft_probs.shape[0]} rows for {T} nodes of {B} "
                              "chains: one for each drafted token")
     for t, name, n in ((uniforms, "uniforms", T), (final_uniforms, "final_uniforms", B)):
-        if tuple(t.shape) != (n,) or t.dtype != torch.float32:
+        if t.shape != (n,) or t.dtype != torch.float32:
             raise ValueError(f"{name} must be ({n},) float32; got {tuple(t.shape)} {t.dtype}")
     uniforms, final_uniforms = uniforms.contiguous(), final_uniforms.contiguous()
     dev = target_probs.device

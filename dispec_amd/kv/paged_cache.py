@@ -77,34 +77,40 @@ def commit_path(key, value, block_table, cu_q, ctx_lens, path, num_accepted, blo
     """
     _lib.require_gpu(key, value, block_table, cu_q, ctx_lens, path, num_accepted, err)
     _lib.same_device(key, value, block_table, cu_q, ctx_lens, path, num_accepted, err)
-    if key.dim() != 4 or key.shape != value.shape or key.dtype != value.dtype:
+    shape, stride = key.shape, key.stride()
+    if len(shape) != 4 or value.shape != shape or value.dtype != key.dtype:
         raise ValueError(f"expected pools (L, slots, KVH, D) of one shape and dtype; got "
                          f"{tuple(key.shape)} {key.dtype}, {tuple(value.shape)} {value.dtype}")
-    L, S, KVH, D = key.shape
-    if key.stride() != value.stride() or key.stride(3) != 1 or key.stride(2) != D:
+    L, S, KVH, D = shape
+    if value.stride() != stride or stride[3] != 1 or stride[2] != D:
         raise ValueError("key and value need the same strides with contiguous rows")
     B = ctx_lens.numel()
-    if (block_table.dim() != 2 or block_table.shape[0] != B or cu_q.numel() != B + 1
-            or path.dim() != 2 or path.shape[0] != B or num_accepted.numel() != B):
+    table, paths = block_table.shape, path.shape
+    if (len(table) != 2 or table[0] != B or cu_q.numel() != B + 1 or len(paths) != 2
+            or paths[0] != B or num_accepted.numel() != B):
         raise ValueError(f"block_table {tuple(block_table.shape)}, cu_q {tuple(cu_q.shape)}, path "
                          f"{tuple(path.shape)}, num_accepted {tuple(num_accepted.shape)} for {B} "
                          "sequences")
-    for t, name in ((block_table, "block_table"), (cu_q, "cu_q"), (ctx_lens, "ctx_lens"),
-                    (path, "path"), (num_accepted, "num_accepted")):
-        if t.dtype != torch.int32:
-            raise ValueError(f"{name} must be int32, got {t.dtype}")
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+    int32 = torch.int32
+    if not (block_table.dtype == cu_q.dtype == ctx_lens.dtype == path.dtype == num_accepted.dtype
+            == int32):
+        name, dtype = next((name, t.dtype) for t, name in (
+            (block_table, "block_table"), (cu_q, "cu_q"), (ctx_lens, "ctx_lens"), (path, "path"),
+            (num_accepted, "num_accepted")) if t.dtype != int32)
+        raise ValueError(f"{name} must be int32, got {dtype}")
+    if block_table.stride(1) != 1 and table[1] > 1:
         block_table = block_table.contiguous()
-    if path.stride(1) != 1 and path.shape[1] > 1:
+    if path.stride(1) != 1 and paths[1] > 1:
         path = path.contiguous()
-    cu_q, ctx_lens, num_accepted = (t.contiguous() for t in (cu_q, ctx_lens, num_accepted))
+    cu_q, ctx_lens = cu_q.contiguous(), ctx_lens.contiguous()
+    num_accepted = num_accepted.contiguous()
     es = key.element_size()
     with _lib.on_device(key):
         _lib.check(_lib.calls().dsp_kv_commit_path(
-            key.data_ptr(), value.data_ptr(), L, key.stride(0) * es, key.stride(1) * es, S,
-            KVH * D * es, block_size, block_table.data_ptr(), block_table.stride(0),
-            block_table.shape[1], cu_q.data_ptr(), ctx_lens.data_ptr(), path.data_ptr(),
-            path.stride(0), path.shape[1], num_accepted.data_ptr(), B, _lib.ptr(err),
+            key.data_ptr(), value.data_ptr(), L, stride[0] * es, stride[1] * es, S, KVH * D * es,
+            block_size, block_table.data_ptr(), block_table.stride(0), table[1], cu_q.data_ptr(),
+            ctx_lens.data_ptr(), path.data_ptr(), path.stride(0), paths[1],
+            num_accepted.data_ptr(), B, _lib.ptr(err),
             _lib.stream_of(key)), "dsp_kv_commit_path")
 
 

@@ -432,7 +432,7 @@ int dsp_paged_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride
  *   path         : int32 [B, max_q_len], the kept nodes from the root (0) on, then -1.
  *   tokens       : int64 [B, max_q_len], their tokens without the root's, the drawn token, then -1.
  *                  (An empty sequence has 0, and -1 throughout.)
- *   workspace    : dsp_verify_workspace_bytes(B, V) bytes, 8-byte aligned. */
+ *   workspace    : dsp_verify_workspace_bytes(B, V) bytes, 16-byte aligned. */
 size_t dsp_verify_workspace_bytes(int32_t B, int64_t V);
 int dsp_verify_draft(const int64_t* draft_tokens, const int32_t* parents,
                      const void* target_probs, int64_t target_stride, int64_t num_rows,
