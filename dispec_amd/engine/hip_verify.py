@@ -17,6 +17,7 @@ import torch
 
 from dispec_amd import _lib
 
+MAX_TREE_NODES = 1024   # of one sequence, its root included
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _INTS = (torch.int64, torch.int32)
 

@@ -18,6 +18,10 @@ the HF modules, unchanged.  What the backend replaces is the KV path inside `_at
                                         blocks (copy-on-write forks of one prompt,
                                         prefix-cache hits) the shared-prefix variant
                                         attends those blocks once for the whole batch
+  * a batch with drafted trees         -> dsp_paged_tree_attention, one launch for the whole
+    (SeqMeta.parents)                   batch, each node with its ancestors (the reference
+                                        drafts chains); the logits then go to verify_draft or
+                                        match_draft and the kept path to cache.commit_path
 
 attn_backend is a string switch as in the reference (:48-52): "hip" (the default here)
 runs the kernels above; "native" keeps the reference's torch attention -- per sequence, the
@@ -38,8 +42,10 @@ import torch.nn.functional as F
 
 from dispec_amd import _lib
 from dispec_amd.engine.hip_attn import (decode_workspace, mq_workspace,
-                                       paged_decode_attention_blocks, paged_mq_attention)
+                                       paged_decode_attention_blocks, paged_mq_attention,
+                                       paged_tree_attention, tree_mask, tree_workspace)
 from dispec_amd.engine.hip_prologue import qk_norm_rope_append
+from dispec_amd.engine.hip_verify import MAX_TREE_NODES
 from dispec_amd.kv.paged_cache import PagedKVCache
 
 
@@ -50,6 +56,14 @@ class SeqMeta:
     block_ids: list[int]
     q_len: int      # new (query) tokens this step
     ctx_len: int    # context length including the new tokens
+    # the new tokens are a drafted tree's nodes (None: a chain): node i's parent, before it; the
+    # root, the last token that was kept, has -1.  A node sees the context and its ancestors; its
+    # position is the root's plus its depth, its slot that of the root's position plus i.
+    parents: list[int] | None = None
+
+    def is_tree(self) -> bool:
+        return (self.parents is not None
+                and any(p != i - 1 for i, p in enumerate(self.parents)))
 
 
 @dataclass
@@ -66,6 +80,7 @@ class _Batch:
     shared_prefix: int = 0   # leading context tokens all sequences share (0: none used)
     balanced: bool = False   # short query blocks on the balanced split-K kernel
     seqs: tuple = ()         # the host SeqMeta list (attn_backend="native" walks it)
+    tree_mask: torch.Tensor | None = None   # of a batch with drafted trees (see tree_mask)
 
 
 _BACKENDS = ("hip", "native")
@@ -165,7 +180,10 @@ class ModelRunner:
     def _batch(self, seq_meta: list[SeqMeta], cache: PagedKVCache) -> _Batch:
         B = len(seq_meta)
         width = max(max((len(m.block_ids) for m in seq_meta), default=1), 1)
-        host = torch.zeros((2 * B + 1 + B * width,), dtype=torch.int32)
+        trees = any(m.is_tree() for m in seq_meta)
+        T = sum(m.q_len for m in seq_meta)
+        end = 2 * B + 1 + B * width
+        host = torch.zeros(end + (T if trees else 0), dtype=torch.int32)
         cu = 0
         for i, m in enumerate(seq_meta):
             if m.ctx_len > len(m.block_ids) * cache.block_size:
@@ -176,18 +194,31 @@ class ModelRunner:
             if m.block_ids:
                 host[2 * B + 1 + i * width: 2 * B + 1 + i * width + len(m.block_ids)] = \
                     torch.tensor(m.block_ids, dtype=torch.int32)
+            if m.parents is not None and (
+                    len(m.parents) != m.q_len
+                    or not all(0 <= p < j or p == j - 1 for j, p in enumerate(m.parents))):
+                raise ValueError(f"sequence {i}: parents {m.parents} of {m.q_len} new tokens: -1, "
+                                 "then one earlier node for each")
+            if trees and m.q_len:
+                if m.q_len > MAX_TREE_NODES:
+                    raise ValueError(f"sequence {i}: {m.q_len} new tokens in a batch with drafted "
+                                     f"trees, which takes {MAX_TREE_NODES} a sequence at most")
+                host[end + cu - m.q_len:end + cu] = torch.tensor(
+                    range(-1, m.q_len - 1) if m.parents is None else m.parents, dtype=torch.int32)
         dev = host.to(cache.key.device)                 # one H2D copy for all metadata
         decode = all(m.q_len == 1 for m in seq_meta)
-        shared = self._shared_prefix(seq_meta, host[2 * B + 1:].view(B, width),
-                                     cache.block_size)
+        shared = 0 if trees else self._shared_prefix(
+            seq_meta, host[2 * B + 1:end].view(B, width), cache.block_size)
         max_q_len = max(m.q_len for m in seq_meta)
         max_ctx = width * cache.block_size
-        balanced = (not decode and not shared and
+        balanced = (not decode and not shared and not trees and
                     self._prefer_balanced(seq_meta, max_q_len, max_ctx, cache.block_size))
-        return _Batch(block_table=dev[2 * B + 1:].view(B, width), ctx_lens=dev[:B],
+        mask = (tree_mask(dev[end:], dev[B:2 * B + 1], max_q_len)
+                if trees and self.attn_backend == "hip" else None)
+        return _Batch(block_table=dev[2 * B + 1:end].view(B, width), ctx_lens=dev[:B],
                       cu_q=dev[B:2 * B + 1], max_q_len=max_q_len, max_ctx=max_ctx,
                       decode=decode, shared_prefix=shared, balanced=balanced,
-                      seqs=tuple(seq_meta))
+                      seqs=tuple(seq_meta), tree_mask=mask)
 
     def _prefer_balanced(self, seq_meta: list[SeqMeta], max_q_len: int, max_ctx: int,
                          bs: int) -> bool:
@@ -245,6 +276,12 @@ class ModelRunner:
                                 attn.k_norm if self.qk_norm else None)
         if self.attn_backend == "native":
             o = self._torch_attention(q, cache, layer_idx, batch.seqs)
+        elif batch.tree_mask is not None:
+            o = paged_tree_attention(
+                q, cache.key[layer_idx], cache.value[layer_idx], batch.block_table, batch.cu_q,
+                batch.ctx_lens, batch.tree_mask, self.kv_groups, block_size=cache.block_size,
+                scale=self.scale, max_q_len=batch.max_q_len, max_ctx=batch.max_ctx,
+                workspace=batch.workspace)
         elif batch.decode and not batch.shared_prefix:
             o = paged_decode_attention_blocks(
                 q, cache.key[layer_idx], cache.value[layer_idx], batch.block_table,
@@ -264,7 +301,7 @@ class ModelRunner:
         (model_runner.py:160-185) -- the sequence's context rows gathered from the pool
         (the prologue has already appended this step's k and v, so a fresh prefill reads
         back exactly the rows it projected), then torch SDPA with the bottom-right causal
-        mask and grouped KV heads.  SDPA runs in float32: torch's bf16 batched matmul on
+        mask (a drafted tree's nodes: their ancestors) and grouped KV heads.  SDPA runs in float32: torch's bf16 batched matmul on
         the transposed key operand SDPA forms is avoided on this platform; the output is
         rounded to the model dtype."""
         from torch.nn.attention.bias import causal_lower_right
@@ -274,10 +311,19 @@ class ModelRunner:
             start, end = end, end + m.q_len
             keys, vals = cache.gather(layer_idx, cache.context_slots(m.block_ids, m.ctx_len))
             as_bhd = lambda t: t.float().transpose(0, 1).unsqueeze(0)  # noqa: E731
+            seen = causal_lower_right(m.q_len, m.ctx_len)
+            if m.is_tree():
+                seen = torch.zeros(m.q_len, m.ctx_len, dtype=torch.bool)
+                seen[:, :m.ctx_len - m.q_len] = True
+                nodes = seen[:, m.ctx_len - m.q_len:]
+                for i, p in enumerate(m.parents):
+                    if p >= 0:
+                        nodes[i] = nodes[p]
+                    nodes[i, i] = True
+                seen = seen.to(q.device)
             o = F.scaled_dot_product_attention(
-                as_bhd(q[start:end]), as_bhd(keys), as_bhd(vals),
-                attn_mask=causal_lower_right(m.q_len, m.ctx_len), scale=self.scale,
-                enable_gqa=True)
+                as_bhd(q[start:end]), as_bhd(keys), as_bhd(vals), attn_mask=seen,
+                scale=self.scale, enable_gqa=True)
             out[start:end] = o[0].transpose(0, 1)
         return out
 
@@ -301,7 +347,11 @@ class ModelRunner:
         x = self.embed(token_ids)
         if batch.workspace is None and self.attn_backend == "hip":
             B = batch.ctx_lens.shape[0]
-            if batch.decode and not batch.shared_prefix:
+            if batch.tree_mask is not None:
+                batch.workspace = tree_workspace(B, self.num_heads, self.num_kv_heads,
+                                                 self.head_dim, batch.max_q_len, batch.max_ctx,
+                                                 cache.key.device)
+            elif batch.decode and not batch.shared_prefix:
                 batch.workspace = decode_workspace(B, self.num_heads, self.num_kv_heads,
                                                    self.head_dim, batch.max_ctx,
                                                    cache.key.device)

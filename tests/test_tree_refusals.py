@@ -197,3 +197,49 @@ def test_library_statuses():
         assert commit(**kw) == _lib.DSP_EINVAL, kw
     for kw in (dict(B=65536), dict(cols=1025)):
         assert commit(**kw) == _lib.DSP_EUNSUPPORTED, kw
+
+
+def test_the_runner_s_batches_of_trees():
+    """What SeqMeta.parents may hold, before anything reaches the GPU."""
+    import types
+
+    from dispec_amd.engine.model_runner import ModelRunner, SeqMeta
+    from tests.toy_lm import toy_lm
+    runner = ModelRunner(toy_lm("qwen3"), attn_backend="native")
+    cache = types.SimpleNamespace(block_size=16, key=torch.zeros(1))
+    meta = lambda n, parents: SeqMeta(list(range(100)), n, 600 + n, parents)  # noqa: E731
+    assert not meta(4, None).is_tree() and not meta(4, [-1, 0, 1, 2]).is_tree()
+    assert meta(4, [-1, 0, 0, 2]).is_tree()
+    for bad in ([-1, 0, 0], [0, 0, 0, 0], [-1, 1, 0, 0], [-1, 0, -1, 0], [-1, 0, 4, 0], []):
+        with pytest.raises(ValueError, match="parents"):
+            runner._batch([meta(4, bad)], cache)
+    with pytest.raises(ValueError, match="1024 a sequence"):
+        runner._batch([meta(4, [-1, 0, 0, 2]), SeqMeta(list(range(100)), 1025, 1025)], cache)
+    got = runner._batch([meta(4, [-1, 0, 0, 2]), meta(1, None), meta(3, None)], cache)
+    assert got.tree_mask is None and not got.shared_prefix and not got.balanced  # (native: on host)
+    assert got.cu_q.tolist() == [0, 4, 5, 8] and got.max_q_len == 4
+
+
+def test_native_attention_of_a_tree():
+    """attn_backend="native": a node's output is that of its path run as a chain."""
+    import types
+
+    from dispec_amd.engine.model_runner import ModelRunner, SeqMeta
+    from tests.toy_lm import toy_lm
+    runner = ModelRunner(toy_lm("qwen3"), attn_backend="native")
+    g = torch.Generator().manual_seed(1)
+    parents, base = [-1, 0, 0, 1, 1, 2], 9
+    n = len(parents)
+    k, v = (torch.randn(base + n, 2, 64, generator=g) for _ in range(2))
+    q = torch.randn(n, 4, 64, generator=g)
+    rows = types.SimpleNamespace(context_slots=lambda ids, c: c, gather=lambda i, c: (k[:c], v[:c]))
+    got = runner._torch_attention(q, rows, 0, (SeqMeta([0], n, base + n, parents),))
+    for i in range(n):
+        path = [i]
+        while parents[path[0]] >= 0:
+            path.insert(0, parents[path[0]])
+        keys = list(range(base)) + [base + j for j in path]
+        one = types.SimpleNamespace(context_slots=lambda ids, c: c,
+                                    gather=lambda i, c: (k[keys], v[keys]))
+        want = runner._torch_attention(q[path], one, 0, (SeqMeta([0], len(path), len(keys)),))
+        torch.testing.assert_close(got[i], want[-1], rtol=1e-5, atol=1e-5)
