@@ -17,9 +17,9 @@
 //  * Two workgroups of 4 waves (128 rows) to a CU for up to 128 rows a KV head, one of 8 waves (256
 //    rows, a chunk loaded once for twice the rows) above.
 //  * The list of (sequence, KV head, tile, chunk) units is cut into as many equal runs as there are
-//    workgroups resident on the chip, computed on the device from the lengths.  A run's end within
-//    kSnap chunks of a tile's end moves onto it.  A tile inside a run is written; a tile that runs
-//    cut leaves its rows' maximum, sum and accumulator per piece, and the second launch merges them.
+//    workgroups resident on the chip, computed on the device from the lengths; a tile's start counts
+//    as kStart chunks.  A tile inside a run is written; a tile that runs cut leaves its rows'
+//    maximum, sum and accumulator per piece, and the second launch merges them.
 //  * What bounds it, heads of 128 in bf16: 32 trees of 16 nodes (G 2, 500 to 4000 tokens, 321 MB) 81
 //    us, where the loads alone take 79; 4 trees of 64 (G 4, 32768 tokens) 205 us, 670 TFLOP/s: two
 //    waves a SIMD issue for 74 % of the time, what they compute runs on the matrix cores for 38 %.
@@ -40,7 +40,11 @@ using namespace dsp_mfma;
 
 constexpr int kChunk = 64;     // keys per chunk
 constexpr int kMinChunks = 2;  // a workgroup gets at least this many chunks
-constexpr int kSnap = 2;
+// What a run spends on a tile beside its chunks (ids, q, the pipeline's first loads, a partial result
+// or the output), in chunks: every tile counts as so many more when the list is cut.  32 sequences
+// of 500 to 4000 tokens, 8 KV heads, D 128, 256 and 512 rows a head: 160 and 269 us (counted as
+// nothing: 171 and 288); 4 to 8 pieces of equal tiles, where each has one start: 73 us (71).
+constexpr int kStart = 4;
 constexpr int kBlocks = 2048;  // block ids of a piece held in LDS
 constexpr int kDesc = 8;       // ints that describe a run's merge: pieces, q0, rows, KV head, tile
 constexpr int kMaskThreads = 256;
@@ -91,7 +95,7 @@ struct Div {
 // One sequence: `tiles` of TR packed rows (its first max_q_len nodes'), each of `chunks` units (one
 // unit a tile where the tiles stay whole).
 struct TreeSeq {
-  int q0, n, ctx, rows, tiles, chunks, units;
+  int q0, n, ctx, rows, tiles, chunks, per_tile, units;
 };
 __device__ __forceinline__ bool tree_bad(int n, int ctx, int max_ctx) {
   return n > 0 && (ctx < n || ctx > max_ctx);
@@ -107,7 +111,8 @@ __device__ __forceinline__ TreeSeq tree_seq(int q0, int q1, int ctx, int G, int 
   s.rows = none ? 0 : min(s.n, max_q_len) * G;
   s.tiles = (s.rows + TR - 1) / TR;
   s.chunks = none ? 0 : (ctx + kChunk - 1) / kChunk;
-  s.units = whole ? s.tiles : s.tiles * s.chunks;
+  s.per_tile = whole ? 1 : kStart + s.chunks;
+  s.units = s.tiles * s.per_tile;
   return s;
 }
 __device__ __forceinline__ TreeSeq lane_seq(const TreeSeq& s, int l) {
@@ -118,6 +123,7 @@ __device__ __forceinline__ TreeSeq lane_seq(const TreeSeq& s, int l) {
   r.rows = __builtin_amdgcn_readlane(s.rows, l);
   r.tiles = __builtin_amdgcn_readlane(s.tiles, l);
   r.chunks = __builtin_amdgcn_readlane(s.chunks, l);
+  r.per_tile = __builtin_amdgcn_readlane(s.per_tile, l);
   r.units = __builtin_amdgcn_readlane(s.units, l);
   return r;
 }
@@ -245,10 +251,10 @@ tree_tile_kernel(
   const int w = xcd < r8 ? xcd * (q8 + 1) + pos : r8 * (q8 + 1) + (xcd - r8) * q8 + pos;
   const Div by_w(W);
   const int share = by_w(C), extra = C - share * W;
-  int b = 0, kvh = 0, tile = 0, c0 = 0;  // where the run stands
+  int b = 0, kvh = 0, tile = 0, x = 0;   // where the run stands: unit x of a tile
   int base = 0;                          // units (of all KV heads) before sequence b
   TreeSeq sq;
-  // unit u -> (b, kvh, tile, c0); u < C
+  // unit u -> (b, kvh, tile, x); u < C
   auto locate = [&](int u) {
     for (int f = 0, pre = 0; f < B; f += 64) {
       if (f != first || B > 64) look(f);
@@ -266,12 +272,12 @@ tree_tile_kernel(
     int rest = u - base;
     kvh = __builtin_amdgcn_readfirstlane(Div(sq.units)(rest));
     rest -= kvh * sq.units;
-    tile = whole ? rest : __builtin_amdgcn_readfirstlane(Div(sq.chunks)(rest));
-    c0 = whole ? 0 : rest - tile * sq.chunks;
+    tile = __builtin_amdgcn_readfirstlane(Div(sq.per_tile)(rest));
+    x = rest - tile * sq.per_tile;
   };
   // the tile after this one (there is one)
   auto next_tile = [&]() {
-    c0 = 0;
+    x = 0;
     if (++tile < sq.tiles) return;
     tile = 0;
     if (++kvh < KVH) return;
@@ -282,8 +288,7 @@ tree_tile_kernel(
       sq = tree_seq<TR>(cu_q[b], cu_q[b + 1], ctx_lens[b], G, max_q_len, max_ctx, whole != 0);
     } while (sq.units <= 0);
   };
-  // Run w begins at unit floor(w C / W), moved onto a tile's end where that is within kSnap chunks
-  // (in the same way by both its neighbours).
+  // Run v begins at unit floor(v C / W), or at the tile's first where that is one of its kStart.
   auto begin_of = [&](int v) {
     return __builtin_amdgcn_readfirstlane(v * share + by_w(v * extra));
   };
@@ -292,21 +297,14 @@ tree_tile_kernel(
     end = begin_of(w + 1);
     if (!whole) {
       locate(end);
-      if (c0 <= kSnap) end -= c0;
-      else if (sq.chunks - c0 <= kSnap) end += sq.chunks - c0;
+      if (x <= kStart) end -= x;
     }
   }
-  int u = begin_of(w);
-  locate(u);
-  int left;
-  if (whole || c0 <= kSnap) {
-    left = end - (u - c0);
-    c0 = 0;
-  } else if (sq.chunks - c0 <= kSnap) {
-    left = end - (u + sq.chunks - c0);
-    if (left > 0) next_tile();
-  } else {
-    left = end - u;
+  int left = end - begin_of(w);
+  locate(begin_of(w));
+  if (!whole && x <= kStart) {
+    left += x;
+    x = 0;
   }
 
   // ---- its pieces: chunks c0 .. c1 of a tile
@@ -325,7 +323,8 @@ tree_tile_kernel(
   int32_t d_np = 0, d_q0 = 0, d_rows = 0, d_kvh = 0, d_tile = 0;
   bool any_bad = false;
   for (bool again = false; left > 0; again = true) {
-    const int nch = sq.chunks, c1 = whole ? nch : min(nch, c0 + left);
+    const int nch = sq.chunks, c0 = x == 0 ? 0 : x - kStart;
+    const int took = min(sq.per_tile - x, left), c1 = x + took == sq.per_tile ? nch : x + took - kStart;
     const int kbeg = c0 * kChunk, kfin = min(c1 * kChunk, sq.ctx), tree0 = sq.ctx - sq.n;
     const int r0 = tile * TR + 32 * wave;   // this wave's first row
     const int64_t bt_row = int64_t(b) * bt_stride;
@@ -703,10 +702,10 @@ tree_tile_kernel(
     }
     if (c0 == 0 && !whole) {
       // this run began the tile: its merge is described here.  Pieces: up to the last run that
-      // begins before the tile's end (those within kSnap moved onto it).
+      // begins before the tile's end.
       int np = 0;
       if (!complete) {
-        const int upto = base + (kvh * sq.tiles + tile + 1) * nch - kSnap;
+        const int upto = base + (kvh * sq.tiles + tile + 1) * sq.per_tile;
         int v = min(W - 1, int(float(upto) * float(W) / float(C)));
         while (begin_of(v) >= upto) --v;
         while (v + 1 < W && begin_of(v + 1) < upto) ++v;
@@ -723,7 +722,7 @@ tree_tile_kernel(
         d[1] = w;
       }
     }
-    left -= whole ? 1 : c1 - c0;
+    left -= took;
     if (left > 0) next_tile();
   }
   if (err_count && any_bad && lane == 0) atomicAdd(err_count, 1);  // once per wave
@@ -872,15 +871,15 @@ TreePlan tree_plan(int32_t B, int32_t KVH, int32_t G, int32_t D, int32_t max_q_l
   // with two of 4, which load a chunk for 128 rows each).
   p.rows = D > 128 || rows <= 128 ? 128 : 256;
   const int64_t per_head = (rows + p.rows - 1) / p.rows, tiles = per_head * B * KVH;
-  const int64_t chunks = (int64_t(max_ctx) + kChunk - 1) / kChunk;
+  const int64_t chunks = (int64_t(max_ctx) + kChunk - 1) / kChunk, units = chunks + kStart;
   // (the numbers that Div divides)
-  p.tile = max_ctx < (1 << 24) && rows < (1 << 24) && tiles * chunks < (1 << 24) && B < (1 << 16);
+  p.tile = max_ctx < (1 << 24) && rows < (1 << 24) && tiles * units < (1 << 24) && B < (1 << 16);
   if (!p.tile) return p;
   p.whole = chunks <= 8;
   p.least = p.whole ? 1 : kMinChunks;
   // workgroups that fit the chip at once (LDS)
   const int64_t slots = int64_t(dsp_detail::device_cus()) * (p.rows == 128 && D <= 128 ? 2 : 1);
-  p.workers = int(std::min((p.whole ? tiles : (tiles * chunks + p.least - 1) / p.least), slots));
+  p.workers = int(std::min((p.whole ? tiles : (tiles * units + p.least - 1) / p.least), slots));
   p.tiles_max = tiles <= p.workers ? int(per_head) : 0;
   p.items = tiles <= p.workers ? int(tiles) : p.workers;
   return p;
