@@ -202,8 +202,9 @@ tree_tile_kernel(
   // Stage c of a piece is V of its chunk c and K of chunk c + 1, what one turn of the loop needs.
   // [buffer][K | V]
   __shared__ __attribute__((aligned(1024))) char lds[NB][2][SLAB];
-  // of each wave's rows: bit 2 wave: K's block id is bad, 2 wave + 1: odd values in V
-  __shared__ __attribute__((aligned(16))) int32_t s_flag[NB][NW];
+  // of a stage, bit 2 wave: a wave's rows of K have a bad block id, 2 wave + 1: its rows of V hold
+  // infinities or NaN.  Set before the stage's barrier, cleared after the next one's.
+  __shared__ int32_t s_flag[4];
   __shared__ int32_t s_blk[kBlocks + 16];        // block ids of a piece (16: read ahead, not used)
 
   const int lane = threadIdx.x & 63;
@@ -399,7 +400,8 @@ tree_tile_kernel(
       fetch(vbase + rows_off, c, slab_of(buf, 1), true);
       send_k(c + 1, buf);
     };
-    if (again) __syncthreads();  // every wave is done with the previous piece's buffers and ids
+    if (again) __syncthreads();  // every wave is done with the previous piece's buffers, ids, flags
+    if (threadIdx.x < 4) s_flag[threadIdx.x] = 0;
     stage_ids(kbeg);
     // the wait for the ids was one for the q rows too (issued before them): none is left to the
     // loop, whose loads the compiler cannot count
@@ -415,22 +417,12 @@ tree_tile_kernel(
     for (; sent < min(held, NB - 1); ++sent) send_stage(sent);
     __builtin_amdgcn_sched_barrier(0);
     wait_chunks<NB - 1, 2 * LPW>(sent);
-    s_flag[NB - 1][wave] = int(((bad_k >> (NB - 1)) & 1u) << 2 * wave);
+    if ((bad_k >> (NB - 1)) & 1u && lane == 0) atomicOr(&s_flag[3], 1 << 2 * wave);
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);
     constexpr int kBadK = 0x5555, kOddV = 0xaaaa;
-    auto flags_of = [&](int buf) {
-      int f = 0;
-#pragma unroll
-      for (int x = 0; x < NW; x += 4) {
-        const dsp_u32x4 four = *reinterpret_cast<const dsp_u32x4*>(&s_flag[buf][x]);
-        f |= int(four[0] | four[1] | four[2] | four[3]);
-      }
-      return f;
-    };
     // Stage c is in LDS, for every wave: its loads are waited for, its flags (of every wave's rows)
-    // returned; the stage NB - 1 further on is sent for into the buffer of stage c - 1, which every
-    // wave is done with.
+    // returned.
     auto arrive = [&](int c) -> int {
       const int buf = c & (NB - 1);
       if (c == sent) {  // (a piece longer than the ids held)
@@ -449,12 +441,15 @@ tree_tile_kernel(
         __builtin_amdgcn_sched_barrier(0);
         flag |= any_nonfinite<Tag, LPW>(my_v) ? 2 : 0;
       }
-      s_flag[buf][wave] = flag << 2 * wave;
+      if (flag != 0 && lane == 0) atomicOr(&s_flag[c & 3], flag << 2 * wave);
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
-      const int flags = flags_of(buf);
+      if (threadIdx.x == 0) s_flag[(c + 3) & 3] = 0;
+      return s_flag[c & 3];
+    };
+    // The stage NB - 1 further on, into the buffer of stage c - 1, which every wave is done with.
+    auto send_next = [&](int c) {
       if (sent < min(held, c + NB)) send_stage(sent++);
-      return flags;
     };
     // ---- operands from LDS.  K: row 32*x + col of buffer buf, 16-byte piece 2*ks + hl, which lies at
     // piece (2*ks + hl) ^ kswz(row): the bits that ks sets are XORed into the address.  V^T: as in
@@ -584,6 +579,7 @@ tree_tile_kernel(
     };
     constexpr int kFirst = NB - 1;  // the buffer of K of chunk 0
     constexpr int kAhead = NDT < 3 ? NDT : 3;  // operands read ahead of their MFMAs
+    constexpr int kSendAt = 1;  // the step of a chunk's first half in which the next stage is sent for
     // A half's exponentials, 1 / NKS of them at a time (step i).
     static_assert(NKS <= 16 && NKS == 2 * NDT, "a step has one exponential or more");
     auto take_probs = [&](f32x16& sc, int i, float neg_m, dsp_u32x4 (&pop)[2]) {
@@ -595,7 +591,7 @@ tree_tile_kernel(
         if (j & 1) pop[j >> 3][(j >> 1) & 3] = narrow2<Tag>(sc[j - 1], sc[j]);
       }
     };
-    int kflags = flags_of(kFirst);  // (in a vector register until it is looked at)
+    int kflags = s_flag[3];  // (in a vector register until it is looked at)
     // Half by half, a pipeline in which the MFMAs of one half's scores and of another's P V have
     // the exponentials of a third beside them, instruction by instruction (a wave issues in order:
     // MFMAs in a row, each after the wait for its operands, left the chip 67 % idle).  half(x): the
@@ -634,6 +630,7 @@ tree_tile_kernel(
           vop[i + kAhead] = read_v(at, x, (i + kAhead) / NDT, (i + kAhead) % NDT);
         }
         next = mfma32x32<Tag>(kop[i], qop[i], next);
+        if (x == 0 && i == kSendAt) send_next(c);
         take_probs(cur, i, neg_m, fresh);
         __builtin_amdgcn_sched_barrier(0);
         acc[i % NDT] = mfma32x32<Tag>(vop[i], pop[i / NDT], acc[i % NDT]);
@@ -656,6 +653,8 @@ tree_tile_kernel(
       if (wave_has_rows) {
         half(std::integral_constant<int, 0>{}, c, 1, buf, kflags, s1, s0);
         if (c + 1 < nc) half(std::integral_constant<int, 1>{}, c + 1, 0, buf, flags, s0, s1);
+      } else {
+        send_next(c);  // (it only loads)
       }
       kflags = flags;
     }
