@@ -241,7 +241,7 @@ tree_tile_kernel(
     }
   }
   const int C = total * KVH;
-  const int W = min(Div(least)(C + least - 1), int(gridDim.x));
+  const int W = min(C / least + (C % least != 0), int(gridDim.x));
   if (lin >= W) {
     if (!whole && tiles_max == 0 && threadIdx.x == 0) ws_desc[kDesc * lin] = 0;
     return;
@@ -251,7 +251,7 @@ tree_tile_kernel(
   const int q8 = W / 8, r8 = W % 8, xcd = lin % 8, pos = lin / 8;
   const int w = xcd < r8 ? xcd * (q8 + 1) + pos : r8 * (q8 + 1) + (xcd - r8) * q8 + pos;
   const Div by_w(W);
-  const int share = by_w(C), extra = C - share * W;
+  const int share = C / W, extra = C - share * W;  // (C: of any size)
   int b = 0, kvh = 0, tile = 0, x = 0;   // where the run stands: unit x of a tile
   int base = 0;                          // units (of all KV heads) before sequence b
   TreeSeq sq;
@@ -325,7 +325,8 @@ tree_tile_kernel(
   bool any_bad = false;
   for (bool again = false; left > 0; again = true) {
     const int nch = sq.chunks, c0 = x == 0 ? 0 : x - kStart;
-    const int took = min(sq.per_tile - x, left), c1 = x + took == sq.per_tile ? nch : x + took - kStart;
+    const int took = min(sq.per_tile - x, left);
+    const int c1 = x + took == sq.per_tile ? nch : x + took - kStart;
     const int kbeg = c0 * kChunk, kfin = min(c1 * kChunk, sq.ctx), tree0 = sq.ctx - sq.n;
     const int r0 = tile * TR + 32 * wave;   // this wave's first row
     const int64_t bt_row = int64_t(b) * bt_stride;
@@ -871,8 +872,9 @@ TreePlan tree_plan(int32_t B, int32_t KVH, int32_t G, int32_t D, int32_t max_q_l
   p.rows = D > 128 || rows <= 128 ? 128 : 256;
   const int64_t per_head = (rows + p.rows - 1) / p.rows, tiles = per_head * B * KVH;
   const int64_t chunks = (int64_t(max_ctx) + kChunk - 1) / kChunk, units = chunks + kStart;
-  // (the numbers that Div divides)
-  p.tile = max_ctx < (1 << 24) && rows < (1 << 24) && tiles * units < (1 << 24) && B < (1 << 16);
+  // (numbers that Div divides: a sequence's units; 32 bits: all)
+  p.tile = max_ctx < (1 << 24) && rows < (1 << 24) && per_head * units * KVH < (1 << 24) &&
+           tiles * units < (int64_t(1) << 31);
   if (!p.tile) return p;
   p.whole = chunks <= 8;
   p.least = p.whole ? 1 : kMinChunks;

@@ -313,3 +313,42 @@ def test_a_shared_workspace(hip):
             assert torch.equal(c.call(workspace=ws), want)
     tiny = torch.zeros(4, device=DEV)
     assert torch.equal(c.call(workspace=tiny), want) and bool((tiny == 0).all())
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128)])
+def test_runs_longer_than_the_ids_held(hip, dtype, D):
+    """Contexts so long, and so many, that a workgroup's part of one is longer than the block ids it
+    holds at a time.  The tables name a few blocks again and again: a slot's weight in 64 bits is
+    its count times its exponential."""
+    from dispec_amd.engine.hip_attn import paged_tree_attention
+    B, H, bs, n, ctx, blocks = 16, 8, 16, 3, 150_001, 40
+    g = torch.Generator().manual_seed(31)
+    k, v = (torch.randn(blocks * bs, H, D, generator=g).to(dtype).to(DEV) for _ in range(2))
+    q = torch.randn(B * n, H, D, generator=g).to(dtype).to(DEV)
+    width = -(-ctx // bs)
+    bt = torch.randint(0, blocks, (B, width), generator=g, dtype=torch.int32)
+    cu = torch.arange(0, B * n + 1, n, dtype=torch.int32, device=DEV)
+    lens = torch.full((B,), ctx, dtype=torch.int32, device=DEV)
+    mask = torch.tensor([[1], [3], [5]] * B, dtype=torch.int32, device=DEV)
+    got = f64(paged_tree_attention(q, k, v, bt.to(DEV), cu, lens, mask, 1, block_size=bs, max_q_len=n,
+                                   max_ctx=ctx))
+    kk, vv, qq = f64(k), f64(v), f64(q)
+    half = torch.finfo(dtype).eps / 2
+    f32 = 2.0 ** -24 * (2 * (D + 2) * np.abs(qq).max() * np.abs(kk).max() * D ** 0.5 + ctx + 64)
+    pos = np.arange(ctx)
+    for b in range(B):
+        slots = bt[b].numpy()[pos // bs].astype(np.int64) * bs + pos % bs
+        base = np.bincount(slots[:ctx - n], minlength=blocks * bs).astype(np.float64)
+        for i, nodes in enumerate(((0,), (0, 1), (0, 2))):
+            count = base.copy()
+            for a in nodes:
+                count[slots[ctx - n + a]] += 1
+            for h in range(H):
+                s = kk[:, h] @ qq[b * n + i, h] * D ** -0.5
+                p = count * np.exp(s - s.max())
+                o, A = p @ vv[:, h] / p.sum(), p @ np.abs(vv[:, h]) / p.sum()
+                bound = half * np.abs(o) + f32 * A
+                bound = bound * (1 + 2 * half) + half * A * (1 + 2 * half)
+                if dtype == F16:
+                    bound = bound + 2.0 ** -25 * ctx * np.abs(vv).max()
+                assert (np.abs(got[b * n + i, h] - o) <= bound).all(), (b, i, h)
