@@ -45,6 +45,11 @@ constexpr int kMinChunks = 2;  // a workgroup gets at least this many chunks
 // of 500 to 4000 tokens, 8 KV heads, D 128, 256 and 512 rows a head: 160 and 269 us (counted as
 // nothing: 171 and 288); 4 to 8 pieces of equal tiles, where each has one start: 73 us (71).
 constexpr int kStart = 4;
+// K and V of a call that take so many bytes bypass the caches' replacement order (non-temporal loads):
+// half of the last-level cache, behind which the next call finds little of its own anyway.  321 MB
+// in 32 sequences 71.8 us (81.9 without), 130 MB in 6 35.5 (40.0); 42 MB that a call before left
+// there 36.2 (33.7).
+constexpr int64_t kStream = int64_t(128) << 20;
 constexpr int kBlocks = 2048;  // block ids of a piece held in LDS
 constexpr int kDesc = 8;       // ints that describe a run's merge: pieces, q0, rows, KV head, tile
 constexpr int kMaskThreads = 256;
@@ -188,7 +193,7 @@ tree_tile_kernel(
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ ctx_lens,
     const uint32_t* __restrict__ mask, int32_t words, int32_t B, int32_t KVH, int32_t G,
     int32_t max_q_len, int32_t max_ctx, float scale_log2, int32_t whole, int32_t least,
-    int32_t tiles_max, float* __restrict__ ws_acc, float* __restrict__ ws_ml,
+    int32_t stream_units, int32_t tiles_max, float* __restrict__ ws_acc, float* __restrict__ ws_ml,
     int32_t* __restrict__ ws_desc, uint16_t* __restrict__ out, int64_t ost, int64_t osh,
     int32_t vec_out, int32_t* __restrict__ err_count) {
   constexpr int NW = S::NW, TR = S::TR, NB = S::bufs(D);
@@ -250,6 +255,7 @@ tree_tile_kernel(
   // tiles and pieces of one (sequence, KV head) share an L2
   const int q8 = W / 8, r8 = W % 8, xcd = lin % 8, pos = lin / 8;
   const int w = xcd < r8 ? xcd * (q8 + 1) + pos : r8 * (q8 + 1) + (xcd - r8) * q8 + pos;
+  const bool stream = C > stream_units;
   const Div by_w(W);
   const int share = C / W, extra = C - share * W;  // (C: of any size)
   int b = 0, kvh = 0, tile = 0, x = 0;   // where the run stands: unit x of a tile
@@ -367,20 +373,26 @@ tree_tile_kernel(
     int32_t id_next = 0;
     auto first_key = [&](int c) { return min(kbeg + c * kChunk + RPW * wave, kfin - 1); };
     auto read_id = [&](int c) { id_next = s_blk[(first_key(c) >> log2_bs) - blk0]; };
-    // rows from `off` into a slab; those past kfin as the last key's (a stale row may hold anything)
+    // rows from `rows` on into a slab; those past kfin as the last key's (a stale row may hold
+    // anything)
     auto fetch = [&](const char* rows, int c, uint32_t m0, bool is_v) {
       if (kbeg + (c + 1) * kChunk > kfin) {
         const int room = kfin - 1 - first_key(c);
 #pragma unroll
         for (int j = 0; j < LPW; ++j) {
           const int rw = j * RPI + lane / CPR, row = RPW * wave + rw, sl = lane % CPR;
-          dma16<false>(rows, uint32_t(min(rw, room)) * slot_bytes +
-                                 16 * (sl ^ (is_v ? vswz(row) : kswz(row))), m0 + j * 1024);
+          dma16<true>(rows, uint32_t(min(rw, room)) * slot_bytes +
+                                16 * (sl ^ (is_v ? vswz(row) : kswz(row))), m0 + j * 1024);
         }
         return;
       }
+      if (stream) {
 #pragma unroll
-      for (int j = 0; j < LPW; ++j) dma16<false>(rows, is_v ? voff[j] : koff[j], m0 + j * 1024);
+        for (int j = 0; j < LPW; ++j) dma16<true>(rows, is_v ? voff[j] : koff[j], m0 + j * 1024);
+      } else {
+#pragma unroll
+        for (int j = 0; j < LPW; ++j) dma16<false>(rows, is_v ? voff[j] : koff[j], m0 + j * 1024);
+      }
     };
     auto slab_of = [&](int buf, int plane) {
       return lds_base + uint32_t((2 * buf + plane) * SLAB + wave * LPW * 1024);
@@ -900,13 +912,17 @@ int launch_tree(const TreePlan& p, const uint16_t* q, int64_t qst, int64_t qsh, 
                 hipStream_t s) {
   float* ws_ml = ws + int64_t(2) * p.workers * p.rows * D;
   int32_t* ws_desc = reinterpret_cast<int32_t*>(ws_ml + int64_t(4) * p.workers * p.rows);
+  // (all tiles of a sequence and KV head read the same chunks)
+  const int stream_units = int(std::min(
+      kStream / (4 * kChunk * D) * ((int64_t(max_q_len) * G + p.rows - 1) / p.rows),
+      (int64_t(1) << 31) - 1));
   const int vec_out = ost % 4 == 0 && osh % 4 == 0 && dsp_aligned(out, 8);
   auto launch = [&](auto shape) {
     using S = decltype(shape);
     tree_tile_kernel<Tag, D, S><<<p.workers, 64 * S::NW, 0, s>>>(
         q, qst, qsh, kc, vc, uint32_t(num_slots >> log2_bs), int32_t(kvs_slot), kvs_head, bt,
         bt_stride, log2_bs, cu_q, ctx_lens, mask, words, B, KVH, G, max_q_len, max_ctx, scale_log2,
-        p.whole, p.least, p.tiles_max, ws, ws_ml, ws_desc, out, ost, osh, vec_out, err_count);
+        p.whole, p.least, stream_units, p.tiles_max, ws, ws_ml, ws_desc, out, ost, osh, vec_out, err_count);
   };
   if constexpr (D <= 128) {
     if (p.rows == 256) launch(Shape<8, 1>{});
