@@ -227,19 +227,29 @@ def stream_of(t) -> int:
 def on_device(t):
     """A context in which t's device is the current one: a launch on a stream of another device
     than the current fails.  (The device is nearly always the current one: no context then.)"""
-    import torch
+    global _current_device
+    if _current_device is None:  # (torch is imported on first use)
+        import torch
+        _current_device = torch.cuda.current_device
     index = t.get_device()
-    return _SAME if index == torch.cuda.current_device() else torch.cuda.device(index)
+    if index == _current_device():
+        return _SAME
+    import torch
+    return torch.cuda.device(index)
 
 
 _SAME = contextlib.nullcontext()
+_current_device = None
 
 
-def same_device(t, *others) -> None:
-    """ValueError unless the tensors (or None) are on t's device."""
-    index = t.get_device()
+def one_gpu(t, *others) -> None:
+    """`require_gpu`, and ValueError unless the tensors (or None) are on one device."""
+    index = t.get_device()   # (-1: the CPU)
+    if index < 0:
+        require_gpu(t, *others)
     for o in others:
         if o is not None and o.get_device() != index:
+            require_gpu(t, *others)
             raise ValueError(f"tensors on {t.device} and {o.device}: one call takes one device")
 
 

@@ -375,8 +375,7 @@ def tree_mask(parents, cu_q, max_q_len=None, num_tokens=None):
                 device->host copy)
     num_tokens: T, for chains
     """
-    _lib.require_gpu(parents, cu_q)
-    _lib.same_device(cu_q, parents)
+    _lib.one_gpu(cu_q, parents)
     if cu_q.dim() != 1 or not cu_q.numel():
         raise ValueError(f"cu_q has shape {tuple(cu_q.shape)}: expected (B + 1,)")
     if parents is None and num_tokens is None:
@@ -427,9 +426,7 @@ def paged_tree_attention(q, k_cache, v_cache, block_table, cu_q, ctx_lens, tree_
     err:         optional int32 device counter of bad lengths and block ids
     returns:     (sum q_len, num_heads, head_dim) in q's dtype
     """
-    _lib.require_gpu(q, k_cache, v_cache, block_table, cu_q, ctx_lens, tree_mask, out, err, workspace)
-    _lib.same_device(q, k_cache, v_cache, block_table, cu_q, ctx_lens, tree_mask, out, err,
-                     workspace)
+    _lib.one_gpu(q, k_cache, v_cache, block_table, cu_q, ctx_lens, tree_mask, out, err, workspace)
     if q.dim() != 3 or k_cache.dim() != 3 or v_cache.shape != k_cache.shape:
         raise ValueError(f"expected q (T, Hq, D) and caches (S, KVH, D); got {tuple(q.shape)}, "
                          f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")

@@ -61,19 +61,10 @@ def _layout(draft_tokens, cu_q, parents, max_q_len):
             None if parents is None else _as(parents, torch.int32), T, B, int(max_q_len))
 
 
-def _outputs(B, width, device):
-    empty = torch.empty
-    return DraftVerdict(empty(B, dtype=torch.int32, device=device),
-                        empty((B, width), dtype=torch.int32, device=device),
-                        empty((B, width), dtype=torch.int64, device=device))
-
-
-def _rows(probs, name, dtype, vocab):
-    shape = probs.shape
-    if len(shape) != 2 or shape[1] != vocab or probs.dtype != dtype:
-        raise ValueError(f"{name} must be (rows, {vocab}) of {dtype}; got {tuple(probs.shape)} "
-                         f"{probs.dtype}")
-    return probs if probs.stride(1) == 1 or vocab == 1 else probs.contiguous()
+def _outputs(B, width, like):
+    empty = like.new_empty   # (of the allocations a call makes the cheapest form)
+    return DraftVerdict(empty(B, dtype=torch.int32), empty((B, width), dtype=torch.int32),
+                        empty((B, width), dtype=torch.int64))
 
 
 def verify_draft(draft_tokens, target_probs, uniforms, final_uniforms, cu_q, parents=None,
@@ -105,40 +96,46 @@ def verify_draft(draft_tokens, target_probs, uniforms, final_uniforms, cu_q, par
                     rows without a positive, finite sum (whose token is -1)
     returns:        DraftVerdict
     """
-    _lib.require_gpu(draft_tokens, target_probs, uniforms, final_uniforms, cu_q, parents,
-                     draft_probs, err)
-    _lib.same_device(target_probs, draft_tokens, uniforms, final_uniforms, cu_q, parents,
-                     draft_probs, err)
+    _lib.one_gpu(target_probs, draft_tokens, uniforms, final_uniforms, cu_q, parents, draft_probs,
+                 err)
     if parents is not None and draft_probs is not None:
         raise ValueError("draft_probs are a chain's: parents and draft_probs exclude each other")
     tokens, cu_q, parents, T, B, max_q_len = _layout(draft_tokens, cu_q, parents, max_q_len)
-    if target_probs.dtype not in _DTYPES or target_probs.dim() != 2:
-        raise ValueError(f"target_probs must be (T, V) bf16, fp16 or fp32; got "
-                         f"{tuple(target_probs.shape)} {target_probs.dtype}")
-    dtype, V = target_probs.dtype, target_probs.shape[1]
-    target_probs = _rows(target_probs, "target_probs", dtype, V)
-    if target_probs.shape[0] != T:
-        raise ValueError(f"target_probs has {target_probs.shape[0]} rows for {T} nodes")
+    dtype, shape = target_probs.dtype, target_probs.shape
+    if dtype not in _DTYPES or len(shape) != 2:
+        raise ValueError(f"target_probs must be (T, V) bf16, fp16 or fp32; got {tuple(shape)} {dtype}")
+    rows, V = shape
+    if rows != T:
+        raise ValueError(f"target_probs has {rows} rows for {T} nodes")
+    stride, last = target_probs.stride()
+    if last != 1 and V > 1:
+        target_probs, stride = target_probs.contiguous(), V
+    draft_stride = draft_rows = 0
     if draft_probs is not None:
-        draft_probs = _rows(draft_probs, "draft_probs", dtype, V)
-        if not max(0, T - B) <= draft_probs.shape[0] <= T:
-            raise ValueError(f"draft_probs has {draft_probs.shape[0]} rows for {T} nodes of {B} "
-                             "chains: one for each drafted token")
+        shape = draft_probs.shape
+        if len(shape) != 2 or shape[1] != V or draft_probs.dtype != dtype:
+            raise ValueError(f"draft_probs must be (rows, {V}) of {dtype}; got {tuple(shape)} "
+                             f"{draft_probs.dtype}")
+        draft_rows = shape[0]
+        if not max(0, T - B) <= draft_rows <= T:
+            raise ValueError(f"draft_probs has {draft_rows} rows for {T} nodes of {B} chains: one "
+                             "for each drafted token")
+        draft_stride, last = draft_probs.stride()
+        if last != 1 and V > 1:
+            draft_probs, draft_stride = draft_probs.contiguous(), V
     for t, name, n in ((uniforms, "uniforms", T), (final_uniforms, "final_uniforms", B)):
         if t.shape != (n,) or t.dtype != torch.float32:
             raise ValueError(f"{name} must be ({n},) float32; got {tuple(t.shape)} {t.dtype}")
     uniforms, final_uniforms = uniforms.contiguous(), final_uniforms.contiguous()
-    dev = target_probs.device
-    got = _outputs(B, max_q_len, dev)
+    got = _outputs(B, max_q_len, target_probs)
     if not T:
         return DraftVerdict(got[0].zero_(), got[1].fill_(-1), got[2].fill_(-1))
     need = _ws_bytes(B, V)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = target_probs.new_empty(need, dtype=torch.uint8)
     with _lib.on_device(target_probs):
         _lib.check(_lib.calls().dsp_verify_draft(
-            tokens.data_ptr(), _lib.ptr(parents), target_probs.data_ptr(), target_probs.stride(0),
-            T, _lib.ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0),
-            0 if draft_probs is None else draft_probs.shape[0], uniforms.data_ptr(),
+            tokens.data_ptr(), _lib.ptr(parents), target_probs.data_ptr(), stride, T,
+            _lib.ptr(draft_probs), draft_stride, draft_rows, uniforms.data_ptr(),
             final_uniforms.data_ptr(), cu_q.data_ptr(), B, max_q_len, V, _lib.dtype_code(dtype),
             ws.data_ptr(), need, got[0].data_ptr(), got[1].data_ptr(), got[2].data_ptr(),
             _lib.ptr(err), _lib.stream_of(target_probs)), "dsp_verify_draft")
@@ -152,11 +149,10 @@ def match_draft(draft_tokens, target_tokens, cu_q, parents=None, max_q_len=None)
 
     draft_tokens, target_tokens: (T,) int32 / int64; cu_q, parents, max_q_len: as there
     """
-    _lib.require_gpu(draft_tokens, target_tokens, cu_q, parents)
-    _lib.same_device(draft_tokens, target_tokens, cu_q, parents)
+    _lib.one_gpu(draft_tokens, target_tokens, cu_q, parents)
     tokens, cu_q, parents, T, B, max_q_len = _layout(draft_tokens, cu_q, parents, max_q_len)
     target_tokens = _ints(target_tokens, "target_tokens", T)
-    got = _outputs(B, max_q_len, tokens.device)
+    got = _outputs(B, max_q_len, tokens)
     if not T:
         return DraftVerdict(got[0].zero_(), got[1].fill_(-1), got[2].fill_(-1))
     with _lib.on_device(tokens):

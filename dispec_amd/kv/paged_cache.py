@@ -75,8 +75,7 @@ def commit_path(key, value, block_table, cu_q, ctx_lens, path, num_accepted, blo
     err:          optional int32 device counter of slots outside the pool and of paths that do not
                   go down a tree (from there on nothing is moved)
     """
-    _lib.require_gpu(key, value, block_table, cu_q, ctx_lens, path, num_accepted, err)
-    _lib.same_device(key, value, block_table, cu_q, ctx_lens, path, num_accepted, err)
+    _lib.one_gpu(key, value, block_table, cu_q, ctx_lens, path, num_accepted, err)
     shape, stride = key.shape, key.stride()
     if len(shape) != 4 or value.shape != shape or value.dtype != key.dtype:
         raise ValueError(f"expected pools (L, slots, KVH, D) of one shape and dtype; got "
