@@ -352,3 +352,40 @@ def test_runs_longer_than_the_ids_held(hip, dtype, D):
                 if dtype == F16:
                     bound = bound + 2.0 ** -25 * ctx * np.abs(vv).max()
                 assert (np.abs(got[b * n + i, h] - o) <= bound).all(), (b, i, h)
+
+
+@pytest.mark.parametrize("dtype,KVH,G,D,top", [(BF16, 8, 1, 64, 500), (BF16, 8, 2, 64, 1700),
+                                               (F16, 8, 1, 128, 1300), (BF16, 2, 3, 256, 900)])
+def test_many_sequences(hip, dtype, KVH, G, D, top):
+    """More tiles than workgroups fit the chip: each has several, some of them cut; sequences
+    without nodes and with a few tokens among them."""
+    rng = random.Random(top)
+    B = 600 // KVH if D < 256 else 140
+    ctx = [rng.choice((1, 2, 17, rng.randint(1, top), rng.randint(top // 2, top))) for _ in range(B)]
+    ctx[rng.randrange(B)] = top
+    q_lens = [min(c, rng.choice((0, 1, 1, 2, 5))) for c in ctx]
+    c = Case(q_lens, ctx, KVH * G, KVH, D, dtype, seed=top)
+    c.check(c.call(), what=f"{B} sequences")
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_batches(hip, seed):
+    """Shapes, lengths, block sizes and masks at random."""
+    rng = random.Random(900 + seed)
+    dtype = rng.choice((BF16, F16))
+    D, KVH, G = rng.choice((64, 64, 128, 128, 256)), rng.choice((1, 2, 3)), rng.choice((1, 2, 5, 7, 8))
+    B, bs = rng.randint(1, 7), rng.choice((16, 16, 32, 128))
+    q_lens, ctx = [], []
+    for _ in range(B):
+        n = rng.choice((0, 1, rng.randint(2, 20), rng.randint(20, 100)))
+        q_lens.append(n)
+        ctx.append(n + rng.choice((0, 0, rng.randint(0, 64), rng.randint(0, 3000))))
+    ctx = [max(x, 1) for x in ctx]
+    if not sum(q_lens):
+        q_lens[0] = 1
+    masks = np.random.default_rng(seed)
+    see = [masks.random((n, n)) < 0.5 for n in q_lens] if seed % 3 == 0 else None
+    c = Case(q_lens, ctx, KVH * G, KVH, D, dtype, seed=seed, bs=bs, see=see)
+    out = torch.full((c.dq.shape[0] + 3, *c.dq.shape[1:]), 7.0, dtype=dtype, device=DEV)
+    c.check(c.call(out=out[:-3]), what=f"{dtype} {KVH}x{G}x{D} {q_lens} {ctx} blocks of {bs}")
+    assert bool((out[-3:] == 7.0).all())
