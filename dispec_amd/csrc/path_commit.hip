@@ -9,6 +9,9 @@
 // rows move in order.  One thread takes one 16-byte column of a (sequence, layer, K or V) through
 // all of its rows, so nothing but its own program order is needed: kBatch rows are read before the
 // first of them is written.  Rows in their place already are not touched.
+// What it reads and writes, and a chain of four loads before it (the path, the table's ids, the
+// rows): 32 trees that keep up to 8 nodes, 36 layers of 8 heads of 128 in bf16, 8.8 us; one tree in
+// 24 layers of 2 heads of 64 3.5 us.
 #include "dsp_common.h"
 
 namespace {

@@ -20,9 +20,12 @@
 //    workgroups resident on the chip, computed on the device from the lengths; a tile's start counts
 //    as kStart chunks.  A tile inside a run is written; a tile that runs cut leaves its rows'
 //    maximum, sum and accumulator per piece, and the second launch merges them.
-//  * What bounds it, heads of 128 in bf16: 32 trees of 16 nodes (G 2, 500 to 4000 tokens, 321 MB) 81
-//    us, where the loads alone take 79; 4 trees of 64 (G 4, 32768 tokens) 205 us, 670 TFLOP/s: two
-//    waves a SIMD issue for 74 % of the time, what they compute runs on the matrix cores for 38 %.
+//  * What bounds it, heads of 128 in bf16: 32 trees of 16 nodes (G 2, 500 to 4000 tokens, 321 MB) 63
+//    us and 6 of merge: 5.1 TB/s, 8 us of it until the first keys are there.  4 trees of 64 (G 4,
+//    32768 tokens) 167 us and 8 of merge, 820 TFLOP/s (205 to 227 after a millisecond: the clock
+//    falls): two waves a SIMD issue for 74 % of the time, the matrix cores are busy for 38 %.  24
+//    trees of 1 to 33 nodes (40 to 3001 tokens) 25 us and 7: 5 chunks of 1.8 us a workgroup behind
+//    the chain lengths, block ids, first keys.
 // Everything else (fp32 caches, other head dims, blocks of fewer than 16 tokens, rows off 16 bytes,
 // a scale that is not positive) runs on the kernels of generic_attn.hip with the same masks.
 #include <float.h>
@@ -142,8 +145,8 @@ __device__ __forceinline__ int wave_incl_scan(int v) {
   return v;
 }
 
-// The shape of a tile: kNW waves of 32 rows, and buffers of a chunk's K and V: 128 KiB of them on a CU,
-// for kPerCU workgroups.
+// The shape of a tile: kNW waves of 32 rows, and buffers of a chunk's K and V: 128 KiB of them on a
+// CU, for kPerCU workgroups.
 template <int kNW, int kPerCU>
 struct Shape {
   static constexpr int NW = kNW, TR = 32 * kNW;
@@ -362,9 +365,9 @@ tree_tile_kernel(
       for (int i = threadIdx.x; i < n; i += 64 * NW) s_blk[i] = bt[bt_row + blk0 + i];
       __syncthreads();
     };
-    // This wave's RPW rows of a chunk lie in one block.  A chunk's K is sent for one stage ahead of its
-    // V: the rows' offset is kept in between, the next chunk's id read from LDS a stage ahead.  (All
-    // uniform.)
+    // This wave's RPW rows of a chunk lie in one block.  A chunk's K is sent for one stage ahead of
+    // its V: the rows' offset is kept in between, the next chunk's id read from LDS a stage ahead.
+    // (All uniform.)
     const char* const kbase = reinterpret_cast<const char*>(kc + int64_t(kvh) * kvs_head);
     const char* const vbase = reinterpret_cast<const char*>(vc + int64_t(kvh) * kvs_head);
     uint64_t rows_off = 0;          // of the chunk whose K was sent for last; its id is bad
@@ -922,7 +925,8 @@ int launch_tree(const TreePlan& p, const uint16_t* q, int64_t qst, int64_t qsh, 
     tree_tile_kernel<Tag, D, S><<<p.workers, 64 * S::NW, 0, s>>>(
         q, qst, qsh, kc, vc, uint32_t(num_slots >> log2_bs), int32_t(kvs_slot), kvs_head, bt,
         bt_stride, log2_bs, cu_q, ctx_lens, mask, words, B, KVH, G, max_q_len, max_ctx, scale_log2,
-        p.whole, p.least, stream_units, p.tiles_max, ws, ws_ml, ws_desc, out, ost, osh, vec_out, err_count);
+        p.whole, p.least, stream_units, p.tiles_max, ws, ws_ml, ws_desc, out, ost, osh, vec_out,
+        err_count);
   };
   if constexpr (D <= 128) {
     if (p.rows == 256) launch(Shape<8, 1>{});

@@ -301,9 +301,9 @@ class ModelRunner:
         (model_runner.py:160-185) -- the sequence's context rows gathered from the pool
         (the prologue has already appended this step's k and v, so a fresh prefill reads
         back exactly the rows it projected), then torch SDPA with the bottom-right causal
-        mask (a drafted tree's nodes: their ancestors) and grouped KV heads.  SDPA runs in float32: torch's bf16 batched matmul on
-        the transposed key operand SDPA forms is avoided on this platform; the output is
-        rounded to the model dtype."""
+        mask (a drafted tree's nodes: their ancestors) and grouped KV heads.  SDPA runs in
+        float32: torch's bf16 batched matmul on the transposed key operand SDPA forms is
+        avoided on this platform; the output is rounded to the model dtype."""
         from torch.nn.attention.bias import causal_lower_right
         out = torch.empty_like(q)
         end = 0

@@ -247,18 +247,18 @@ def test_sampled_step_keeps_what_the_verdict_says(dtype, with_draft):
     assert new == [n for _, n in want]
     assert max(len(x) for x in new) >= 3
     # the forward above ran other tokens where the likeliest replaced them: run the step again with
-    # the tokens that were judged, so that the cache holds theirs
+    # the tokens that were taken, so that the cache holds theirs
     e2, plain = Engine(model, dtype), Engine(model, dtype)
     e2.forward(first)
-    at, judged = 0, []
+    at, taken = 0, []
     for b, ids, par in rows:
-        judged.append((b, tokens[at:at + len(ids)], par))
+        taken.append((b, tokens[at:at + len(ids)], par))
         at += len(ids)
-    e2.forward(judged)
-    e2.keep(judged, verdict)
+    e2.forward(taken)
+    e2.keep(taken, verdict)
     plain.forward(first)
     plain.forward([(b, [tok[i] for i in path], None)
-                   for (b, tok, _), (path, _) in zip(judged, want)])
+                   for (b, tok, _), (path, _) in zip(taken, want)])
     step = [(b, [n[-1]], None) for b, (_, n) in enumerate(want)]
     got, ref = e2.forward(step), plain.forward(step)
     cos = torch.nn.functional.cosine_similarity(got, ref, dim=-1)
