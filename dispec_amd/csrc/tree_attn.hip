@@ -42,7 +42,9 @@ namespace {
 using namespace dsp_mfma;
 
 constexpr int kChunk = 64;     // keys per chunk
-constexpr int kMinChunks = 2;  // a workgroup gets at least this many chunks
+// A workgroup gets at least this many chunks: 4 heads of 63 26 us (29 with 1, 25.9 with 4), 2 of 16 13.2
+// (12.3 with 1, 15.1 with 4).
+constexpr int kMinChunks = 2;
 // What a run spends on a tile beside its chunks (ids, q, the pipeline's first loads, a partial result
 // or the output), in chunks: every tile counts as so many more when the list is cut.  32 sequences
 // of 500 to 4000 tokens, 8 KV heads, D 128, 256 and 512 rows a head: 160 and 269 us (counted as
@@ -891,11 +893,21 @@ TreePlan tree_plan(int32_t B, int32_t KVH, int32_t G, int32_t D, int32_t max_q_l
   p.tile = max_ctx < (1 << 24) && rows < (1 << 24) && per_head * units * KVH < (1 << 24) &&
            tiles * units < (int64_t(1) << 31);
   if (!p.tile) return p;
-  p.whole = chunks <= 8;
-  p.least = p.whole ? 1 : kMinChunks;
   // workgroups that fit the chip at once (LDS)
   const int64_t slots = int64_t(dsp_detail::device_cus()) * (p.rows == 128 && D <= 128 ? 2 : 1);
-  p.workers = int(std::min((p.whole ? tiles : (tiles * units + p.least - 1) / p.least), slots));
+  // Short contexts: tiles stay whole where that costs less, in chunks, than equal runs, a start each
+  // and the merge (its launch 3, its partial results 2 where there are as many as fit; half of all
+  // that at D 256, whose chunks take twice the time).  The lengths are bounds here: only up to 16
+  // chunks.  Whole against cut, heads of 128: 512 tiles of 200 to 500 tokens 26.9 us (36.0), of 300
+  // to 1000 42.7 (46.5), 128 tiles 19.3 (20.4) and 28.8 (24.3); heads of 64, 2 tiles of 300 tokens
+  // 12.2 (12.3), of 500 16.1 (13.1), of 1000 24.7 (13.2); of 256, 64 tiles of 200 to 500 34.2 (27.6).
+  const int64_t runs = std::min((tiles * units + kMinChunks - 1) / kMinChunks, slots);
+  const int64_t share = std::max((tiles * units + slots - 1) / slots, int64_t(kMinChunks));
+  p.whole = chunks <= 16 &&
+            (tiles + slots - 1) / slots * units <=
+                share + (kStart + 3 + 2 * runs / slots) / (D > 128 ? 2 : 1);
+  p.least = p.whole ? 1 : kMinChunks;
+  p.workers = int(p.whole ? std::min(tiles, slots) : runs);
   p.tiles_max = tiles <= p.workers ? int(per_head) : 0;
   p.items = tiles <= p.workers ? int(tiles) : p.workers;
   return p;
