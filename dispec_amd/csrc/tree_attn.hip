@@ -169,9 +169,10 @@ __device__ __forceinline__ void wait_chunks(int n) {
   }
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 template <typename Tag>
 __device__ __forceinline__ uint32_t narrow2(float a, float b) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
   if constexpr (std::is_same<Tag, Bf16Tag>::value)
@@ -768,7 +769,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
     const int32_t* __restrict__ ws_desc, const int32_t* __restrict__ cu_q,
     const int32_t* __restrict__ ctx_lens, int32_t items, int32_t groups, int32_t KVH, int32_t G,
     int32_t max_q_len, int32_t max_ctx, int32_t tiles_max, int32_t tile_rows,
-    uint16_t* __restrict__ out, int64_t ost, int64_t osh) {
+    uint16_t* __restrict__ out, int64_t ost, int64_t osh, int32_t vec_out) {
   constexpr int TPR = D / 4, R = tree_merge_rows(D, kSplit), kBatch = 8;
   __shared__ float s_acc[kSplit][R][D];
   __shared__ float s_ml[kSplit][R][2];
@@ -799,7 +800,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
     if (np <= 0) return;
   }
   const int lr = group * R + threadIdx.x / TPR % R, d = 4 * (threadIdx.x % TPR);
-  const int split = threadIdx.x / (TPR * R);
+  const int split = kSplit == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (TPR * R));
+  static_assert(kSplit == 1 || TPR * R == 64, "a wave's pieces");
   const int r = tile * tile_rows + lr;
   if (tile * tile_rows + group * R >= rows || np <= 0) return;  // (uniform)
   const bool live = lr < tile_rows && r < rows;
@@ -808,29 +810,31 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
   if (live)
     for (int p0 = split; p0 < np; p0 += kSplit * kBatch) {
       f32x4 va[kBatch];
-      float vm[kBatch], vl[kBatch];
+      f32x2 ml[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int p = min(p0 + kSplit * i, np - 1);  // (past the last: again, for nothing)
-        const int64_t row = (p == 0 ? 2 * w + 1 : 2 * (w + p)) * tile_rows + lr;
-        va[i] = *reinterpret_cast<const f32x4*>(ws_acc + row * D + d);
-        vm[i] = ws_ml[2 * row];
-        vl[i] = ws_ml[2 * row + 1];
+        const int p = p0 + kSplit * i;
+        va[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        ml[i] = f32x2{-INFINITY, 0.f};
+        if (p < np) {  // (uniform: no load for nothing)
+          const int64_t row = (p == 0 ? 2 * w + 1 : 2 * (w + p)) * tile_rows + lr;
+          va[i] = *reinterpret_cast<const f32x4*>(ws_acc + row * D + d);
+          ml[i] = *reinterpret_cast<const f32x2*>(ws_ml + 2 * row);
+        }
       }
       float bm = M;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) bm = fmaxf(bm, vm[i]);
+      for (int i = 0; i < kBatch; ++i) bm = fmaxf(bm, ml[i][0]);
       const float Mu = bm == -INFINITY ? 0.f : bm;
       const float keep = dsp_exp2(M - Mu);
       L *= keep;
       A *= keep;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const float x = p0 + kSplit * i < np ? dsp_exp2(vm[i] - Mu) : 0.f;
-        const bool in = p0 + kSplit * i < np;
-        L = fmaf(in ? vl[i] : 0.f, x, L);
+        const float x = dsp_exp2(ml[i][0] - Mu);
+        L = fmaf(ml[i][1], x, L);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) A[e] = fmaf(in ? va[i][e] : 0.f, x, A[e]);
+        for (int e = 0; e < 4; ++e) A[e] = fmaf(va[i][e], x, A[e]);
       }
       M = bm;
     }
@@ -862,8 +866,16 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int qi = r / G;
   uint16_t* o = out + int64_t(q0 + qi) * ost + int64_t(kvh * G + r - qi * G) * osh + d;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = narrow<Tag>(A[e] * inv);
+  const uint32_t lo = narrow2<Tag>(A[0] * inv, A[1] * inv);
+  const uint32_t hi = narrow2<Tag>(A[2] * inv, A[3] * inv);
+  if (vec_out) {
+    *reinterpret_cast<dsp_u32x2*>(o) = dsp_u32x2{lo, hi};
+  } else {
+    o[0] = uint16_t(lo);
+    o[1] = uint16_t(lo >> 16);
+    o[2] = uint16_t(hi);
+    o[3] = uint16_t(hi >> 16);
+  }
 }
 
 // ---- which launch a shape takes
@@ -956,7 +968,7 @@ int launch_tree(const TreePlan& p, const uint16_t* q, int64_t qst, int64_t qsh, 
     tree_merge_kernel<Tag, D, kSplit>
         <<<unsigned((int64_t(p.items) * groups + 7) / 8 * 8), 256, 0, s>>>(
             ws, ws_ml, ws_desc, cu_q, ctx_lens, p.items, groups, KVH, G, max_q_len, max_ctx,
-            p.tiles_max, p.rows, out, ost, osh);
+            p.tiles_max, p.rows, out, ost, osh, vec_out);
   };
   // an item's pieces shared by four threads where there are many: 32 pieces 28.9 us a call (33.9 by
   // one thread), 5 pieces 38.5 (34.1)
