@@ -21,10 +21,10 @@
 //    as kStart chunks.  A tile inside a run is written; a tile that runs cut leaves its rows'
 //    maximum, sum and accumulator per piece, and the second launch merges them.
 //  * What bounds it, heads of 128 in bf16: 32 trees of 16 nodes (G 2, 500 to 4000 tokens, 321 MB) 63
-//    us and 6 of merge: 5.1 TB/s, 8 us of it until the first keys are there.  4 trees of 64 (G 4,
+//    us and 5 of merge: 5.1 TB/s, 5 us of it until the first keys are there.  4 trees of 64 (G 4,
 //    32768 tokens) 167 us and 8 of merge, 820 TFLOP/s (205 to 227 after a millisecond: the clock
 //    falls): two waves a SIMD issue for 74 % of the time, the matrix cores are busy for 38 %.  24
-//    trees of 1 to 33 nodes (40 to 3001 tokens) 25 us and 7: 5 chunks of 1.8 us a workgroup behind
+//    trees of 1 to 33 nodes (40 to 3001 tokens) 25 us and 6: 5 chunks of 1.8 us a workgroup behind
 //    the chain lengths, block ids, first keys.
 // Everything else (fp32 caches, other head dims, blocks of fewer than 16 tokens, rows off 16 bytes,
 // a scale that is not positive) runs on the kernels of generic_attn.hip with the same masks.
@@ -760,7 +760,7 @@ tree_tile_kernel(
 // piece), its pieces loaded 8 at a time; the kSplit threads' results meet in LDS.  Neighbours in
 // the grid are the row groups of one item; the runs that begin a tile often lie a multiple of 8
 // apart, so the groups of every next 8 items start one XCD further (all of one XCD's: 47 us instead
-// of 15 at 32 tiles of 256 rows in 8 pieces).
+// of 15 at 32 tiles of 256 rows in 8 pieces).  256 tiles of 128 rows in 2 to 3 pieces, 45 MB: 11.8 us.
 constexpr int tree_merge_rows(int D, int split) { return 1024 / D / split; }
 
 template <typename Tag, int D, int kSplit>
