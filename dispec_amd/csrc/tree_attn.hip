@@ -543,10 +543,11 @@ tree_tile_kernel(
       return __builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0;
     };
     // The running maximum moves only then (p <= 2^8 otherwise): the sum and the accumulators share
-    // it, so the result is the same.
+    // it, so the result is the same.  The factor stays above 0: the accumulators may hold an
+    // infinity, also of a key whose score is yet to come (take_odd), and 0 * inf is NaN.
     auto rescale = [&]() -> float {
       const float m_new = fmaxf(m, mx);
-      const float alpha = m_new == -INFINITY ? 1.f : dsp_exp2(m - m_new);
+      const float alpha = fmaxf(dsp_exp2(m - m_new), 0x1p-126f);  // (-inf - -inf: 2^-126 of zeros)
       m = m_new;
       lpart *= alpha;
 #pragma unroll
@@ -763,6 +764,12 @@ tree_tile_kernel(
 // of 15 at 32 tiles of 256 rows in 8 pieces).  256 tiles of 128 rows in 2 to 3 pieces, 45 MB: 11.8 us.
 constexpr int tree_merge_rows(int D, int split) { return 1024 / D / split; }
 
+// 2^x for a piece whose maximum lies x <= 0 from the row's, above 0 so that an infinity in its sums
+// stays one; 0 for a piece without keys (x = -inf).  (NaN: both maxima infinite, NaN sums.)
+__device__ __forceinline__ float piece_weight(float x) {
+  return x < -126.f ? (x == -INFINITY ? 0.f : 0x1p-126f) : dsp_exp2(x);
+}
+
 template <typename Tag, int D, int kSplit>
 __global__ __launch_bounds__(256) void tree_merge_kernel(
     const float* __restrict__ ws_acc, const float* __restrict__ ws_ml,
@@ -826,12 +833,12 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) bm = fmaxf(bm, ml[i][0]);
       const float Mu = bm == -INFINITY ? 0.f : bm;
-      const float keep = dsp_exp2(M - Mu);
+      const float keep = piece_weight(M - Mu);
       L *= keep;
       A *= keep;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const float x = dsp_exp2(ml[i][0] - Mu);
+        const float x = piece_weight(ml[i][0] - Mu);
         L = fmaf(ml[i][1], x, L);
 #pragma unroll
         for (int e = 0; e < 4; ++e) A[e] = fmaf(va[i][e], x, A[e]);
@@ -850,12 +857,12 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
     float bm = M;
 #pragma unroll
     for (int i = 1; i < kSplit; ++i) bm = fmaxf(bm, s_ml[i][at][0]);
-    const float Mu = bm == -INFINITY ? 0.f : bm, keep = dsp_exp2(M - Mu);
+    const float Mu = bm == -INFINITY ? 0.f : bm, keep = piece_weight(M - Mu);
     L *= keep;
     A *= keep;
 #pragma unroll
     for (int i = 1; i < kSplit; ++i) {
-      const float x = dsp_exp2(s_ml[i][at][0] - Mu);
+      const float x = piece_weight(s_ml[i][at][0] - Mu);
       const f32x4 o = *reinterpret_cast<const f32x4*>(&s_acc[i][at][d]);
       L = fmaf(s_ml[i][at][1], x, L);
 #pragma unroll
