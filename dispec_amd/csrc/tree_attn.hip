@@ -517,7 +517,8 @@ tree_tile_kernel(
                              kbeg + c * kChunk + 32 * x - tree0) >> (4 * hl);
     };
     // Half x of chunk c: keys that count for nothing (kflags: the flags that came with its K), and
-    // whether a row's maximum exceeds the running one by more than 2^8; mx: the half's, base 2.
+    // whether a row's maximum exceeds the running one by more than 2^kLag; mx: the half's, base 2.
+    constexpr float kLag = 8.f;
     float mx = 0.f;
     auto settle = [&](int c, int x, int kflags, f32x16& sc) -> bool {
       if (kbeg + (c + 1) * kChunk > tree0) {
@@ -540,14 +541,16 @@ tree_tile_kernel(
 #pragma unroll
       for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[j]);
       mx = fmaxf(mx, dsp_shfl_xor(mx, 32)) * scale_log2;  // -inf stays -inf
-      return __builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0;
+      return __builtin_amdgcn_ballot_w64(mx > m + kLag) != 0;
     };
-    // The running maximum moves only then (p <= 2^8 otherwise): the sum and the accumulators share
-    // it, so the result is the same.  The factor stays above 0: the accumulators may hold an
+    // The running maximum of such a row moves (p <= 2^8 otherwise): the sum and the accumulators
+    // share it, so the result is the same.  Other rows of the wave keep theirs: what a row gives
+    // does not depend on its neighbours.  The factor stays above 0: the accumulators may hold an
     // infinity, also of a key whose score is yet to come (take_odd), and 0 * inf is NaN.
     auto rescale = [&]() -> float {
-      const float m_new = fmaxf(m, mx);
-      const float alpha = fmaxf(dsp_exp2(m - m_new), 0x1p-126f);  // (-inf - -inf: 2^-126 of zeros)
+      const bool moves = mx > m + kLag;
+      const float m_new = moves ? mx : m;
+      const float alpha = moves ? fmaxf(dsp_exp2(m - m_new), 0x1p-126f) : 1.f;
       m = m_new;
       lpart *= alpha;
 #pragma unroll
@@ -630,7 +633,8 @@ tree_tile_kernel(
       }
       __builtin_amdgcn_sched_barrier(0);
       if (settle(c, cx, kfl, cur)) {
-        // the probabilities that still wait for their P V move along, rounded once more
+        // the probabilities that still wait for their P V move along, rounded once more (the
+        // factor is below 2^-8 where it is not 1, and so is what that adds to the row's error)
         const float alpha = rescale();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
