@@ -10,8 +10,8 @@
 //
 // Tile (16-bit caches): NW waves of 32 packed rows each (row r: query r / G of head kvh G + r % G)
 // share 64-key chunks of K and V that the LDS DMA brings in; S^T = K Q^T and O^T = V^T P^T on
-// v_mfma_f32_32x32x16, with P in registers (dsp_tile32.h), a running maximum that moves when it is
-// exceeded by 2^8, sums and accumulators in fp32.  The probabilities enter P V as one 16-bit operand
+// v_mfma_f32_32x32x16, with P in registers (dsp_tile32.h), a row's running maximum that moves when it
+// is exceeded by 2^8, sums and accumulators in fp32.  The probabilities enter P V as one 16-bit operand
 // (rounded to nearest; the sum takes the unrounded ones): half a step of the type, as much as the
 // output's own rounding.
 //  * Two workgroups of 4 waves (128 rows) to a CU for up to 128 rows a KV head, one of 8 waves (256
@@ -518,7 +518,10 @@ tree_tile_kernel(
     };
     // Half x of chunk c: keys that count for nothing (kflags: the flags that came with its K), and
     // whether a row's maximum exceeds the running one by more than 2^kLag; mx: the half's, base 2.
-    constexpr float kLag = 8.f;
+    // What m holds is the running maximum less kRef: fp16's least number is 2^-24, bf16's far below,
+    // so fp16 operands go up to 2^15 and end at 2^-31 of a row's largest probability (without it a
+    // tail of keys below 2^-25 of a row's first key counted for nothing).
+    constexpr float kLag = 8.f, kRef = std::is_same<Tag, F16Tag>::value ? 7.f : 0.f;
     float mx = 0.f;
     auto settle = [&](int c, int x, int kflags, f32x16& sc) -> bool {
       if (kbeg + (c + 1) * kChunk > tree0) {
@@ -541,15 +544,15 @@ tree_tile_kernel(
 #pragma unroll
       for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[j]);
       mx = fmaxf(mx, dsp_shfl_xor(mx, 32)) * scale_log2;  // -inf stays -inf
-      return __builtin_amdgcn_ballot_w64(mx > m + kLag) != 0;
+      return __builtin_amdgcn_ballot_w64(mx > m + (kRef + kLag)) != 0;
     };
-    // The running maximum of such a row moves (p <= 2^8 otherwise): the sum and the accumulators
+    // The running maximum of such a row moves (p <= 2^kLag otherwise): the sum and the accumulators
     // share it, so the result is the same.  Other rows of the wave keep theirs: what a row gives
     // does not depend on its neighbours.  The factor stays above 0: the accumulators may hold an
     // infinity, also of a key whose score is yet to come (take_odd), and 0 * inf is NaN.
     auto rescale = [&]() -> float {
-      const bool moves = mx > m + kLag;
-      const float m_new = moves ? mx : m;
+      const bool moves = mx > m + (kRef + kLag);
+      const float m_new = moves ? mx - kRef : m;
       const float alpha = moves ? fmaxf(dsp_exp2(m - m_new), 0x1p-126f) : 1.f;
       m = m_new;
       lpart *= alpha;
