@@ -122,6 +122,11 @@ __device__ __forceinline__ float dsp_shfl_xor(float x, int mask) {
 
 __device__ __forceinline__ float dsp_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// 2^x, x <= 0, kept above 0, so that an infinity that it weighs stays one; 0 for x = -inf (no key).
+__device__ __forceinline__ float dsp_weight(float x) {
+  return dsp_exp2(x) + (x > -INFINITY ? 0x1p-126f : 0.f);
+}
+
 // Which of the 32 keys from one on a tree's query sees (bit i: key i): all before the tree, and of
 // the tree's n nodes those of its mask, `words` 32-bit words at `row`.  a: the first key's node
 // (negative: so many keys before the tree).  Bits past the mask or the tree are 0.

@@ -102,6 +102,13 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v + dsp_shfl_xor(v, 32);
 }
 
+// The weight of a key or a part.  kTree: above 0 where there is one (an infinity in V of a key that a
+// row sees gives an infinity, however small the key's probability).
+template <bool kTree>
+__device__ __forceinline__ float weight(float x) {
+  return kTree ? dsp_weight(x) : dsp_exp2(x);
+}
+
 template <typename Tag, int D, bool kTree>
 __global__ __launch_bounds__(64) void generic_attn_kernel(
     const typename Tag::store* __restrict__ q, int64_t qst, int64_t qsh,
@@ -181,13 +188,13 @@ __global__ __launch_bounds__(64) void generic_attn_kernel(
       mx = fmaxf(mx, s[u]);
     }
     const float mu = mx == -INFINITY ? 0.f : mx;
-    const float alpha = dsp_exp2(m - mu);
+    const float alpha = weight<kTree>(m - mu);
     l *= alpha;
 #pragma unroll
     for (int j = 0; j < NV; ++j) acc[j] *= alpha;
 #pragma unroll
     for (int u = 0; u < kKeysPerStep; ++u) {
-      const float p = dsp_exp2(s[u] - mu);
+      const float p = weight<kTree>(s[u] - mu);
       l += p;
 #pragma unroll
       for (int j = 0; j < NV; ++j) acc[j] = fmaf(p, vv[u][j], acc[j]);
@@ -368,14 +375,14 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
     mx = fmaxf(mx, dsp_shfl_xor(mx, 16));
     mx = fmaxf(mx, dsp_shfl_xor(mx, 32));
     const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
-    const float alpha = dsp_exp2(m - mu);
+    const float alpha = weight<kTree>(m - mu);
     m = mn;
     l *= alpha;
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] *= alpha;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      p[j] = dsp_exp2(p[j] - mu);
+      p[j] = weight<kTree>(p[j] - mu);
       l += p[j];
     }
     if (t0 + 16 > vis0) {  // a chunk that the tile's first row does not see whole (uniform)
@@ -456,7 +463,7 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
     float L = 0.f, A = 0.f;
 #pragma unroll
     for (int w = 0; w < kTileWaves; ++w) {
-      const float x = dsp_exp2(s_m[w][rr] - Mu);
+      const float x = weight<kTree>(s_m[w][rr] - Mu);
       L = fmaf(s_l[w][rr], x, L);
       A = fmaf(s_acc[w][rr][d], x, A);
     }
@@ -512,13 +519,13 @@ __global__ __launch_bounds__(256) void generic_merge_kernel(
 #pragma unroll
     for (int u = 0; u < kMergeBatch; ++u) bm = fmaxf(bm, vm[u]);
     const float bmu = bm == -INFINITY ? 0.f : bm;
-    const float keep = dsp_exp2(M - bmu);
+    const float keep = weight<kTree>(M - bmu);
     L *= keep;
 #pragma unroll
     for (int j = 0; j < NV; ++j) A[j] *= keep;
 #pragma unroll
     for (int u = 0; u < kMergeBatch; ++u) {
-      const float w = dsp_exp2(vm[u] - bmu);
+      const float w = weight<kTree>(vm[u] - bmu);
       L = fmaf(vl[u], w, L);
 #pragma unroll
       for (int j = 0; j < NV; ++j) A[j] = fmaf(va[u][j], w, A[j]);

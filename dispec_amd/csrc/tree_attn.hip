@@ -181,6 +181,18 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
 }
 
+// Of each of two operands' 16-bit numbers, not negative (or NaN, the largest here), the larger and
+// the smaller.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t not_below(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ uint32_t not_above(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
+}
+
 template <typename Tag>
 __device__ __forceinline__ float low(uint32_t two) {
   return std::is_same<Tag, Bf16Tag>::value ? dsp_bf16lo(two) : dsp_f16lo(two);
@@ -567,12 +579,18 @@ tree_tile_kernel(
       lpart += p;
       return p;
     };
-    auto probs = [&](const f32x16& sc, dsp_u32x4 (&pop)[2]) {
+    // Of a chunk before the tree, which every row sees, an operand is kept above 0 (kLeast: 2^-31 of
+    // the row's largest probability in fp16, 2^-126 in bf16), so that an infinity in V meets a
+    // positive factor.  (Keys with a bad block id: V is zeros.  A chunk that holds nodes: take_odd.)
+    constexpr uint32_t kLeast = std::is_same<Tag, F16Tag>::value ? 0x00010001u : 0x00800080u;
+    auto least_of = [&](int c) { return kbeg + (c + 1) * kChunk > tree0 ? 0u : kLeast; };
+    auto probs = [&](int c, const f32x16& sc, dsp_u32x4 (&pop)[2]) {
+      const uint32_t least = least_of(c);
       const float neg_m = m == -INFINITY ? 0.f : -m;
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {
         const float p0 = prob(sc, j, neg_m), p1 = prob(sc, j + 1, neg_m);
-        pop[j >> 3][(j >> 1) & 3] = narrow2<Tag>(p0, p1);
+        pop[j >> 3][(j >> 1) & 3] = not_below(narrow2<Tag>(p0, p1), least);
       }
     };
     // (rare) infinities and NaN of V of chunk c, in buffer buf, to the rows that see them; then they
@@ -608,13 +626,14 @@ tree_tile_kernel(
     constexpr int kSendAt = 1;  // the step of a chunk's first half in which the next stage is sent for
     // A half's exponentials, 1 / NKS of them at a time (step i).
     static_assert(NKS <= 16 && NKS == 2 * NDT, "a step has one exponential or more");
-    auto take_probs = [&](f32x16& sc, int i, float neg_m, dsp_u32x4 (&pop)[2]) {
+    auto take_probs = [&](f32x16& sc, int i, float neg_m, uint32_t least, dsp_u32x4 (&pop)[2]) {
       constexpr int PER = 16 / NKS;
 #pragma unroll
       for (int e = 0; e < PER; ++e) {
         const int j = PER * i + e;
         sc[j] = prob(sc, j, neg_m);
-        if (j & 1) pop[j >> 3][(j >> 1) & 3] = narrow2<Tag>(sc[j - 1], sc[j]);
+        if (j & 1)
+          pop[j >> 3][(j >> 1) & 3] = not_below(narrow2<Tag>(sc[j - 1], sc[j]), least);
       }
     };
     int kflags = s_flag[3];  // (in a vector register until it is looked at)
@@ -642,10 +661,12 @@ tree_tile_kernel(
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const uint32_t two = pop[i >> 2][i & 3];
-          pop[i >> 2][i & 3] = narrow2<Tag>(low<Tag>(two) * alpha, high<Tag>(two) * alpha);
+          pop[i >> 2][i & 3] = not_below(
+              narrow2<Tag>(low<Tag>(two) * alpha, high<Tag>(two) * alpha), not_above(two, kLeast));
         }
       }
       const float neg_m = m == -INFINITY ? 0.f : -m;
+      const uint32_t least = least_of(c);
       dsp_u32x4 fresh[2];
 #pragma unroll
       for (int j = 0; j < 16; ++j) next[j] = 0.f;
@@ -658,7 +679,7 @@ tree_tile_kernel(
         }
         next = mfma32x32<Tag>(kop[i], qop[i], next);
         if (x == 0 && i == kSendAt) send_next(c);
-        take_probs(cur, i, neg_m, fresh);
+        take_probs(cur, i, neg_m, least, fresh);
         __builtin_amdgcn_sched_barrier(0);
         acc[i % NDT] = mfma32x32<Tag>(vop[i], pop[i / NDT], acc[i % NDT]);
       }
@@ -669,7 +690,7 @@ tree_tile_kernel(
     if (wave_has_rows) {
       scores(kFirst, 0, s0);
       if (settle(0, 0, kflags, s0)) rescale();
-      probs(s0, pop);
+      probs(0, s0, pop);
       scores(kFirst, 1, s1);
     }
     for (int c = 0; c < nc; ++c) {
@@ -771,12 +792,6 @@ tree_tile_kernel(
 // of 15 at 32 tiles of 256 rows in 8 pieces).  256 tiles of 128 rows in 2 to 3 pieces, 45 MB: 11.8 us.
 constexpr int tree_merge_rows(int D, int split) { return 1024 / D / split; }
 
-// 2^x for a piece whose maximum lies x <= 0 from the row's, above 0 so that an infinity in its sums
-// stays one; 0 for a piece without keys (x = -inf).  (NaN: both maxima infinite, NaN sums.)
-__device__ __forceinline__ float piece_weight(float x) {
-  return x < -126.f ? (x == -INFINITY ? 0.f : 0x1p-126f) : dsp_exp2(x);
-}
-
 template <typename Tag, int D, int kSplit>
 __global__ __launch_bounds__(256) void tree_merge_kernel(
     const float* __restrict__ ws_acc, const float* __restrict__ ws_ml,
@@ -840,12 +855,12 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) bm = fmaxf(bm, ml[i][0]);
       const float Mu = bm == -INFINITY ? 0.f : bm;
-      const float keep = piece_weight(M - Mu);
+      const float keep = dsp_weight(M - Mu);
       L *= keep;
       A *= keep;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const float x = piece_weight(ml[i][0] - Mu);
+        const float x = dsp_weight(ml[i][0] - Mu);
         L = fmaf(ml[i][1], x, L);
 #pragma unroll
         for (int e = 0; e < 4; ++e) A[e] = fmaf(va[i][e], x, A[e]);
@@ -864,12 +879,12 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(
     float bm = M;
 #pragma unroll
     for (int i = 1; i < kSplit; ++i) bm = fmaxf(bm, s_ml[i][at][0]);
-    const float Mu = bm == -INFINITY ? 0.f : bm, keep = piece_weight(M - Mu);
+    const float Mu = bm == -INFINITY ? 0.f : bm, keep = dsp_weight(M - Mu);
     L *= keep;
     A *= keep;
 #pragma unroll
     for (int i = 1; i < kSplit; ++i) {
-      const float x = piece_weight(s_ml[i][at][0] - Mu);
+      const float x = dsp_weight(s_ml[i][at][0] - Mu);
       const f32x4 o = *reinterpret_cast<const f32x4*>(&s_acc[i][at][d]);
       L = fmaf(s_ml[i][at][1], x, L);
 #pragma unroll

@@ -68,3 +68,23 @@ def test_a_maximum_far_above_an_infinity(hip, dtype, D, later):
     c.dv[int(c.slots[0][3]), 0, 7] = INF
     got = c.call(scale=float(np.log(2.0)))
     _check(c, got, {(i, 0, 7): INF for i in range(n)}, keep)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D", [64, 128, 256, 32])
+@pytest.mark.parametrize("gap", [20.0, 33.0, 60.0, 200.0])
+@pytest.mark.parametrize("ctx,sink,odd", [(300, 10, 100), (300, 100, 10), (300, 297, 40),
+                                          (9000, 8000, 70), (9000, 70, 8000)])
+def test_an_infinity_behind_a_small_probability(hip, dtype, D, gap, ctx, sink, odd):
+    """A key that every row sees, whose probability is 2^-gap of the row's largest."""
+    c = Case([5, 2], [ctx, 20], 4, 2, D, dtype, seed=D + 3, see=[np.ones((5, 5), dtype=bool),
+                                                               np.ones((2, 2), dtype=bool)])
+    c.dk.zero_()
+    c.dk[int(c.slots[0][sink]), :, 0] = gap
+    c.dq[:, :, 0] = 1.0
+    keep = c.call(scale=float(np.log(2.0)))
+    hits = {}
+    for kvh, x in ((0, INF), (1, -INF)):
+        c.dv[int(c.slots[0][odd]), kvh, 3 + kvh] = x
+        hits.update({(i, kvh, 3 + kvh): x for i in range(5)})
+    _check(c, c.call(scale=float(np.log(2.0))), hits, keep)
