@@ -11,9 +11,12 @@
 // Tile (16-bit caches): NW waves of 32 packed rows each (row r: query r / G of head kvh G + r % G)
 // share 64-key chunks of K and V that the LDS DMA brings in; S^T = K Q^T and O^T = V^T P^T on
 // v_mfma_f32_32x32x16, with P in registers (dsp_tile32.h), a row's running maximum that moves when it
-// is exceeded by 2^8, sums and accumulators in fp32.  The probabilities enter P V as one 16-bit operand
-// (rounded to nearest; the sum takes the unrounded ones): half a step of the type, as much as the
-// output's own rounding.
+// is exceeded by 2^8, sums and accumulators in fp32.  Up to 128 dims the probabilities enter P V as
+// one 16-bit operand (rounded to nearest; the sum takes the unrounded ones): half a step of the
+// type, as much as the output's own rounding, and what the other attention kernels do there.  At
+// 256 dims they are three operands, all 24 bits, as in the other attention of such heads, which a
+// tree's batch takes over from: 12 sequences of 16 nodes (G 2, 500 to 4000 tokens) 91 us, with one
+// operand 68.5.
 //  * Two workgroups of 4 waves (128 rows) to a CU for up to 128 rows a KV head, one of 8 waves (256
 //    rows, a chunk loaded once for twice the rows) above.
 //  * The list of (sequence, KV head, tile, chunk) units is cut into as many equal runs as there are
@@ -221,6 +224,7 @@ tree_tile_kernel(
   constexpr int RPI = 1024 / ROWB;               // rows per 1-KiB DMA load
   constexpr int LPW = SLAB / 1024 / NW;          // loads per wave and slab
   constexpr int RPW = kChunk / NW;               // rows per wave: one block's
+  constexpr int kTerms = D > 128 ? 3 : 1;        // operands that hold a probability
   static_assert(LPW >= 1 && LPW * RPI == RPW && RPW <= 16, "a wave's rows lie in one block");
   // Stage c of a piece is V of its chunk c and K of chunk c + 1, what one turn of the loop needs.
   // [buffer][K | V]
@@ -512,15 +516,36 @@ tree_tile_kernel(
       for (int ks = 0; ks < NKS; ++ks)
         sc = mfma32x32<Tag>(read_k(buf * 2 * SLAB, x, ks), qop[ks], sc);
     };
-    // O^T += V^T . P^T over half x of the chunk in buffer buf.
-    auto add_pv = [&](int buf, int x, const dsp_u32x4 (&pop)[2]) {
+    // The probabilities of a half that wait for their P V: as operands (P^T of two 16-key steps: step
+    // ps takes registers j = 8*ps .. 8*ps + 7, i.e. keys 16*ps + 4*hl + {0..3, 8..11}), or, where
+    // three operands hold one, in fp32 until their step (the operands of both would take 24
+    // registers).
+    dsp_u32x4 pop[2];
+    f32x16 pend;
+    auto operands = [&](int ps, dsp_u32x4 (&t)[kTerms]) {
+      if constexpr (kTerms == 1) {
+        t[0] = pop[ps];
+      } else {
+        float p[8];
 #pragma unroll
-      for (int ps = 0; ps < 2; ++ps)
+        for (int i = 0; i < 8; ++i) p[i] = pend[8 * ps + i];
+        pack8<Tag, kTerms>(p, t);
+      }
+    };
+    // O^T += V^T . P^T over half x of the chunk in buffer buf.
+    auto add_pv = [&](int buf, int x) {
+#pragma unroll
+      for (int ps = 0; ps < 2; ++ps) {
+        dsp_u32x4 t[kTerms];
+        operands(ps, t);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
           __builtin_amdgcn_sched_barrier(0);  // (registers)
-          acc[dt] = mfma32x32<Tag>(read_v(buf * 2 * SLAB, x, ps, dt), pop[ps], acc[dt]);
+          const dsp_u32x4 v = read_v(buf * 2 * SLAB, x, ps, dt);
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k) acc[dt] = mfma32x32<Tag>(v, t[k], acc[dt]);
         }
+      }
     };
     // Which keys of half x of chunk c the row sees, in a chunk that holds nodes (bit i: key 32*x +
     // 4*hl + i of it).
@@ -532,8 +557,10 @@ tree_tile_kernel(
     // whether a row's maximum exceeds the running one by more than 2^kLag; mx: the half's, base 2.
     // What m holds is the running maximum less kRef: fp16's least number is 2^-24, bf16's far below,
     // so fp16 operands go up to 2^15 and end at 2^-31 of a row's largest probability (without it a
-    // tail of keys below 2^-25 of a row's first key counted for nothing).
-    constexpr float kLag = 8.f, kRef = std::is_same<Tag, F16Tag>::value ? 7.f : 0.f;
+    // tail of keys below 2^-25 of a row's first key counted for nothing), three operands at 2^-39
+    // (pack8: the maximum does not lag then).
+    constexpr bool kF16 = std::is_same<Tag, F16Tag>::value;
+    constexpr float kLag = kF16 && kTerms == 3 ? 0.f : 8.f, kRef = kF16 ? 15.f - kLag : 0.f;
     float mx = 0.f;
     auto settle = [&](int c, int x, int kflags, f32x16& sc) -> bool {
       if (kbeg + (c + 1) * kChunk > tree0) {
@@ -572,25 +599,31 @@ tree_tile_kernel(
       for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
       return alpha;
     };
-    // One probability of a half, and the operands they make (P^T of two 16-key steps: step ps takes
-    // registers j = 8*ps .. 8*ps + 7, i.e. keys 16*ps + 4*hl + {0..3, 8..11}).
     auto prob = [&](const f32x16& sc, int j, float neg_m) {
       const float p = dsp_exp2(fmaf(sc[j], scale_log2, neg_m));
       lpart += p;
       return p;
     };
-    // Of a chunk before the tree, which every row sees, an operand is kept above 0 (kLeast: 2^-31 of
-    // the row's largest probability in fp16, 2^-126 in bf16), so that an infinity in V meets a
-    // positive factor.  (Keys with a bad block id: V is zeros.  A chunk that holds nodes: take_odd.)
-    constexpr uint32_t kLeast = std::is_same<Tag, F16Tag>::value ? 0x00010001u : 0x00800080u;
-    auto least_of = [&](int c) { return kbeg + (c + 1) * kChunk > tree0 ? 0u : kLeast; };
-    auto probs = [&](int c, const f32x16& sc, dsp_u32x4 (&pop)[2]) {
-      const uint32_t least = least_of(c);
-      const float neg_m = m == -INFINITY ? 0.f : -m;
+    // Of a chunk before the tree, which every row sees, an operand is kept above 0 (one: 2^-31 of the
+    // row's largest probability in fp16, 2^-126 in bf16; three: pack8 keeps those of what is not
+    // below kLeastP), so that an infinity in V meets a positive factor.  (Keys with a bad block id:
+    // V is zeros.  A chunk that holds nodes: take_odd.)
+    constexpr uint32_t kLeast = kF16 ? 0x00010001u : 0x00800080u;
+    constexpr float kLeastP = kF16 ? 0x1p-24f : 0x1p-126f;
+    auto before_tree = [&](int c) { return kbeg + (c + 1) * kChunk <= tree0; };
+    // Exponentials e .. e + n of the half sc (n even) of chunk c (before: before_tree(c)), and their
+    // operands.
+    auto take_probs = [&](f32x16& sc, int e, int n, float neg_m, bool before, dsp_u32x4 (&to)[2]) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        const float p0 = prob(sc, j, neg_m), p1 = prob(sc, j + 1, neg_m);
-        pop[j >> 3][(j >> 1) & 3] = not_below(narrow2<Tag>(p0, p1), least);
+      for (int j = e; j < e + n; ++j) {
+        sc[j] = prob(sc, j, neg_m);
+        if constexpr (kTerms == 1) {
+          if (j & 1)
+            to[j >> 3][(j >> 1) & 3] =
+                not_below(narrow2<Tag>(sc[j - 1], sc[j]), before ? kLeast : 0u);
+        } else {
+          sc[j] = fmaxf(sc[j], before ? kLeastP : 0.f);  // (NaN: the sum has it)
+        }
       }
     };
     // (rare) infinities and NaN of V of chunk c, in buffer buf, to the rows that see them; then they
@@ -624,18 +657,7 @@ tree_tile_kernel(
     constexpr int kFirst = NB - 1;  // the buffer of K of chunk 0
     constexpr int kAhead = NDT < 3 ? NDT : 3;  // operands read ahead of their MFMAs
     constexpr int kSendAt = 1;  // the step of a chunk's first half in which the next stage is sent for
-    // A half's exponentials, 1 / NKS of them at a time (step i).
     static_assert(NKS <= 16 && NKS == 2 * NDT, "a step has one exponential or more");
-    auto take_probs = [&](f32x16& sc, int i, float neg_m, uint32_t least, dsp_u32x4 (&pop)[2]) {
-      constexpr int PER = 16 / NKS;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        const int j = PER * i + e;
-        sc[j] = prob(sc, j, neg_m);
-        if (j & 1)
-          pop[j >> 3][(j >> 1) & 3] = not_below(narrow2<Tag>(sc[j - 1], sc[j]), least);
-      }
-    };
     int kflags = s_flag[3];  // (in a vector register until it is looked at)
     // Half by half, a pipeline in which the MFMAs of one half's scores and of another's P V have
     // the exponentials of a third beside them, instruction by instruction (a wave issues in order:
@@ -643,7 +665,6 @@ tree_tile_kernel(
     // probabilities of cur; of half x of a stage, next = the scores and acc += P V with the
     // probabilities before (pop).
     f32x16 s0, s1;
-    dsp_u32x4 pop[2];
     auto half = [&](auto xc, int c, int cx, int buf, int kfl, f32x16& cur, f32x16& next) {
       constexpr int x = decltype(xc)::value;
       const uint32_t at = uint32_t(buf * 2 * SLAB);
@@ -655,19 +676,26 @@ tree_tile_kernel(
       }
       __builtin_amdgcn_sched_barrier(0);
       if (settle(c, cx, kfl, cur)) {
-        // the probabilities that still wait for their P V move along, rounded once more (the
-        // factor is below 2^-8 where it is not 1, and so is what that adds to the row's error)
+        // the probabilities that still wait for their P V move along (one operand: rounded once
+        // more, but the factor is below 2^-8 where it is not 1, and so is what that adds to the
+        // row's error)
         const float alpha = rescale();
+        if constexpr (kTerms == 1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t two = pop[i >> 2][i & 3];
-          pop[i >> 2][i & 3] = not_below(
-              narrow2<Tag>(low<Tag>(two) * alpha, high<Tag>(two) * alpha), not_above(two, kLeast));
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t two = pop[i >> 2][i & 3];
+            pop[i >> 2][i & 3] =
+                not_below(narrow2<Tag>(low<Tag>(two) * alpha, high<Tag>(two) * alpha),
+                          not_above(two, kLeast));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) pend[j] = fmaxf(pend[j] * alpha, fminf(pend[j], kLeastP));
         }
       }
       const float neg_m = m == -INFINITY ? 0.f : -m;
-      const uint32_t least = least_of(c);
-      dsp_u32x4 fresh[2];
+      const bool before = before_tree(c);
+      dsp_u32x4 fresh[2], t[kTerms];
 #pragma unroll
       for (int j = 0; j < 16; ++j) next[j] = 0.f;
 #pragma unroll
@@ -679,18 +707,25 @@ tree_tile_kernel(
         }
         next = mfma32x32<Tag>(kop[i], qop[i], next);
         if (x == 0 && i == kSendAt) send_next(c);
-        take_probs(cur, i, neg_m, least, fresh);
+        take_probs(cur, 16 / NKS * i, 16 / NKS, neg_m, before, fresh);
+        if (i % NDT == 0) operands(i / NDT, t);
         __builtin_amdgcn_sched_barrier(0);
-        acc[i % NDT] = mfma32x32<Tag>(vop[i], pop[i / NDT], acc[i % NDT]);
+#pragma unroll
+        for (int k = 0; k < kTerms; ++k) acc[i % NDT] = mfma32x32<Tag>(vop[i], t[k], acc[i % NDT]);
       }
       __builtin_amdgcn_sched_barrier(0);
-      pop[0] = fresh[0];
-      pop[1] = fresh[1];
+      if constexpr (kTerms == 1) {
+        pop[0] = fresh[0];
+        pop[1] = fresh[1];
+      } else {
+        pend = cur;
+      }
     };
     if (wave_has_rows) {
       scores(kFirst, 0, s0);
       if (settle(0, 0, kflags, s0)) rescale();
-      probs(0, s0, pop);
+      take_probs(s0, 0, 16, m == -INFINITY ? 0.f : -m, before_tree(0), pop);
+      if constexpr (kTerms > 1) pend = s0;
       scores(kFirst, 1, s1);
     }
     for (int c = 0; c < nc; ++c) {
@@ -706,7 +741,7 @@ tree_tile_kernel(
       }
       kflags = flags;
     }
-    if (wave_has_rows) add_pv((nc - 1) & (NB - 1), 1, pop);
+    if (wave_has_rows) add_pv((nc - 1) & (NB - 1), 1);
     // ---- the piece's rows: acc[dt][j] = O[row col][dim 32*dt + 8*(j/4) + 4*hl + j%4]
     lpart += dsp_shfl_xor(lpart, 32);
     const bool complete = c0 == 0 && c1 == nch;

@@ -1,5 +1,7 @@
 """How many bits paged_tree_attention keeps of its probabilities, and what they depend on."""
 
+import math
+
 import pytest
 import torch
 
@@ -54,3 +56,53 @@ def test_a_tail_below_a_sink_key_counts(hip, dtype, D, gap, ctx):
         err = (got[at:at + n] - want).abs()
         assert bool((err <= bound).all()), f"{float((err / bound).max()):.3g} of the bound"
         at += n
+
+
+def _wide_bits(dtype, D, ctx, n, values):
+    """n nodes of 3 heads over one KV head; keys 0 to 2 score 0, q0 and q1 and have the values
+    `values`(p) in each dimension, p (rows, 3) their probabilities over the row's largest times
+    some power of two; the others score -16 and have value 0.  Returns (got, want, size) per
+    dimension, whose row is d % rows: the attention, and sum p |v| over sum p."""
+    B, G, scale, f64 = 2, 3, 0.5, torch.float64
+    g = torch.Generator().manual_seed(7)
+    c = Case([n] * B, [ctx] * B, G, 1, D, dtype, seed=1, kind="chain")
+    q = torch.zeros((n, G, D), dtype=f64)
+    q[..., :2] = torch.rand((n, G, 2), generator=g) * 3 - 1.5
+    q[..., 2] = 4
+    q = q.to(dtype)
+    c.dq.copy_(q.repeat(B, 1, 1))
+    c.dk.zero_()
+    c.dv.zero_()
+    rows, ids = n * G, [torch.from_numpy(s).to(c.dk.device) for s in c.slots]
+    p = (scale * (q.to(f64).view(rows, D)[:, :2] * 2)).exp()
+    p = torch.cat((torch.ones(rows, 1, dtype=f64), p), 1)
+    mine = torch.arange(D) % rows
+    v = values(p[mine]).to(dtype)                             # (3, D)
+    for s in ids:
+        c.dk[s[1], 0, 0], c.dk[s[2], 0, 1] = 2, 2
+        c.dk[s[3:], 0, 2] = -8
+        c.dv[s[:3], 0] = v.to(c.dv.device)
+    seen = ctx - n + 1 + torch.arange(n).repeat_interleave(G)
+    total = (p.sum(1) + (seen - 3) * math.exp(-16))[mine]
+    terms = p[mine] * v.to(f64).t()
+    got = c.call(scale=scale).to(f64).cpu().view(B, rows, D)[:, mine, torch.arange(D)]
+    return got, terms.sum(1) / total, terms.abs().sum(1) / total
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 256), (F32, 64), (F32, 256), (BF16, 32)])
+@pytest.mark.parametrize("ctx,n", [(300, 5), (2000, 5), (2000, 60)])
+def test_cancelling_sums_keep_24_bits(hip, dtype, D, ctx, n):
+    """Where probabilities are fp32 (256-wide heads, fp32 caches, the general kernel), as in the
+    other attention.  The values are chosen so that p0 v0 + p1 v1 + p2 v2 cancels to about 2^-18
+    of its terms.  A score errs by the roundings of its exponent (below 2^-22 of p here) and of
+    exp2 (2^-23), a sum of three by 2^-23: below 2^-21 in all, of sum p |v|.  16 bits of p would
+    err by 2^-17."""
+    def values(p):
+        v0 = torch.ones(len(p), dtype=torch.float64)
+        v1 = (-p[:, 0] / p[:, 1]).to(dtype).double()
+        v2 = -(p[:, 0] + p[:, 1] * v1) / p[:, 2]
+        return torch.stack((v0, v1, v2))
+    got, want, size = _wide_bits(dtype, D, ctx, n, values)
+    half = torch.finfo(dtype).eps / 2                         # (the output's own rounding)
+    worst = float((((got - want).abs() - half * want.abs()) / size).max())
+    assert worst <= 2.0 ** -20, f"2^{math.log2(worst):.2f}"
