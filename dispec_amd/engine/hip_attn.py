@@ -391,6 +391,8 @@ def tree_mask(parents, cu_q, max_q_len=None, num_tokens=None):
     max_q_len = int(max_q_len)
     words = max(1, -(-max_q_len // 32))
     mask = torch.zeros((num_tokens, words), dtype=torch.int32, device=cu_q.device)
+    if not num_tokens:
+        return mask
     with _lib.on_device(cu_q):
         _lib.check(_lib.calls().dsp_tree_mask(
             _lib.ptr(parents), cu_q.data_ptr(), num_tokens, B, max_q_len, words, mask.data_ptr(),
@@ -462,7 +464,7 @@ def paged_tree_attention(q, k_cache, v_cache, block_table, cu_q, ctx_lens, tree_
     out = torch.empty_like(q) if out is None else out
     if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ValueError("out must have q's shape and dtype with head_dim contiguous")
-    if not T:
+    if not (T and B and max_q_len):   # (rows behind the last sequence stay as they are)
         return out
     need = _tree_ws_bytes(B, Hq, KVH, D, max_q_len, max_ctx)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):

@@ -128,7 +128,7 @@ def verify_draft(draft_tokens, target_probs, uniforms, final_uniforms, cu_q, par
             raise ValueError(f"{name} must be ({n},) float32; got {tuple(t.shape)} {t.dtype}")
     uniforms, final_uniforms = uniforms.contiguous(), final_uniforms.contiguous()
     got = _outputs(B, max_q_len, target_probs)
-    if not T:
+    if not (T and B and max_q_len):   # no node at all (T: rows behind the last sequence)
         return DraftVerdict(got[0].zero_(), got[1].fill_(-1), got[2].fill_(-1))
     need = _ws_bytes(B, V)
     ws = target_probs.new_empty(need, dtype=torch.uint8)
@@ -153,7 +153,7 @@ def match_draft(draft_tokens, target_tokens, cu_q, parents=None, max_q_len=None)
     tokens, cu_q, parents, T, B, max_q_len = _layout(draft_tokens, cu_q, parents, max_q_len)
     target_tokens = _ints(target_tokens, "target_tokens", T)
     got = _outputs(B, max_q_len, tokens)
-    if not T:
+    if not (T and B and max_q_len):   # no node at all (T: rows behind the last sequence)
         return DraftVerdict(got[0].zero_(), got[1].fill_(-1), got[2].fill_(-1))
     with _lib.on_device(tokens):
         _lib.check(_lib.calls().dsp_match_draft(

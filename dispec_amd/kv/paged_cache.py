@@ -97,6 +97,8 @@ def commit_path(key, value, block_table, cu_q, ctx_lens, path, num_accepted, blo
             (block_table, "block_table"), (cu_q, "cu_q"), (ctx_lens, "ctx_lens"), (path, "path"),
             (num_accepted, "num_accepted")) if t.dtype != int32)
         raise ValueError(f"{name} must be int32, got {dtype}")
+    if not B or paths[1] <= 1:   # a path's first node is the root, which stays
+        return
     if block_table.stride(1) != 1 and table[1] > 1:
         block_table = block_table.contiguous()
     if path.stride(1) != 1 and paths[1] > 1:

@@ -431,7 +431,8 @@ int dsp_paged_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride
  *   num_accepted : int32 [B], the kept nodes besides the root.
  *   path         : int32 [B, max_q_len], the kept nodes from the root (0) on, then -1.
  *   tokens       : int64 [B, max_q_len], their tokens without the root's, the drawn token, then -1.
- *                  (An empty sequence has 0, and -1 throughout.)
+ *                  (An empty sequence has 0, and -1 throughout.  With B or max_q_len 0 nothing is
+ *                  launched and no output is written.)
  *   workspace    : dsp_verify_workspace_bytes(B, V) bytes, 16-byte aligned. */
 size_t dsp_verify_workspace_bytes(int32_t B, int64_t V);
 int dsp_verify_draft(const int64_t* draft_tokens, const int32_t* parents,
