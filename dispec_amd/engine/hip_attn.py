@@ -360,8 +360,10 @@ def _ragged(q, k_cache, v_cache, block_table, cu_q, ctx_lens, block_size, scale,
 
 # ---- drafted trees: the last tokens of a context are the nodes of a tree
 @functools.lru_cache(maxsize=256)
-def _tree_ws_bytes(B, Hq, KVH, D, max_q_len, max_ctx) -> int:
-    return _lib.lib().dsp_paged_tree_workspace_bytes(B, Hq, KVH, D, max_q_len, max_ctx)
+def _tree_ws_bytes(device, B, Hq, KVH, D, max_q_len, max_ctx) -> int:
+    # (of the device, by its index: the launch is as wide as the chip)
+    with torch.cuda.device(device):
+        return _lib.lib().dsp_paged_tree_workspace_bytes(B, Hq, KVH, D, max_q_len, max_ctx)
 
 
 def tree_mask(parents, cu_q, max_q_len=None, num_tokens=None):
@@ -403,7 +405,9 @@ def tree_mask(parents, cu_q, max_q_len=None, num_tokens=None):
 def tree_workspace(batch, num_heads, num_kv_heads, head_dim, max_q_len, max_ctx, device):
     """A float32 workspace for every `paged_tree_attention` launch of this shape, or None when it
     needs none.  One buffer serves all layers of a forward: the launches run in stream order."""
-    need = _tree_ws_bytes(batch, num_heads, num_kv_heads, head_dim, max_q_len, max_ctx)
+    index = torch.device(device).index
+    need = _tree_ws_bytes(torch.cuda.current_device() if index is None else index, batch,
+                          num_heads, num_kv_heads, head_dim, max_q_len, max_ctx)
     return torch.empty(need // 4 + 1, dtype=torch.float32, device=device) if need else None
 
 
@@ -466,7 +470,7 @@ def paged_tree_attention(q, k_cache, v_cache, block_table, cu_q, ctx_lens, tree_
         raise ValueError("out must have q's shape and dtype with head_dim contiguous")
     if not (T and B and max_q_len):   # (rows behind the last sequence stay as they are)
         return out
-    need = _tree_ws_bytes(B, Hq, KVH, D, max_q_len, max_ctx)
+    need = _tree_ws_bytes(q.get_device(), B, Hq, KVH, D, max_q_len, max_ctx)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         # (of a size with the chip, not the batch: from torch's stream-ordered allocator per call)
         workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
