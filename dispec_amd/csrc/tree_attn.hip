@@ -25,10 +25,11 @@
 //    maximum, sum and accumulator per piece, and the second launch merges them.
 //  * What bounds it, heads of 128 in bf16: 32 trees of 16 nodes (G 2, 500 to 4000 tokens, 321 MB) 63
 //    us and 5 of merge: 5.1 TB/s, 5 us of it until the first keys are there.  4 trees of 64 (G 4,
-//    32768 tokens) 167 us and 8 of merge, 820 TFLOP/s (205 to 227 after a millisecond: the clock
-//    falls): two waves a SIMD issue for 74 % of the time, the matrix cores are busy for 38 %.  24
-//    trees of 1 to 33 nodes (40 to 3001 tokens) 25 us and 6: 5 chunks of 1.8 us a workgroup behind
-//    the chain lengths, block ids, first keys.
+//    32768 tokens) 170 us and 8 of merge, 810 TFLOP/s (205 to 223 after a millisecond: the clock
+//    falls): the matrix cores are busy for 37 % of the cycles, and two waves a SIMD, which issue in
+//    order, spend 26 % of theirs waiting to issue and 34 % on barriers, loads and LDS.  24 trees of
+//    1 to 33 nodes (40 to 3001 tokens) 26 us and 6: 5 chunks of 1.8 us a workgroup behind the chain
+//    lengths, block ids, first keys.
 // Everything else (fp32 caches, other head dims, blocks of fewer than 16 tokens, rows off 16 bytes,
 // a scale that is not positive) runs on the kernels of generic_attn.hip with the same masks.
 #include <float.h>
@@ -973,10 +974,11 @@ TreePlan tree_plan(int32_t B, int32_t KVH, int32_t G, int32_t D, int32_t max_q_l
   const int64_t slots = int64_t(dsp_detail::device_cus()) * (p.rows == 128 && D <= 128 ? 2 : 1);
   // Short contexts: tiles stay whole where that costs less, in chunks, than equal runs, a start each
   // and the merge (its launch 3, its partial results 2 where there are as many as fit; half of all
-  // that at D 256, whose chunks take twice the time).  The lengths are bounds here: only up to 16
-  // chunks.  Whole against cut, heads of 128: 512 tiles of 200 to 500 tokens 26.9 us (36.0), of 300
-  // to 1000 42.7 (46.5), 128 tiles 19.3 (20.4) and 28.8 (24.3); heads of 64, 2 tiles of 300 tokens
-  // 12.2 (12.3), of 500 16.1 (13.1), of 1000 24.7 (13.2); of 256, 64 tiles of 200 to 500 34.2 (27.6).
+  // that at D 256, whose chunks take two to four times as long).  The lengths are bounds here: only
+  // up to 16 chunks.  Whole against cut, heads of 128: 512 tiles of 200 to 500 tokens 26.9 us
+  // (36.0), of 300 to 1000 42.7 (46.5), 128 tiles 19.3 (20.4) and 28.8 (24.3); heads of 64, 2 tiles
+  // of 300 tokens 12.2 (12.3), of 500 16.1 (13.1), of 1000 24.7 (13.2); of 256, captured in a graph,
+  // 64 tiles of 200 to 500 36.6 (28.9), 256 tiles 51.6 (55.9).
   const int64_t runs = std::min((tiles * units + kMinChunks - 1) / kMinChunks, slots);
   const int64_t share = std::max((tiles * units + slots - 1) / slots, int64_t(kMinChunks));
   p.whole = chunks <= 16 &&

@@ -394,7 +394,9 @@ int dsp_tree_mask(const int32_t* parents, const int32_t* cu_q, int64_t num_rows,
  * dtype DSP_BF16, DSP_F16 or DSP_F32, D a power of two from 8 to 256, any G.  A sequence with
  * q_len > ctx or ctx > max_ctx is counted in err_count and its rows written as zeros; keys of
  * block ids outside the cache are counted and skipped.  Infinities and NaN of a key's V reach the
- * rows that see the key. */
+ * rows that see the key, infinities as such however small the key's probability, and no others.
+ * Probabilities: fp32, but one 16-bit operand (rounded once; fp16 ends at 2^-31 of a row's largest)
+ * for 16-bit caches with D 64 or 128. */
 size_t dsp_paged_tree_workspace_bytes(int32_t B, int32_t Hq, int32_t KVH, int32_t D,
                                       int32_t max_q_len, int32_t max_ctx);
 int dsp_paged_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
