@@ -555,14 +555,16 @@ tree_tile_kernel(
                              kbeg + c * kChunk + 32 * x - tree0) >> (4 * hl);
     };
     // Half x of chunk c: keys that count for nothing (kflags: the flags that came with its K), and
-    // whether a row's maximum exceeds the running one by more than 2^kLag; mx: the half's, base 2.
-    // What m holds is the running maximum less kRef: fp16's least number is 2^-24, bf16's far below,
-    // so fp16 operands go up to 2^15 and end at 2^-31 of a row's largest probability (without it a
-    // tail of keys below 2^-25 of a row's first key counted for nothing), three operands at 2^-39
-    // (pack8: the maximum does not lag then).
+    // whether a row's probabilities would exceed 2^(kRef + kLag); top: the largest score.
+    // What m holds is the running maximum (base 2) less kRef: fp16's least number is 2^-24, bf16's
+    // far below, so fp16 operands go up to 2^15 and end at 2^-31 of a row's largest probability
+    // (without it a tail of keys below 2^-25 of a row's first key counted for nothing), three
+    // operands at 2^-37.  Differences to m are one fma each, here as in prob, and the largest is
+    // looked at before it is used: at 2^25 a step of fp32 is 4, and an fp16 operand could overflow.
     constexpr bool kF16 = std::is_same<Tag, F16Tag>::value;
-    constexpr float kLag = kF16 && kTerms == 3 ? 0.f : 8.f, kRef = kF16 ? 15.f - kLag : 0.f;
-    float mx = 0.f;
+    constexpr float kLag = kF16 && kTerms == 3 ? 2.f : 8.f, kRef = kF16 ? 15.f - kLag : 0.f;
+    float top = 0.f;
+    auto exceeds = [&] { return fmaf(top, scale_log2, -m) > kRef + kLag; };  // (-inf, -inf: no)
     auto settle = [&](int c, int x, int kflags, f32x16& sc) -> bool {
       if (kbeg + (c + 1) * kChunk > tree0) {
         const uint32_t seen = window(c, x);
@@ -580,19 +582,21 @@ tree_tile_kernel(
             for (int j = 0; j < 8; ++j) sc[8 * g + j] = -INFINITY;
           }
       }
-      mx = -INFINITY;
+      top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[j]);
-      mx = fmaxf(mx, dsp_shfl_xor(mx, 32)) * scale_log2;  // -inf stays -inf
-      return __builtin_amdgcn_ballot_w64(mx > m + (kRef + kLag)) != 0;
+      for (int j = 0; j < 16; ++j) top = fmaxf(top, sc[j]);
+      top = fmaxf(top, dsp_shfl_xor(top, 32));
+      return __builtin_amdgcn_ballot_w64(exceeds()) != 0;
     };
-    // The running maximum of such a row moves (p <= 2^kLag otherwise): the sum and the accumulators
+    // The running maximum of such a row moves: the sum and the accumulators
     // share it, so the result is the same.  Other rows of the wave keep theirs: what a row gives
     // does not depend on its neighbours.  The factor stays above 0: the accumulators may hold an
     // infinity, also of a key whose score is yet to come (take_odd), and 0 * inf is NaN.
     auto rescale = [&]() -> float {
-      const bool moves = mx > m + (kRef + kLag);
-      const float m_new = moves ? mx - kRef : m;
+      const bool moves = exceeds();
+      float m_new = moves ? fmaf(top, scale_log2, -kRef) : m;
+      if (moves && fmaf(top, scale_log2, -m_new) > 15.f)  // (steps of 16 and more: the next one up)
+        m_new = __uint_as_float(__float_as_uint(m_new) + (m_new > 0.f ? 1 : -1));
       const float alpha = moves ? fmaxf(dsp_exp2(m - m_new), 0x1p-126f) : 1.f;
       m = m_new;
       lpart *= alpha;

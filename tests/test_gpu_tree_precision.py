@@ -106,3 +106,38 @@ def test_cancelling_sums_keep_24_bits(hip, dtype, D, ctx, n):
     half = torch.finfo(dtype).eps / 2                         # (the output's own rounding)
     worst = float((((got - want).abs() - half * want.abs()) / size).max())
     assert worst <= 2.0 ** -20, f"2^{math.log2(worst):.2f}"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("size,step", [(10, 1), (20, 8), (24, 8), (25, 4), (25, 8), (26, 8), (27, 16),
+                                       (28, 32)])
+@pytest.mark.parametrize("scale", [math.log(2.0), 1.0])
+def test_large_scores(hip, dtype, D, size, step, scale):
+    """Scores of 2^size and, from key 40 or 170 on, `step` more (both exact in fp32; a later one
+    exceeds the first by a step of fp32 or a few): no operand overflows, and the weights are 1 and
+    e^(scale step), whose exponent is off by a rounding of it and of log2(e) scale, 2^-23 of it
+    each at most.  (The tile kernel: the general kernel and the fp32 tiles round scores first.)"""
+    for turn in (40, 170):
+        c = Case([6], [300], 4, 2, D, dtype, seed=size)
+        c.dk.zero_()
+        c.dq.zero_()
+        first, second = (torch.from_numpy(s).to(c.dk.device)
+                         for s in (c.slots[0][:turn], c.slots[0][turn:]))
+        c.dq[:, :, 0], c.dq[:, :, 1] = 2.0 ** (size // 2), 1
+        c.dk[:, :, 0] = 2.0 ** (size - size // 2)
+        c.dk[second, :, 1] = step
+        c.dv[first], c.dv[second] = 1.0, 0.0
+        got = c.call(scale=scale).double().cpu()
+        seen = torch.from_numpy(c.see[0].sum(1)).double()[:, None, None] + 300 - 6 - turn
+        share = turn / (turn + seen * math.exp(scale * step))   # of the first keys, whose value is 1
+        half = torch.finfo(dtype).eps / 2
+        bound = share * (2 * half * (1 + half) + 2.0 ** -21 * step + 300 * 2.0 ** -24)
+        if dtype == F16:
+            # the running maximum is a multiple of fp32's step at that size, up to half of one above
+            # what it stands for, and the end of fp16 as much nearer
+            unit = 2.0 ** (math.floor(math.log2(2.0 ** size * scale * math.log2(math.e))) - 23)
+            bound = bound + 2.0 ** -25 + turn * 2.0 ** (-31 + unit / 2) / (turn + seen)
+        err = (got - share).abs()
+        assert bool(torch.isfinite(got).all()), turn
+        assert bool((err <= bound).all()), (turn, float((err / bound).max()))
