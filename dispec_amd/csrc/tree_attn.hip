@@ -13,8 +13,9 @@
 // v_mfma_f32_32x32x16, with P in registers (dsp_tile32.h), a row's running maximum that moves when it
 // is exceeded by 2^8, sums and accumulators in fp32.  Up to 128 dims the probabilities enter P V as
 // one 16-bit operand (rounded to nearest; the sum takes the unrounded ones): half a step of the
-// type, as much as the output's own rounding, and what the other attention kernels do there.  At
-// 256 dims they are three operands, all 24 bits, as in the other attention of such heads, which a
+// type, as much as the output's own rounding, as on the 16- and 128-row tiles of the multi-query
+// attention (its ragged verify batches and decode of more than 8 heads a KV head hold more).  At 256
+// dims they are three operands, all 24 bits, as in the other attention of such heads, which a
 // tree's batch takes over from: 12 sequences of 16 nodes (G 2, 500 to 4000 tokens) 91 us, with one
 // operand 68.5.
 //  * Two workgroups of 4 waves (128 rows) to a CU for up to 128 rows a KV head, one of 8 waves (256
