@@ -89,7 +89,8 @@ def verify_draft(draft_tokens, target_probs, uniforms, final_uniforms, cu_q, par
     cu_q:           (B+1,) int32 node offsets
     parents:        (T,) int32 parent of each node within its sequence (None: chains)
     draft_probs:    (T - B, V) like target_probs: q_0 .. q_{n-2} of each chain, packed (an empty
-                    sequence has no row)
+                    sequence has no row); with rows behind the last sequence, or empty ones,
+                    T - B to T rows, of which those behind the last chain's are not read
     max_q_len:      bound of the nodes of a sequence, at most 1024 (computed from cu_q if omitted,
                     which costs a device->host copy)
     err:            optional int32 device counter of drafted tokens outside the vocabulary and of
