@@ -23,6 +23,7 @@ DSP_BF16, DSP_F16, DSP_F32 = 0, 1, 2
 DSP_OK, DSP_EINVAL, DSP_EALIGN, DSP_EUNSUPPORTED, DSP_EWORKSPACE = 0, -1, -2, -3, -4
 DSP_ESCRATCH = -5
 DSP_NOALLOC_SCRATCH_BYTES = 32 << 20   # fixed workspace of dsp_paged_decode_noalloc
+DSP_KV_PLAIN, DSP_KV_FP8, DSP_KV_FP4 = 0, 1, 2   # what a cache's rows hold
 DSP_SPLIT_BALANCED = -1   # partition_tokens of dsp_paged_mq_attention: balanced split-K
 
 # (name, restype, argtypes) for every symbol the header declares.
@@ -74,6 +75,15 @@ SIGNATURES: dict[str, tuple] = {
         c_int, [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, _P, c_int64, c_int32,
                 _P, _P, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_int32,
                 c_int32, _P, c_size_t, _P, c_int64, c_int64, c_int32, _P, _P]),
+    "dsp_kv_append_quant": (c_int, [_P, _P, _P, _P, *[c_int64] * 6, _P, c_int64, c_int64, c_int64, _P,
+        c_int64, c_int64, c_int64, _P, c_int64, c_int32, c_int32, c_int32, c_int32, _P, _P]),
+    "dsp_kv_gather_quant": (c_int, [_P, _P, _P, _P, *[c_int64] * 6, _P, c_int64, c_int32, c_int32,
+        c_int32, _P, _P, c_int32, _P, _P]),
+    "dsp_paged_window_workspace_bytes": (c_size_t, [c_int32] * 10),
+    "dsp_paged_window_attention": (c_int, [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64,
+        _P, _P, c_int64, c_int64, c_int32, _P, c_int64, c_int32, _P, _P, c_int32, c_int32, c_int32,
+        c_int32, c_float, c_int32, c_int32, c_int32, c_int32, _P, c_size_t, _P, c_int64, c_int64,
+        c_int32, _P, _P]),
     "dsp_tree_mask": (c_int, [_P, _P, c_int64, c_int32, c_int32, c_int32, _P, _P]),
     "dsp_paged_tree_workspace_bytes": (c_size_t, [c_int32] * 6),
     "dsp_paged_tree_attention": (c_int, [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64,
@@ -112,7 +122,8 @@ _CALLS = None
 FAST_CALLS = ("dsp_paged_decode", "dsp_kv_append", "dsp_paged_mq_attention",
               "dsp_paged_mq_attention_ragged", "dsp_paged_mq_attention_shared_prefix",
               "dsp_qk_norm_rope_append", "dsp_paged_tree_attention", "dsp_verify_draft",
-              "dsp_match_draft", "dsp_kv_commit_path")
+              "dsp_match_draft", "dsp_kv_commit_path", "dsp_kv_append_quant",
+              "dsp_paged_window_attention")
 
 
 class HipLibraryError(RuntimeError):
@@ -208,6 +219,16 @@ def dtype_code(dtype) -> int:
     if code is None:
         raise ValueError(f"unsupported dtype {dtype}")
     return code
+
+
+_KV_FORMATS = {"fp8": DSP_KV_FP8, "fp4": DSP_KV_FP4}
+
+
+def kv_format(name: str) -> int:
+    """The code of a quantised cache's format."""
+    if name not in _KV_FORMATS:
+        raise ValueError(f"unknown cache format {name!r}: one of {tuple(_KV_FORMATS)}")
+    return _KV_FORMATS[name]
 
 
 def ptr(t) -> int | None:

@@ -122,4 +122,19 @@ int generic_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
                       int64_t o_stride_t, int64_t o_stride_h, int32_t dtype, int32_t* err_count,
                       hipStream_t s, const uint32_t* tree = nullptr, int32_t words = 0);
 
+// The same kernels with dsp_paged_window_attention's window (a context's end at most, >= 1) and
+// sinks: a bad context gives zeros in decode too.  span: generic_window_keys of the same arguments, the
+// keys that a sequence's queries see at most; the workspace is
+// generic_workspace_bytes(B, Hq, D, max_q_len, span, P) long.
+int64_t generic_window_keys(int32_t max_q_len, int32_t max_ctx, int32_t window, int32_t sinks);
+int generic_window_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                             const void* k_cache, const void* v_cache, int64_t num_slots,
+                             int64_t kv_stride_slot, int64_t kv_stride_head, const int32_t* table,
+                             int64_t table_stride, int32_t log2_bs, const int32_t* cu_q,
+                             const int32_t* ctx_lens, int32_t B, int32_t Hq, int32_t KVH,
+                             int32_t D, float scale, int32_t window, int32_t sinks,
+                             int32_t max_q_len, int32_t max_ctx, int32_t span, int32_t P,
+                             void* workspace, void* out, int64_t o_stride_t, int64_t o_stride_h,
+                             int32_t dtype, int32_t* err_count, hipStream_t s);
+
 }  // namespace dsp_detail

@@ -94,6 +94,15 @@ typedef int (*match_fn)(void*, void*, void*, void*, int64_t, int32_t, int32_t, v
 typedef int (*commit_fn)(void*, void*, int64_t, int64_t, int64_t, int64_t, int64_t, int32_t,
                          void*, int64_t, int32_t, void*, void*, void*, int64_t, int32_t,
                          void*, int32_t, void*, void*);
+typedef int (*append_quant_fn)(void*, void*, void*, void*, int64_t, int64_t, int64_t, int64_t,
+                               int64_t, int64_t, void*, int64_t, int64_t, int64_t, void*,
+                               int64_t, int64_t, int64_t, void*, int64_t, int32_t, int32_t,
+                               int32_t, int32_t, void*, void*);
+typedef int (*window_fn)(void*, int64_t, int64_t, void*, void*, int64_t, int64_t, int64_t,
+                         void*, void*, int64_t, int64_t, int32_t, void*, int64_t, int32_t,
+                         void*, void*, int32_t, int32_t, int32_t, int32_t, float, int32_t,
+                         int32_t, int32_t, int32_t, void*, size_t, void*, int64_t, int64_t,
+                         int32_t, void*, void*);
 
 static decode_fn p_decode;
 static append_fn p_append;
@@ -105,6 +114,8 @@ static tree_fn p_tree;
 static verify_fn p_verify;
 static match_fn p_match;
 static commit_fn p_commit;
+static append_quant_fn p_append_quant;
+static window_fn p_window;
 
 #define UNBOUND(ptr, name)                                                        \
   if (!(ptr)) {                                                                   \
@@ -259,6 +270,36 @@ static PyObject* w_commit(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(st);
 }
 
+static const char kAppendQuantSig[] = "PPPPqqqqqqPqqqPqqqPqiiiiPP";
+static PyObject* w_append_quant(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  arg_t v[40];
+  UNBOUND(p_append_quant, "dsp_kv_append_quant");
+  if (!convert("dsp_kv_append_quant", kAppendQuantSig, a, n, v)) return NULL;
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = p_append_quant(v[0].p, v[1].p, v[2].p, v[3].p, v[4].q, v[5].q, v[6].q, v[7].q, v[8].q,
+                      v[9].q, v[10].p, v[11].q, v[12].q, v[13].q, v[14].p, v[15].q, v[16].q,
+                      v[17].q, v[18].p, v[19].q, v[20].i, v[21].i, v[22].i, v[23].i, v[24].p,
+                      v[25].p);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
+static const char kWindowSig[] = "PqqPPqqqPPqqiPqiPPiiiifiiiiPzPqqiPP";
+static PyObject* w_window(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  arg_t v[40];
+  UNBOUND(p_window, "dsp_paged_window_attention");
+  if (!convert("dsp_paged_window_attention", kWindowSig, a, n, v)) return NULL;
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = p_window(v[0].p, v[1].q, v[2].q, v[3].p, v[4].p, v[5].q, v[6].q, v[7].q, v[8].p, v[9].p,
+                v[10].q, v[11].q, v[12].i, v[13].p, v[14].q, v[15].i, v[16].p, v[17].p, v[18].i,
+                v[19].i, v[20].i, v[21].i, v[22].f, v[23].i, v[24].i, v[25].i, v[26].i, v[27].p,
+                v[28].z, v[29].p, v[30].q, v[31].q, v[32].i, v[33].p, v[34].p);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
 /* bind(name, address): the entry point `name` of the loaded library is at `address`. */
 static PyObject* w_bind(PyObject* self, PyObject* args) {
   const char* name;
@@ -275,6 +316,8 @@ static PyObject* w_bind(PyObject* self, PyObject* args) {
   else if (!strcmp(name, "dsp_verify_draft")) p_verify = (verify_fn)p;
   else if (!strcmp(name, "dsp_match_draft")) p_match = (match_fn)p;
   else if (!strcmp(name, "dsp_kv_commit_path")) p_commit = (commit_fn)p;
+  else if (!strcmp(name, "dsp_kv_append_quant")) p_append_quant = (append_quant_fn)p;
+  else if (!strcmp(name, "dsp_paged_window_attention")) p_window = (window_fn)p;
   else {
     PyErr_Format(PyExc_KeyError, "no fast binding for %s", name);
     return NULL;
@@ -296,6 +339,8 @@ static PyMethodDef kMethods[] = {
     {"dsp_verify_draft", (PyCFunction)(void (*)(void))w_verify, METH_FASTCALL, NULL},
     {"dsp_match_draft", (PyCFunction)(void (*)(void))w_match, METH_FASTCALL, NULL},
     {"dsp_kv_commit_path", (PyCFunction)(void (*)(void))w_commit, METH_FASTCALL, NULL},
+    {"dsp_kv_append_quant", (PyCFunction)(void (*)(void))w_append_quant, METH_FASTCALL, NULL},
+    {"dsp_paged_window_attention", (PyCFunction)(void (*)(void))w_window, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fastcall", NULL, -1, kMethods};
@@ -316,7 +361,9 @@ PyMODINIT_FUNC PyInit__fastcall(void) {
                {"dsp_paged_tree_attention", kTreeSig},
                {"dsp_verify_draft", kVerifySig},
                {"dsp_match_draft", kMatchSig},
-               {"dsp_kv_commit_path", kCommitSig}};
+               {"dsp_kv_commit_path", kCommitSig},
+               {"dsp_kv_append_quant", kAppendQuantSig},
+               {"dsp_paged_window_attention", kWindowSig}};
   PyObject* m = PyModule_Create(&kModule);
   if (!m) return NULL;
   PyObject* sigs = PyDict_New();

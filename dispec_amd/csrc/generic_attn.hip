@@ -17,12 +17,16 @@
 //  * a row with more than one partition is merged by the second kernel (16 partitions'
 //    partials in flight per lane).
 //
+// With a window (kWindowed) a sequence's keys are numbered without those between the sinks and the
+// first query's window (Gap), and partitions are cut in these numbers.
+//
 // Grid x runs over B * max_q_len row slots z (b = z / max_q_len, i = z % max_q_len), as the
 // tiled kernels' grids do: a sequence's rows beyond max_q_len are not computed.  Partial
 // results go to ws row (z * Hq + h) * num_parts + part (B * max_q_len * Hq rows of
 // num_parts partitions, then their (max, sum) pairs).
 #include <float.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "dsp_common.h"
@@ -54,6 +58,24 @@ __device__ __forceinline__ typename Tag::store st1(float f) {
     return f;
 }
 
+// Which keys a row sees: up to its own; those of a tree's mask; those of a window and the sinks.
+enum Sees { kCausal, kTreeMask, kWindowed };
+
+// The keys that no query of a sequence sees, `size` of them from key `from` on, are left out of the
+// numbering: number x is key x, or x + size from `from` on.
+struct Gap {
+  int from = 0, size = 0;
+  __device__ __forceinline__ int key(int x) const { return x < from ? x : x + size; }
+};
+// base: the position of the first query
+__device__ __forceinline__ Gap gap_of(int base, int window, int sinks) {
+  Gap g;
+  const int lo = max(base - window + 1, 0);
+  g.from = min(sinks, lo);
+  g.size = lo - g.from;
+  return g;
+}
+
 constexpr int kKeysPerStep = 8;
 constexpr int kMergeBatch = 16;
 
@@ -65,13 +87,16 @@ struct RowInfo {
   bool live;     // false: slot beyond the sequence's q_len (nothing to write)
   bool counted;  // this slot reports the sequence's bad lengths (one slot per sequence)
   int qlen;      // the sequence's queries
+  int pos;       // kWindowed: this query's position
+  Gap gap;
 };
 
-// (kTree: a row's keys end with the context, its mask says which of the tree's it sees)
-template <bool kTree>
+// (kTreeMask: a row's keys end with the context, its mask says which of the tree's it sees)
+template <int kSees>
 __device__ __forceinline__ RowInfo row_info(const int32_t* __restrict__ cu_q,
                                             const int32_t* __restrict__ ctx_lens,
-                                            int max_q_len, int max_ctx, int z) {
+                                            int max_q_len, int max_ctx, int window, int sinks,
+                                            int z) {
   RowInfo r;
   r.qlen = 1;
   r.b = z / max_q_len;
@@ -82,6 +107,11 @@ __device__ __forceinline__ RowInfo row_info(const int32_t* __restrict__ cu_q,
     r.live = true;
     r.vis = ctx < 0 ? 0 : (ctx > max_ctx ? max_ctx : ctx);
     r.counted = ctx < 0 || ctx > max_ctx;
+    if constexpr (kSees == kWindowed) {
+      r.pos = ctx - 1;
+      r.gap = gap_of(r.pos, window, sinks);
+      r.vis = r.counted ? 0 : ctx - r.gap.size;
+    }
     return r;
   }
   const int c0 = cu_q[r.b];
@@ -89,9 +119,14 @@ __device__ __forceinline__ RowInfo row_info(const int32_t* __restrict__ cu_q,
   r.tok = int64_t(c0) + i;
   r.live = i < qlen;
   const bool bad = qlen < 0 || ctx < qlen || ctx > max_ctx;
-  r.vis = bad ? 0 : kTree ? ctx : ctx - qlen + i + 1;
+  r.vis = bad ? 0 : kSees == kTreeMask ? ctx : ctx - qlen + i + 1;
   r.counted = bad && i == 0;
   r.qlen = qlen;
+  if constexpr (kSees == kWindowed) {
+    r.pos = ctx - qlen + i;
+    r.gap = gap_of(ctx - qlen, window, sinks);
+    if (!bad) r.vis -= r.gap.size;
+  }
   return r;
 }
 
@@ -102,14 +137,14 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v + dsp_shfl_xor(v, 32);
 }
 
-// The weight of a key or a part.  kTree: above 0 where there is one (an infinity in V of a key that a
-// row sees gives an infinity, however small the key's probability).
-template <bool kTree>
+// The weight of a key or a part.  With masks or a window: above 0 where there is one (an infinity in V
+// of a key that a row sees gives an infinity, however small the key's probability).
+template <int kSees>
 __device__ __forceinline__ float weight(float x) {
-  return kTree ? dsp_weight(x) : dsp_exp2(x);
+  return kSees != kCausal ? dsp_weight(x) : dsp_exp2(x);
 }
 
-template <typename Tag, int D, bool kTree>
+template <typename Tag, int D, int kSees>
 __global__ __launch_bounds__(64) void generic_attn_kernel(
     const typename Tag::store* __restrict__ q, int64_t qst, int64_t qsh,
     const typename Tag::store* __restrict__ kc, const typename Tag::store* __restrict__ vc,
@@ -118,12 +153,14 @@ __global__ __launch_bounds__(64) void generic_attn_kernel(
     const int32_t* __restrict__ ctx_lens, int32_t G, int32_t max_ctx, int32_t max_q_len,
     float scale_log2, int32_t P, int32_t num_parts, float* __restrict__ ws_acc,
     float* __restrict__ ws_ml, typename Tag::store* __restrict__ out, int64_t ost, int64_t osh,
-    int32_t* __restrict__ err_count, const uint32_t* __restrict__ tree, int32_t words) {
+    int32_t* __restrict__ err_count, const uint32_t* __restrict__ tree, int32_t words,
+    int32_t window, int32_t sinks) {
+  constexpr bool kTree = kSees == kTreeMask, kWin = kSees == kWindowed;
   constexpr int NV = D > 64 ? D / 64 : 1;  // dims per lane
   const int z = blockIdx.x, h = blockIdx.y, part = blockIdx.z, Hq = gridDim.y;
   const int lane = threadIdx.x;
   const bool act = lane < D;
-  const RowInfo r = row_info<kTree>(cu_q, ctx_lens, max_q_len, max_ctx, z);
+  const RowInfo r = row_info<kSees>(cu_q, ctx_lens, max_q_len, max_ctx, window, sinks, z);
   if (!r.live) return;
   if (r.counted && part == 0 && h == 0 && lane == 0 && err_count) atomicAdd(err_count, 1);
   const int vis = r.vis;
@@ -150,6 +187,8 @@ __global__ __launch_bounds__(64) void generic_attn_kernel(
   float m = -INFINITY, l = 0.f;
   bool bad_slot = false;
   for (int k0 = kbeg; k0 < kend; k0 += kKeysPerStep) {
+    if constexpr (kWin)  // (uniform)
+      if (k0 >= sinks && r.gap.key(k0 + kKeysPerStep - 1) <= r.pos - window) continue;
     uint32_t seen = ~0u;
     if constexpr (kTree)
       seen = dsp_tree_window(tree + r.tok * words, words, r.qlen, k0 - (vis - r.qlen));
@@ -157,15 +196,16 @@ __global__ __launch_bounds__(64) void generic_attn_kernel(
     bool ok[kKeysPerStep];
 #pragma unroll
     for (int u = 0; u < kKeysPerStep; ++u) {
-      const int key = k0 + u;
+      const int at = k0 + u, key = kWin ? r.gap.key(at) : at;
+      const bool in = at < kend && (!kWin || key > r.pos - window || key < sinks);
       int64_t sl = 0;
-      if (key < kend) {
+      if (in) {
         sl = log2_bs >= 0 ? (int64_t(trow[key >> log2_bs]) << log2_bs) +
                                 (key & ((1 << log2_bs) - 1))
                           : int64_t(trow[key]);
       }
-      ok[u] = key < kend && sl >= 0 && sl < num_slots;
-      bad_slot |= key < kend && !ok[u];
+      ok[u] = in && sl >= 0 && sl < num_slots;
+      bad_slot |= in && !ok[u];
       if constexpr (kTree) ok[u] = ok[u] && ((seen >> u) & 1u);
       const int64_t e = (ok[u] ? sl : 0) * kvs_slot + head_off;
 #pragma unroll
@@ -188,13 +228,13 @@ __global__ __launch_bounds__(64) void generic_attn_kernel(
       mx = fmaxf(mx, s[u]);
     }
     const float mu = mx == -INFINITY ? 0.f : mx;
-    const float alpha = weight<kTree>(m - mu);
+    const float alpha = weight<kSees>(m - mu);
     l *= alpha;
 #pragma unroll
     for (int j = 0; j < NV; ++j) acc[j] *= alpha;
 #pragma unroll
     for (int u = 0; u < kKeysPerStep; ++u) {
-      const float p = weight<kTree>(s[u] - mu);
+      const float p = weight<kSees>(s[u] - mu);
       l += p;
 #pragma unroll
       for (int j = 0; j < NV; ++j) acc[j] = fmaf(p, vv[u][j], acc[j]);
@@ -203,7 +243,7 @@ __global__ __launch_bounds__(64) void generic_attn_kernel(
   }
   if (bad_slot && lane == 0 && err_count) atomicAdd(err_count, 1);
   if (nparts == 1) {
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = (kWin ? l != 0.f : l > 0.f) ? 1.f / l : 0.f;
     if (act) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) o[lane + 64 * j] = st1<Tag>(acc[j] * inv);
@@ -260,7 +300,7 @@ __device__ __forceinline__ void load_f32(const float* __restrict__ p, bool ok, f
 
 constexpr int kTileWaves = 4;
 
-template <int D, bool kTree>
+template <int D, int kSees>
 __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2))) void f32_tile_kernel(
     const float* __restrict__ q, int64_t qst, int64_t qsh, const float* __restrict__ kc,
     const float* __restrict__ vc, int64_t num_slots, int64_t kvs_slot, int64_t kvs_head,
@@ -269,7 +309,8 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
     int32_t max_ctx, int32_t max_q_len, float scale_log2, int32_t P, int32_t num_parts,
     float* __restrict__ ws_acc, float* __restrict__ ws_ml, float* __restrict__ out, int64_t ost,
     int64_t osh, int32_t* __restrict__ err_count, const uint32_t* __restrict__ tree,
-    int32_t words) {
+    int32_t words, int32_t window, int32_t sinks) {
+  constexpr bool kTree = kSees == kTreeMask, kWin = kSees == kWindowed;
   constexpr int KE = D >= 16 ? 4 : 2;          // floats per K load
   constexpr int KJ = D / (4 * KE);             // K loads per row and lane
   constexpr int VE = D >= 64 ? 4 : (D >= 32 ? 2 : 1);  // floats per V load
@@ -290,13 +331,16 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
   if (bad_len && threadIdx.x == 0 && tile == 0 && part == 0 && kvh == 0 && err_count)
     atomicAdd(err_count, 1);
   if (dec) ctx = ctx < 0 ? 0 : (ctx > max_ctx ? max_ctx : ctx);
+  const int base = ctx - qlen;  // the first query's position; kTree: the tree's first key
+  Gap gap;
+  if constexpr (kWin) gap = gap_of(base, window, sinks);
   // keys visible to row r: its query's position + 1 (none for bad lengths or no context)
-  // (kTree: ctx, of which a row's mask says which of the tree's it sees)
+  // (kTree: ctx, of which a row's mask says which of the tree's it sees; kWin: by their numbers)
   auto visible = [&](int r) {
-    return !dec && bad_len ? 0 : kTree ? ctx : ctx - qlen + r / G + 1;
+    return (!dec || kWin) && bad_len ? 0 : kTree ? ctx : ctx - qlen + r / G + 1 - gap.size;
   };
-  const int base = ctx - qlen;  // kTree: the tree's first key
-  const int kend = visible(min(r0 + 15, rows - 1)), vis0 = kTree ? base : visible(r0);
+  const int last = min(r0 + 15, rows - 1);
+  const int kend = visible(last), vis0 = kTree ? base : visible(r0);
   const int kbeg = part * P, kfin = min(kbeg + P, kend);
   if (kbeg >= kend && part > 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -304,6 +348,11 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
   const int r = r0 + n;
   const bool row_ok = r < rows;
   const int vis = row_ok ? visible(r) : 0;
+  // kWin: the first number past the sinks that some row of the tile sees (the last row: from the next
+  // of seen_last on)
+  const int seen0 = kWin ? base + r0 / G - window + 1 - gap.size : 0;
+  const int seen_last = kWin ? base + last / G - window - gap.size : 0;
+  auto hidden = [&](int at) { return kWin && at >= sinks && at < seen0; };  // from every row
   const float* qrow = q + int64_t(q0 + (row_ok ? r / G : 0)) * qst +
                       int64_t(kvh * G + (row_ok ? r % G : 0)) * qsh;
   float qf[KJ][KE];
@@ -311,8 +360,9 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
   for (int j = 0; j < KJ; ++j) load_f32<KE>(qrow + 4 * KE * j + KE * grp, row_ok, qf[j]);
   const int32_t* trow = table + int64_t(b) * table_stride;
   const int64_t head_off = int64_t(kvh) * kvs_head;
-  auto slot_of = [&](int key) -> int64_t {  // -1: past the partition, or outside the cache
-    if (key >= kfin) return -1;
+  auto slot_of = [&](int at) -> int64_t {  // -1: past the partition, outside the cache, or hidden
+    if (at >= kfin || hidden(at)) return -1;
+    const int key = kWin ? gap.key(at) : at;
     const int64_t sl = log2_bs >= 0 ? (int64_t(trow[key >> log2_bs]) << log2_bs) +
                                           (key & ((1 << log2_bs) - 1))
                                     : int64_t(trow[key]);
@@ -323,10 +373,18 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   int first_bad = INT32_MAX;
-  int64_t slot = slot_of(kbeg + 16 * wave + n);  // of this lane's key of the next chunk
-  for (int t0 = kbeg + 16 * wave; t0 < kfin; t0 += 16 * kTileWaves) {
+  // the next of this wave's chunks, from t on, of which some row of the tile sees a key
+  auto from = [&](int t) {
+    if (kWin && t >= sinks && t + 15 < seen0)
+      t += (seen0 - 15 - t + 16 * kTileWaves - 1) / (16 * kTileWaves) * (16 * kTileWaves);
+    return t;
+  };
+  const int first = from(kbeg + 16 * wave);
+  int64_t slot = slot_of(first + n);  // of this lane's key of the next chunk
+  for (int t0 = first, next; t0 < kfin; t0 = next) {
+    next = from(t0 + 16 * kTileWaves);
     const int64_t cur = slot;
-    if (t0 + n < kfin && cur < 0 && first_bad == INT32_MAX) first_bad = t0 + n;
+    if (t0 + n < kfin && cur < 0 && !hidden(t0 + n) && first_bad == INT32_MAX) first_bad = t0 + n;
     float kf[KJ][KE], vf[4][VH][VE];
     const float* krow = kc + (cur < 0 ? 0 : cur) * kvs_slot + head_off + KE * grp;
 #pragma unroll
@@ -343,7 +401,7 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
       for (int h = 0; h < VH; ++h)
         load_f32<VE>(vrow + 64 * h, ok[j] && (D >= 16 || n < D), vf[j][h]);
     }
-    slot = slot_of(t0 + 16 * kTileWaves + n);
+    slot = slot_of(next + n);
     // scores of keys t0 + 4 * grp + j, row n: up to four chains
     constexpr int CH = KJ * KE < 4 ? KJ * KE : 4;
     f32x4 sc[CH];
@@ -364,7 +422,11 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
         bits = dsp_tree_window(tree + int64_t(q0 + r / G) * words, words, qlen, t0 - base) >>
                (4 * grp);
     auto sees = [&](int j) {
-      return kTree ? ((bits >> j) & 1u) != 0 : t0 + 4 * grp + j < vis;
+      const int at = t0 + 4 * grp + j;
+      if constexpr (kWin)
+        return at < vis && (at >= vis - window || gap.key(at) < sinks);
+      else
+        return kTree ? ((bits >> j) & 1u) != 0 : at < vis;
     };
     float p[4], mx = -INFINITY;
 #pragma unroll
@@ -375,17 +437,18 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
     mx = fmaxf(mx, dsp_shfl_xor(mx, 16));
     mx = fmaxf(mx, dsp_shfl_xor(mx, 32));
     const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
-    const float alpha = weight<kTree>(m - mu);
+    const float alpha = weight<kSees>(m - mu);
     m = mn;
     l *= alpha;
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] *= alpha;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      p[j] = weight<kTree>(p[j] - mu);
+      p[j] = weight<kSees>(p[j] - mu);
       l += p[j];
     }
-    if (t0 + 16 > vis0) {  // a chunk that the tile's first row does not see whole (uniform)
+    // a chunk that the tile's first row does not see whole, or the last one (uniform)
+    if (t0 + 16 > vis0 || (kWin && t0 <= seen_last && t0 + 16 > sinks)) {
       bool odd = false;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -463,7 +526,7 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
     float L = 0.f, A = 0.f;
 #pragma unroll
     for (int w = 0; w < kTileWaves; ++w) {
-      const float x = weight<kTree>(s_m[w][rr] - Mu);
+      const float x = weight<kSees>(s_m[w][rr] - Mu);
       L = fmaf(s_l[w][rr], x, L);
       A = fmaf(s_acc[w][rr][d], x, A);
     }
@@ -485,17 +548,18 @@ __global__ __launch_bounds__(64 * kTileWaves) __attribute__((amdgpu_waves_per_eu
 // Merge of a row's partitions: one wave per (row slot, head), four heads per workgroup (most row
 // slots of a ragged batch are empty: a quarter of the workgroups to start and end); lane d
 // folds dims d, d+64, ...
-template <typename Tag, int D, bool kTree>
+template <typename Tag, int D, int kSees>
 __global__ __launch_bounds__(256) void generic_merge_kernel(
     const float* __restrict__ ws_acc, const float* __restrict__ ws_ml,
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ ctx_lens, int32_t max_ctx,
     int32_t max_q_len, int32_t P, int32_t num_parts, int32_t Hq,
-    typename Tag::store* __restrict__ out, int64_t ost, int64_t osh) {
+    typename Tag::store* __restrict__ out, int64_t ost, int64_t osh, int32_t window,
+    int32_t sinks) {
   constexpr int NV = D > 64 ? D / 64 : 1;
   const int z = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (h >= Hq) return;
-  const RowInfo r = row_info<kTree>(cu_q, ctx_lens, max_q_len, max_ctx, z);
+  const RowInfo r = row_info<kSees>(cu_q, ctx_lens, max_q_len, max_ctx, window, sinks, z);
   if (!r.live || r.vis <= P) return;  // one partition at most: written by the attention kernel
   const int nparts = (r.vis + P - 1) / P;
   const int64_t row0 = (int64_t(z) * Hq + h) * num_parts;
@@ -519,20 +583,20 @@ __global__ __launch_bounds__(256) void generic_merge_kernel(
 #pragma unroll
     for (int u = 0; u < kMergeBatch; ++u) bm = fmaxf(bm, vm[u]);
     const float bmu = bm == -INFINITY ? 0.f : bm;
-    const float keep = weight<kTree>(M - bmu);
+    const float keep = weight<kSees>(M - bmu);
     L *= keep;
 #pragma unroll
     for (int j = 0; j < NV; ++j) A[j] *= keep;
 #pragma unroll
     for (int u = 0; u < kMergeBatch; ++u) {
-      const float w = weight<kTree>(vm[u] - bmu);
+      const float w = weight<kSees>(vm[u] - bmu);
       L = fmaf(vl[u], w, L);
 #pragma unroll
       for (int j = 0; j < NV; ++j) A[j] = fmaf(va[u][j], w, A[j]);
     }
     M = bm;
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = (kSees == kWindowed ? L != 0.f : L > 0.f) ? 1.f / L : 0.f;
   if (act) {
     typename Tag::store* o = out + r.tok * ost + int64_t(h) * osh;
 #pragma unroll
@@ -561,56 +625,95 @@ struct GenericArgs {
   int32_t* err_count;
   const uint32_t* tree;  // tree masks of `words` words a row, or null
   int32_t words;
+  int32_t window, sinks;
 };
 
-template <typename Tag, int D, bool kTree>
+template <typename Tag, int D, int kSees>
 int launch_generic_d(const GenericArgs& a, dim3 grid, dim3 mgrid, hipStream_t s) {
   using S = typename Tag::store;
   if constexpr (std::is_same<Tag, GF32>::value)
-    f32_tile_kernel<D, kTree><<<grid, 64 * kTileWaves, 0, s>>>(
+    f32_tile_kernel<D, kSees><<<grid, 64 * kTileWaves, 0, s>>>(
         static_cast<const S*>(a.q), a.qst, a.qsh, static_cast<const S*>(a.kc),
         static_cast<const S*>(a.vc), a.num_slots, a.kvs_slot, a.kvs_head, a.table, a.table_stride,
         a.log2_bs, a.cu_q, a.ctx_lens, a.G, a.max_ctx, a.max_q_len, a.scale_log2, a.P,
         a.num_parts, a.ws_acc, a.ws_ml, static_cast<S*>(a.out), a.ost, a.osh, a.err_count, a.tree,
-        a.words);
+        a.words, a.window, a.sinks);
   else
-    generic_attn_kernel<Tag, D, kTree><<<grid, 64, 0, s>>>(
+    generic_attn_kernel<Tag, D, kSees><<<grid, 64, 0, s>>>(
         static_cast<const S*>(a.q), a.qst, a.qsh, static_cast<const S*>(a.kc),
         static_cast<const S*>(a.vc), a.num_slots, a.kvs_slot, a.kvs_head, a.table, a.table_stride,
         a.log2_bs, a.cu_q, a.ctx_lens, a.G, a.max_ctx, a.max_q_len, a.scale_log2, a.P,
         a.num_parts, a.ws_acc, a.ws_ml, static_cast<S*>(a.out), a.ost, a.osh, a.err_count, a.tree,
-        a.words);
+        a.words, a.window, a.sinks);
   const int st = dsp_launch_status();
   if (st != DSP_OK || a.num_parts <= 1) return st;
-  generic_merge_kernel<Tag, D, kTree><<<mgrid, 256, 0, s>>>(a.ws_acc, a.ws_ml, a.cu_q, a.ctx_lens,
+  generic_merge_kernel<Tag, D, kSees><<<mgrid, 256, 0, s>>>(a.ws_acc, a.ws_ml, a.cu_q, a.ctx_lens,
                                                      a.max_ctx, a.max_q_len, a.P, a.num_parts,
-                                                     a.Hq, static_cast<S*>(a.out), a.ost, a.osh);
+                                                     a.Hq, static_cast<S*>(a.out), a.ost, a.osh,
+                                                     a.window, a.sinks);
   return dsp_launch_status();
 }
 
-template <typename Tag, bool kTree>
+template <typename Tag, int kSees>
 int launch_generic(int D, const GenericArgs& a, dim3 grid, dim3 mgrid, hipStream_t s) {
   switch (D) {
-    case 8: return launch_generic_d<Tag, 8, kTree>(a, grid, mgrid, s);
-    case 16: return launch_generic_d<Tag, 16, kTree>(a, grid, mgrid, s);
-    case 32: return launch_generic_d<Tag, 32, kTree>(a, grid, mgrid, s);
-    case 64: return launch_generic_d<Tag, 64, kTree>(a, grid, mgrid, s);
-    case 128: return launch_generic_d<Tag, 128, kTree>(a, grid, mgrid, s);
-    case 256: return launch_generic_d<Tag, 256, kTree>(a, grid, mgrid, s);
+    case 8: return launch_generic_d<Tag, 8, kSees>(a, grid, mgrid, s);
+    case 16: return launch_generic_d<Tag, 16, kSees>(a, grid, mgrid, s);
+    case 32: return launch_generic_d<Tag, 32, kSees>(a, grid, mgrid, s);
+    case 64: return launch_generic_d<Tag, 64, kSees>(a, grid, mgrid, s);
+    case 128: return launch_generic_d<Tag, 128, kSees>(a, grid, mgrid, s);
+    case 256: return launch_generic_d<Tag, 256, kSees>(a, grid, mgrid, s);
     default: return DSP_EUNSUPPORTED;
   }
 }
 
-template <bool kTree>
+template <int kSees>
 int launch_generic_type(int32_t dtype, int D, const GenericArgs& a, dim3 grid, dim3 mgrid,
                         hipStream_t s) {
   switch (dtype) {
-    case DSP_BF16: return launch_generic<GBf16, kTree>(D, a, grid, mgrid, s);
-    case DSP_F16: return launch_generic<GF16, kTree>(D, a, grid, mgrid, s);
-    case DSP_F32: return launch_generic<GF32, kTree>(D, a, grid, mgrid, s);
+    case DSP_BF16: return launch_generic<GBf16, kSees>(D, a, grid, mgrid, s);
+    case DSP_F16: return launch_generic<GF16, kSees>(D, a, grid, mgrid, s);
+    case DSP_F32: return launch_generic<GF32, kSees>(D, a, grid, mgrid, s);
     default: return DSP_EUNSUPPORTED;
   }
 }
+
+// span: keys that a sequence's queries see at most (max_ctx without a window).  window 0: none.
+int launch(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
+           const void* v_cache, int64_t num_slots, int64_t kv_stride_slot, int64_t kv_stride_head,
+           const int32_t* table, int64_t table_stride, int32_t log2_bs, const int32_t* cu_q,
+           const int32_t* ctx_lens, int32_t B, int32_t Hq, int32_t KVH, int32_t D, float scale,
+           int32_t max_q_len, int32_t max_ctx, int32_t span, int32_t P, void* workspace, void* out,
+           int64_t o_stride_t, int64_t o_stride_h, int32_t dtype, int32_t* err_count,
+           hipStream_t s, const uint32_t* tree, int32_t words, int32_t window, int32_t sinks) {
+  if (B == 0 || max_q_len == 0) return DSP_OK;
+  const int32_t num_parts = span > 0 ? (span + P - 1) / P : 1;
+  const int64_t rows = int64_t(B) * max_q_len;
+  // grid: x row slots (a sequence's rows side by side: they read the same keys), y query
+  // heads, z partitions
+  if (rows > (int64_t(1) << 26) || Hq > 65535 || num_parts > 65535) return DSP_EUNSUPPORTED;
+  float* ws_acc = static_cast<float*>(workspace);
+  GenericArgs a{q, q_stride_t, q_stride_h, k_cache, v_cache, num_slots, kv_stride_slot,
+                kv_stride_head, table, table_stride, log2_bs, cu_q, ctx_lens, Hq / KVH, Hq,
+                max_ctx, max_q_len, scale * 1.4426950408889634f, P, num_parts, ws_acc,
+                num_parts > 1 ? ws_acc + rows * Hq * num_parts * D : nullptr, out, o_stride_t,
+                o_stride_h, err_count, tree, words, window, sinks};
+  dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(Hq),
+            static_cast<unsigned>(num_parts));
+  dim3 mgrid(static_cast<unsigned>(rows), static_cast<unsigned>((Hq + 3) / 4));
+  if (dtype == DSP_F32) {
+    // 16-row tiles: x (tile, partition), y KV heads, z sequences
+    const int64_t tiles = (int64_t(max_q_len) * (Hq / KVH) + 15) / 16;
+    if (tiles * num_parts >= (int64_t(1) << 31) || KVH > 65535 || B > 65535)
+      return DSP_EUNSUPPORTED;
+    grid = dim3(static_cast<unsigned>(tiles * num_parts), static_cast<unsigned>(KVH),
+                static_cast<unsigned>(B));
+  }
+  if (window > 0) return launch_generic_type<kWindowed>(dtype, D, a, grid, mgrid, s);
+  return tree ? launch_generic_type<kTreeMask>(dtype, D, a, grid, mgrid, s)
+              : launch_generic_type<kCausal>(dtype, D, a, grid, mgrid, s);
+}
+
 
 }  // namespace
 
@@ -636,31 +739,29 @@ int generic_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
                       int32_t max_ctx, int32_t P, void* workspace, void* out,
                       int64_t o_stride_t, int64_t o_stride_h, int32_t dtype, int32_t* err_count,
                       hipStream_t s, const uint32_t* tree, int32_t words) {
-  if (B == 0 || max_q_len == 0) return DSP_OK;
-  const int32_t num_parts = max_ctx > 0 ? (max_ctx + P - 1) / P : 1;
-  const int64_t rows = int64_t(B) * max_q_len;
-  // grid: x row slots (a sequence's rows side by side: they read the same keys), y query
-  // heads, z partitions
-  if (rows > (int64_t(1) << 26) || Hq > 65535 || num_parts > 65535) return DSP_EUNSUPPORTED;
-  float* ws_acc = static_cast<float*>(workspace);
-  GenericArgs a{q, q_stride_t, q_stride_h, k_cache, v_cache, num_slots, kv_stride_slot,
-                kv_stride_head, table, table_stride, log2_bs, cu_q, ctx_lens, Hq / KVH, Hq,
-                max_ctx, max_q_len, scale * 1.4426950408889634f, P, num_parts, ws_acc,
-                num_parts > 1 ? ws_acc + rows * Hq * num_parts * D : nullptr, out, o_stride_t,
-                o_stride_h, err_count, tree, words};
-  dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(Hq),
-            static_cast<unsigned>(num_parts));
-  dim3 mgrid(static_cast<unsigned>(rows), static_cast<unsigned>((Hq + 3) / 4));
-  if (dtype == DSP_F32) {
-    // 16-row tiles: x (tile, partition), y KV heads, z sequences
-    const int64_t tiles = (int64_t(max_q_len) * (Hq / KVH) + 15) / 16;
-    if (tiles * num_parts >= (int64_t(1) << 31) || KVH > 65535 || B > 65535)
-      return DSP_EUNSUPPORTED;
-    grid = dim3(static_cast<unsigned>(tiles * num_parts), static_cast<unsigned>(KVH),
-                static_cast<unsigned>(B));
-  }
-  return tree ? launch_generic_type<true>(dtype, D, a, grid, mgrid, s)
-              : launch_generic_type<false>(dtype, D, a, grid, mgrid, s);
+  return launch(q, q_stride_t, q_stride_h, k_cache, v_cache, num_slots, kv_stride_slot,
+                kv_stride_head, table, table_stride, log2_bs, cu_q, ctx_lens, B, Hq, KVH, D, scale,
+                max_q_len, max_ctx, max_ctx, P, workspace, out, o_stride_t, o_stride_h, dtype,
+                err_count, s, tree, words, 0, 0);
+}
+
+int64_t generic_window_keys(int32_t max_q_len, int32_t max_ctx, int32_t window, int32_t sinks) {
+  return window > 0 ? std::min<int64_t>(max_ctx, int64_t(sinks) + window + max_q_len) : max_ctx;
+}
+
+int generic_window_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                             const void* k_cache, const void* v_cache, int64_t num_slots,
+                             int64_t kv_stride_slot, int64_t kv_stride_head, const int32_t* table,
+                             int64_t table_stride, int32_t log2_bs, const int32_t* cu_q,
+                             const int32_t* ctx_lens, int32_t B, int32_t Hq, int32_t KVH,
+                             int32_t D, float scale, int32_t window, int32_t sinks,
+                             int32_t max_q_len, int32_t max_ctx, int32_t span, int32_t P,
+                             void* workspace, void* out, int64_t o_stride_t, int64_t o_stride_h,
+                             int32_t dtype, int32_t* err_count, hipStream_t s) {
+  return launch(q, q_stride_t, q_stride_h, k_cache, v_cache, num_slots, kv_stride_slot,
+                kv_stride_head, table, table_stride, log2_bs, cu_q, ctx_lens, B, Hq, KVH, D, scale,
+                max_q_len, max_ctx, span, P, workspace, out, o_stride_t, o_stride_h, dtype,
+                err_count, s, nullptr, 0, window, sinks);
 }
 
 }  // namespace dsp_detail

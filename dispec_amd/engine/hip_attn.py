@@ -358,6 +358,146 @@ def _ragged(q, k_cache, v_cache, block_table, cu_q, ctx_lens, block_size, scale,
     return True
 
 
+# ---- a sliding window and sinks; quantised caches
+@functools.lru_cache(maxsize=256)
+def _window_ws_bytes(device, B, Hq, KVH, D, max_q_len, max_ctx, window, sinks, fmt, dtype) -> int:
+    # (of the device, by its index: tiles are cut for the chip's size)
+    with torch.cuda.device(device):
+        return _lib.lib().dsp_paged_window_workspace_bytes(B, Hq, KVH, D, max_q_len, max_ctx, window,
+                                                           sinks, fmt, dtype)
+
+
+def window_workspace(batch, num_heads, num_kv_heads, head_dim, max_q_len, max_ctx, device,
+                     dtype=torch.bfloat16, window=0, sinks=0, format=None):
+    """A float32 workspace for every `paged_window_attention` launch of this shape (format None) or
+    `paged_quant_attention` launch over a cache of `format`, or None when it needs none.  One buffer
+    serves all layers of a forward: the launches run in stream order."""
+    index = torch.device(device).index
+    need = _window_ws_bytes(torch.cuda.current_device() if index is None else index, batch, num_heads,
+                            num_kv_heads, head_dim, max_q_len, max_ctx, window, sinks,
+                            _lib.DSP_KV_PLAIN if format is None else _lib.kv_format(format),
+                            _lib.dtype_code(dtype))
+    return torch.empty(need // 4 + 1, dtype=torch.float32, device=device) if need else None
+
+
+def _windowed(q, k_cache, v_cache, scales, fmt, block_table, cu_q, ctx_lens, kv_groups, window, sinks,
+              block_size, scale, max_q_len, max_ctx, out, err, workspace):
+    k_scale, v_scale = scales
+    _lib.one_gpu(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, ctx_lens, out, err, workspace)
+    if q.dim() != 3 or k_cache.dim() != 3 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"expected q (T, Hq, D) and caches (S, KVH, width); got {tuple(q.shape)}, "
+                         f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    T, Hq, D = q.shape
+    S, KVH, width = k_cache.shape
+    if width != (D // 2 if fmt == _lib.DSP_KV_FP4 else D) or Hq != KVH * kv_groups:
+        raise ValueError(f"q has {Hq} heads of {D}, cache {KVH} heads of width {width}, kv_groups "
+                         f"{kv_groups}")
+    if k_cache.stride() != v_cache.stride() or k_cache.stride(2) != 1:
+        raise ValueError("k_cache and v_cache need the same strides with head_dim contiguous")
+    window, sinks = int(window), int(sinks)
+    if window < 0 or sinks < 0 or sinks and not window:
+        raise ValueError(f"window {window} with {sinks} sinks: a window of 0 (the whole context) or "
+                         "more, sinks beside a window only")
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    ctx_lens, block_table = _i32(ctx_lens), _i32(block_table)
+    B = ctx_lens.numel()
+    if cu_q is None:
+        if T != B:
+            raise ValueError(f"q has {T} rows for {B} sequences: without cu_q one query a sequence")
+        max_q_len = min(B, 1)
+    else:
+        cu_q = _i32(cu_q)
+    if (cu_q is not None and cu_q.numel() != B + 1 or block_table.dim() != 2
+            or block_table.shape[0] != B):
+        raise ValueError(f"cu_q has {None if cu_q is None else cu_q.numel()} entries, block_table shape "
+                         f"{tuple(block_table.shape)} for {B} sequences")
+    if max_q_len is None:
+        max_q_len = int((cu_q[1:] - cu_q[:-1]).max().item()) if B else 0
+    if max_ctx is None:
+        max_ctx = block_table.shape[1] * block_size
+    max_q_len, max_ctx = int(max_q_len), int(max_ctx)
+    if max_ctx > block_table.shape[1] * block_size:
+        raise ValueError(f"max_ctx {max_ctx} exceeds the table's {block_table.shape[1]} blocks")
+    scale = D ** -0.5 if scale is None else scale
+    out = torch.empty_like(q) if out is None else out
+    if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("out must have q's shape and dtype with head_dim contiguous")
+    if not (T and B and max_q_len):   # (rows behind the last sequence stay as they are)
+        return out
+    dtype, es = _lib.dtype_code(q.dtype), k_cache.element_size()
+    need = _window_ws_bytes(q.get_device(), B, Hq, KVH, D, max_q_len, max_ctx, window, sinks, fmt, dtype)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        # (from torch's stream-ordered allocator, per call)
+        workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+    with _lib.on_device(q):
+        _lib.check(_lib.calls().dsp_paged_window_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), S,
+            k_cache.stride(0) * es, k_cache.stride(1) * es, _lib.ptr(k_scale), _lib.ptr(v_scale),
+            0 if k_scale is None else k_scale.stride(0), 0 if k_scale is None else k_scale.stride(1),
+            fmt, block_table.data_ptr(), block_table.stride(0), block_size, _lib.ptr(cu_q),
+            ctx_lens.data_ptr(), B, Hq, KVH, D, float(scale), window, sinks, max_q_len, max_ctx,
+            _lib.ptr(workspace), need, out.data_ptr(), out.stride(0), out.stride(1), dtype,
+            _lib.ptr(err), _lib.stream_of(q)), "dsp_paged_window_attention")
+    return out
+
+
+def paged_window_attention(q, k_cache, v_cache, block_table, cu_q, ctx_lens, kv_groups, window=0,
+                           sinks=0, block_size=16, scale=None, max_q_len=None, max_ctx=None, out=None,
+                           err=None, workspace=None):
+    """Paged attention with a sliding window and sinks (dsp_paged_window_attention).
+
+    Per sequence b, rows q[cu_q[b]:cu_q[b+1]] are the last tokens of a ctx_b-token context already in
+    the cache.  The token at position i sees the keys j <= i with i - j < window or j < sinks.
+
+    q:           (sum q_len, num_heads, head_dim), packed by sequence
+    block_table: (B, max_blocks) int32; entries of blocks none of whose keys a query of the sequence
+                 sees are not read (such blocks may have been freed)
+    cu_q:        (B+1,) int32 query offsets, or None: one query a sequence
+    ctx_lens:    (B,) int32 context lengths
+    window:      tokens that a token sees, itself included; 0: the whole context
+    sinks:       first tokens of a sequence that stay visible beside the window
+    max_q_len, max_ctx: host-side bounds (computed from cu_q / the table if omitted, the former at
+                 the cost of a device->host copy)
+    workspace:   optional preallocated buffer (`window_workspace`), for one stream at a time
+    err:         optional int32 device counter of bad lengths and block ids
+    returns:     (sum q_len, num_heads, head_dim) in q's dtype
+    """
+    if q.dtype not in _DTYPES or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError(f"q/k/v dtypes {q.dtype}/{k_cache.dtype}/{v_cache.dtype}: "
+                         "the HIP kernels take bf16, fp16 or fp32, all the same")
+    return _windowed(q, k_cache, v_cache, (None, None), _lib.DSP_KV_PLAIN, block_table, cu_q, ctx_lens,
+                     kv_groups, window, sinks, block_size, scale, max_q_len, max_ctx, out, err,
+                     workspace)
+
+
+def paged_quant_attention(q, k_cache, k_scale, v_cache, v_scale, block_table, cu_q, ctx_lens,
+                          kv_groups, window=0, sinks=0, block_size=16, scale=None, max_q_len=None,
+                          max_ctx=None, out=None, err=None, workspace=None):
+    """`paged_window_attention` over one layer of a quantised cache (`kv.quant_cache`): codes k_cache,
+    v_cache (S, KVH, head_dim) uint8 ("fp8") or (S, KVH, head_dim / 2) ("fp4") and scales k_scale,
+    v_scale (S, KVH, head_dim / 32) uint8.  q in bf16, fp16 or fp32, head_dim 64, 128 or 256; the
+    cache's numbers count as `quant_gather` gives them in q's dtype; scale > 0.
+    """
+    if q.dtype not in _DTYPES or any(t.dtype != torch.uint8 for t in (k_cache, k_scale, v_cache, v_scale)):
+        raise ValueError(f"q {q.dtype}, codes {k_cache.dtype}/{v_cache.dtype}, scales {k_scale.dtype}/"
+                         f"{v_scale.dtype}: q in bf16, fp16 or fp32, codes and scales in uint8")
+    D = q.shape[-1]
+    rows = k_cache.shape[:-1] + (D // 32,)
+    if D not in (64, 128, 256) or k_scale.shape != rows or v_scale.shape != rows:
+        raise ValueError(f"scales {tuple(k_scale.shape)}, {tuple(v_scale.shape)} for codes "
+                         f"{tuple(k_cache.shape)} and head_dim {D}: one for 32 elements, head_dim 64, "
+                         "128 or 256")
+    if k_scale.stride() != v_scale.stride() or k_scale.stride(2) != 1:
+        raise ValueError("k_scale and v_scale need the same strides with a head's scales contiguous")
+    if scale is not None and not 0 < scale < float("inf"):
+        raise ValueError(f"scale {scale}: positive and finite over a quantised cache")
+    fmt = _lib.DSP_KV_FP4 if 2 * k_cache.shape[-1] == D else _lib.DSP_KV_FP8
+    return _windowed(q, k_cache, v_cache, (k_scale, v_scale), fmt, block_table, cu_q, ctx_lens,
+                     kv_groups, window, sinks, block_size, scale, max_q_len, max_ctx, out, err,
+                     workspace)
+
+
 # ---- drafted trees: the last tokens of a context are the nodes of a tree
 @functools.lru_cache(maxsize=256)
 def _tree_ws_bytes(device, B, Hq, KVH, D, max_q_len, max_ctx) -> int:

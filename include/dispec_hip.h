@@ -57,6 +57,12 @@ enum dsp_status {
  * the balanced split-K kernel instead of fixed key partitions. */
 enum dsp_split { DSP_SPLIT_BALANCED = -1 };
 
+/* What a cache's rows hold: numbers of the model's type, or a quantised format's codes.  Of a quantised
+ * row, 32 neighbouring elements of a head share a scale 2^(byte - 127), one byte in an array of
+ * [num_slots, num_kv_heads, head_dim / 32]; an element is e4m3, one byte, or e2m1, half a byte, the
+ * first of two in the low half.  Byte 255: a group that held an infinity or NaN, all NaN. */
+enum dsp_kv_format { DSP_KV_PLAIN = 0, DSP_KV_FP8 = 1, DSP_KV_FP4 = 2 };
+
 /* Human-readable text for a status code (static storage; never NULL). */
 const char* dsp_error_string(int status);
 
@@ -364,6 +370,76 @@ int dsp_paged_mq_attention_shared_prefix(
     int32_t max_q_len, int32_t max_ctx, int32_t prefix_tokens, int32_t partition_tokens,
     void* workspace, size_t workspace_bytes, void* out, int64_t o_stride_t, int64_t o_stride_h,
     int32_t dtype, int32_t* err_count, dsp_stream_t stream);
+
+/* --------------------------------------------------- quantised caches, sliding windows
+ * The reference's pool holds the model's type and every query sees its whole context
+ * (dispec/kv/paged_cache.py:61-72, dispec/engine/model_runner.py:160-185).
+ *
+ * Rows into a quantised cache, over num_layers layers in one launch.  Of each group of 32 elements x,
+ * with M = 448 (DSP_KV_FP8) or 6 (DSP_KV_FP4) and e the least of -100 .. 118 with max |x| <= M 2^e, the
+ * scale is 2^e and an element's code that of the number nearest to x / 2^e (halves to the even code;
+ * beyond M, as where e is 118, M).  fp16 rows are first clamped to +-61440 (FP8) or +-49152 (FP4), so
+ * that all that is read back is finite in fp16.
+ *   k_pool, v_pool   : codes, num_slots rows of whole heads at pool_slot_stride_bytes in a layer (layer
+ *                      and slot strides and pointers multiples of 8 bytes).
+ *   k_scale, v_scale : scales, rows of KVH * D / 32 bytes at scale_slot_stride_bytes in a layer.
+ *   k, v             : rows of `dtype`, [layer, token, head, D] at strides, D contiguous.
+ *   slots            : int64 [num_tokens], unique, of every layer.  One outside the cache is skipped and
+ *                      counted once in err_count.
+ * D a multiple of 32, KVH * D <= 2^20 (else DSP_EUNSUPPORTED). */
+int dsp_kv_append_quant(void* k_pool, void* k_scale, void* v_pool, void* v_scale,
+                        int64_t num_layers, int64_t pool_layer_stride_bytes,
+                        int64_t pool_slot_stride_bytes, int64_t scale_layer_stride_bytes,
+                        int64_t scale_slot_stride_bytes, int64_t num_slots, const void* k,
+                        int64_t k_stride_l, int64_t k_stride_t, int64_t k_stride_h, const void* v,
+                        int64_t v_stride_l, int64_t v_stride_t, int64_t v_stride_h,
+                        const int64_t* slots, int64_t num_tokens, int32_t KVH, int32_t D,
+                        int32_t format, int32_t dtype, int32_t* err_count, dsp_stream_t stream);
+
+/* The values of a quantised cache's rows, rounded to `dtype` (exact in bf16 and fp32, and in fp16 for
+ * rows that were written from fp16; infinite past fp16's range): k_out, v_out [num_layers, num_tokens,
+ * KVH, D], contiguous.  A slot outside the cache leaves its rows as they were and is counted. */
+int dsp_kv_gather_quant(const void* k_pool, const void* k_scale, const void* v_pool,
+                        const void* v_scale, int64_t num_layers, int64_t pool_layer_stride_bytes,
+                        int64_t pool_slot_stride_bytes, int64_t scale_layer_stride_bytes,
+                        int64_t scale_slot_stride_bytes, int64_t num_slots, const int64_t* slots,
+                        int64_t num_tokens, int32_t KVH, int32_t D, int32_t format, void* k_out,
+                        void* v_out, int32_t dtype, int32_t* err_count, dsp_stream_t stream);
+
+/* Paged attention with a sliding window and sinks, over a cache in the model's type or a quantised one.
+ * As dsp_paged_mq_attention, but query i of sequence b, at position pos = ctx_lens[b] - q_len_b + i, sees
+ * the keys j <= pos with j > pos - window or j < sinks.  window 0: all keys j <= pos (sinks 0 then).
+ *   kv strides       : in BYTES, of k_cache and v_cache alike; scale strides of k_scale and v_scale (NULL
+ *                      and unread with DSP_KV_PLAIN).
+ *   cu_q             : int32 [B+1], or NULL: one query a sequence (max_q_len 1).
+ *   max_q_len        : bound of q_len_b; of a longer sequence the first max_q_len rows are computed.
+ *   block_table      : the entry of a block none of whose keys a query of the sequence sees is not read:
+ *                      such blocks may be freed.
+ *   workspace        : dsp_paged_window_workspace_bytes bytes for the same arguments on the same device
+ *                      (16-byte aligned; none where that is 0).
+ * A sequence with q_len > ctx or ctx > max_ctx is counted in err_count and its rows written as zeros (no
+ * cu_q and ctx 0: zeros, not counted); keys of block ids outside the cache are counted and skipped.
+ * DSP_KV_PLAIN: dtype DSP_BF16, DSP_F16 or DSP_F32, of q, cache and out, D a power of two from 8 to 256,
+ * any G.  A quantised cache: q and out of `dtype`, D 64, 128 or 256, rows of 16 (FP8) or 8 (FP4) bytes
+ * alignment, blocks of >= 16 tokens, num_slots a multiple of them, scale > 0 (else DSP_EUNSUPPORTED);
+ * its numbers count as dsp_kv_gather_quant gives them.  Infinities and NaN of a key's V reach the rows
+ * that see the key and no others.  Probabilities: fp32, but one 16-bit operand (rounded once; fp16 ends
+ * at 2^-31 of a row's largest) where q has 16 bits and D is 64, 128 or 256. */
+size_t dsp_paged_window_workspace_bytes(int32_t B, int32_t Hq, int32_t KVH, int32_t D,
+                                        int32_t max_q_len, int32_t max_ctx, int32_t window,
+                                        int32_t sinks, int32_t format, int32_t dtype);
+int dsp_paged_window_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                               const void* k_cache, const void* v_cache, int64_t num_slots,
+                               int64_t kv_stride_slot_bytes, int64_t kv_stride_head_bytes,
+                               const uint8_t* k_scale, const uint8_t* v_scale,
+                               int64_t scale_stride_slot, int64_t scale_stride_head,
+                               int32_t format, const int32_t* block_table, int64_t bt_stride,
+                               int32_t block_size, const int32_t* cu_q, const int32_t* ctx_lens,
+                               int32_t B, int32_t Hq, int32_t KVH, int32_t D, float scale,
+                               int32_t window, int32_t sinks, int32_t max_q_len, int32_t max_ctx,
+                               void* workspace, size_t workspace_bytes, void* out,
+                               int64_t o_stride_t, int64_t o_stride_h, int32_t dtype,
+                               int32_t* err_count, dsp_stream_t stream);
 
 /* ------------------------------------------------------------------- drafted trees
  * Speculative decoding with a tree of drafted tokens instead of a chain (the reference drafts
