@@ -123,7 +123,7 @@ FAST_CALLS = ("dsp_paged_decode", "dsp_kv_append", "dsp_paged_mq_attention",
               "dsp_paged_mq_attention_ragged", "dsp_paged_mq_attention_shared_prefix",
               "dsp_qk_norm_rope_append", "dsp_paged_tree_attention", "dsp_verify_draft",
               "dsp_match_draft", "dsp_kv_commit_path", "dsp_kv_append_quant",
-              "dsp_paged_window_attention")
+              "dsp_kv_gather_quant", "dsp_paged_window_attention")
 
 
 class HipLibraryError(RuntimeError):
@@ -272,6 +272,30 @@ def one_gpu(t, *others) -> None:
         if o is not None and o.get_device() != index:
             require_gpu(t, *others)
             raise ValueError(f"tensors on {t.device} and {o.device}: one call takes one device")
+
+
+def same_gpu(t, *others) -> int:
+    """`one_gpu` with the device's index."""
+    index = t.get_device()
+    if index < 0:
+        require_gpu(t, *others)
+    for o in others:
+        if o is not None and o.get_device() != index:
+            one_gpu(t, *others)
+    return index
+
+
+def call_on(index: int, fn, args) -> int:
+    """fn(*args) with device `index` the current one (see on_device)."""
+    global _current_device
+    if _current_device is None:
+        import torch
+        _current_device = torch.cuda.current_device
+    if index == _current_device():
+        return fn(*args)
+    import torch
+    with torch.cuda.device(index):
+        return fn(*args)
 
 
 def require_gpu(*tensors) -> None:

@@ -98,6 +98,9 @@ typedef int (*append_quant_fn)(void*, void*, void*, void*, int64_t, int64_t, int
                                int64_t, int64_t, void*, int64_t, int64_t, int64_t, void*,
                                int64_t, int64_t, int64_t, void*, int64_t, int32_t, int32_t,
                                int32_t, int32_t, void*, void*);
+typedef int (*gather_quant_fn)(void*, void*, void*, void*, int64_t, int64_t, int64_t, int64_t,
+                               int64_t, int64_t, void*, int64_t, int32_t, int32_t, int32_t,
+                               void*, void*, int32_t, void*, void*);
 typedef int (*window_fn)(void*, int64_t, int64_t, void*, void*, int64_t, int64_t, int64_t,
                          void*, void*, int64_t, int64_t, int32_t, void*, int64_t, int32_t,
                          void*, void*, int32_t, int32_t, int32_t, int32_t, float, int32_t,
@@ -115,6 +118,7 @@ static verify_fn p_verify;
 static match_fn p_match;
 static commit_fn p_commit;
 static append_quant_fn p_append_quant;
+static gather_quant_fn p_gather_quant;
 static window_fn p_window;
 
 #define UNBOUND(ptr, name)                                                        \
@@ -285,6 +289,20 @@ static PyObject* w_append_quant(PyObject* self, PyObject* const* a, Py_ssize_t n
   return PyLong_FromLong(st);
 }
 
+static const char kGatherQuantSig[] = "PPPPqqqqqqPqiiiPPiPP";
+static PyObject* w_gather_quant(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  arg_t v[40];
+  UNBOUND(p_gather_quant, "dsp_kv_gather_quant");
+  if (!convert("dsp_kv_gather_quant", kGatherQuantSig, a, n, v)) return NULL;
+  int st;
+  Py_BEGIN_ALLOW_THREADS
+  st = p_gather_quant(v[0].p, v[1].p, v[2].p, v[3].p, v[4].q, v[5].q, v[6].q, v[7].q, v[8].q,
+                      v[9].q, v[10].p, v[11].q, v[12].i, v[13].i, v[14].i, v[15].p, v[16].p,
+                      v[17].i, v[18].p, v[19].p);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(st);
+}
+
 static const char kWindowSig[] = "PqqPPqqqPPqqiPqiPPiiiifiiiiPzPqqiPP";
 static PyObject* w_window(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   arg_t v[40];
@@ -317,6 +335,7 @@ static PyObject* w_bind(PyObject* self, PyObject* args) {
   else if (!strcmp(name, "dsp_match_draft")) p_match = (match_fn)p;
   else if (!strcmp(name, "dsp_kv_commit_path")) p_commit = (commit_fn)p;
   else if (!strcmp(name, "dsp_kv_append_quant")) p_append_quant = (append_quant_fn)p;
+  else if (!strcmp(name, "dsp_kv_gather_quant")) p_gather_quant = (gather_quant_fn)p;
   else if (!strcmp(name, "dsp_paged_window_attention")) p_window = (window_fn)p;
   else {
     PyErr_Format(PyExc_KeyError, "no fast binding for %s", name);
@@ -340,6 +359,7 @@ static PyMethodDef kMethods[] = {
     {"dsp_match_draft", (PyCFunction)(void (*)(void))w_match, METH_FASTCALL, NULL},
     {"dsp_kv_commit_path", (PyCFunction)(void (*)(void))w_commit, METH_FASTCALL, NULL},
     {"dsp_kv_append_quant", (PyCFunction)(void (*)(void))w_append_quant, METH_FASTCALL, NULL},
+    {"dsp_kv_gather_quant", (PyCFunction)(void (*)(void))w_gather_quant, METH_FASTCALL, NULL},
     {"dsp_paged_window_attention", (PyCFunction)(void (*)(void))w_window, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL}};
 
@@ -363,6 +383,7 @@ PyMODINIT_FUNC PyInit__fastcall(void) {
                {"dsp_match_draft", kMatchSig},
                {"dsp_kv_commit_path", kCommitSig},
                {"dsp_kv_append_quant", kAppendQuantSig},
+               {"dsp_kv_gather_quant", kGatherQuantSig},
                {"dsp_paged_window_attention", kWindowSig}};
   PyObject* m = PyModule_Create(&kModule);
   if (!m) return NULL;

@@ -9,111 +9,17 @@
 // of K and V in LDS; S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16 (dsp_tile32.h), P in registers.
 // The chunks of a tile are those that hold a key that one of its rows sees: the sinks', then those of
 // the window; of a block none of whose keys is seen neither id nor rows are read.
-#include <float.h>
+#include "window_attn.h"
 
-#include <algorithm>
-
-#include "dsp_common.h"
-#include "dsp_internal.h"
-#include "dsp_mfma.h"
-#include "dsp_quant.h"
-#include "dsp_tile32.h"
+using namespace dsp_window;
 
 namespace {
 
-using namespace dsp_mfma;
-using dsp_quant::kFp4;
-using dsp_quant::kFp8;
-using dsp_quant::kNone;
-
 constexpr int kChunk = 64;           // keys per chunk
-constexpr int kWholeWindow = 1 << 30;  // a window that no context reaches the end of
-
-struct WinArgs {
-  const void* q;
-  int64_t qst, qsh;                // elements
-  const char* kc;
-  const char* vc;
-  const uint8_t* ks;               // scales of a quantised cache
-  const uint8_t* vs;
-  uint32_t num_blocks;
-  int64_t slot_bytes, head_bytes;  // of kc and vc
-  int64_t scale_slot, scale_head;  // of ks and vs
-  const int32_t* bt;
-  int64_t bt_stride;
-  int32_t log2_bs;
-  const int32_t* cu_q;             // null: one query a sequence
-  const int32_t* ctx_lens;
-  int32_t B, KVH, G, max_q_len, max_ctx, window, sinks;
-  float scale_log2;
-  int32_t tiles, parts, part_chunks;  // of a (sequence, KV head); of a tile
-  float* ws_acc;
-  float* ws_ml;
-  void* out;
-  int64_t ost, osh;
-  int32_t vec_out;
-  int32_t* err;
-};
-
-// A number that every lane of the wave reads alike, by a scalar load.
-__device__ __forceinline__ int32_t scalar_load(const int32_t* p) {
-  return *reinterpret_cast<__attribute__((address_space(4))) const int32_t*>(
-      reinterpret_cast<uintptr_t>(p));
-}
-
-struct Seq {
-  int q0, n, ctx;
-  bool bad;   // lengths that are none: counted, rows of zeros
-  int rows;   // packed rows that are computed
-};
-__device__ __forceinline__ Seq sequence(const WinArgs& a, int b) {
-  Seq s;
-  s.ctx = scalar_load(a.ctx_lens + b);
-  s.q0 = a.cu_q ? scalar_load(a.cu_q + b) : b;
-  s.n = a.cu_q ? scalar_load(a.cu_q + b + 1) - s.q0 : 1;
-  s.bad = s.n > 0 && (s.ctx < s.n || s.ctx > a.max_ctx);
-  s.rows = min(s.n, a.max_q_len) * a.G;
-  return s;
-}
-
-// Chunks of a tile whose rows are those of queries at positions pf .. pl: `sink` from key 0 on, then
-// those from key 64 * first on, n in all.
-struct Span {
-  int lo, hi;      // keys of the window: lo .. hi - 1
-  int sink, first, n;
-};
-__device__ __forceinline__ Span span_of(int pf, int pl, int window, int sinks) {
-  Span s;
-  s.hi = pl + 1;
-  s.lo = max(pf - window + 1, 0);
-  s.first = s.lo / kChunk;
-  s.sink = min((sinks + kChunk - 1) / kChunk, s.first);
-  s.n = s.sink + (s.hi + kChunk - 1) / kChunk - s.first;
-  return s;
-}
-
 template <int kNW, int kBufs, int kOcc>
 struct Shape {
   static constexpr int NW = kNW, TR = 32 * kNW, NB = kBufs, OCC = kOcc;
 };
-
-template <typename Tag>
-__device__ __forceinline__ uint32_t narrow2(float a, float b) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  if constexpr (std::is_same<Tag, Bf16Tag>::value)
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
-}
-
-// Of each of two operands' 16-bit numbers, not negative (or NaN, the largest here), the larger.
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t not_below(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
-                                                                __builtin_bit_cast(u16x2, b)));
-}
 
 // Waits until at most n stages' loads (kLoads each) of this wave are out, n <= kMost.
 template <int kMost, int kLoads>
@@ -186,7 +92,7 @@ window_tile_kernel(const WinArgs a) {
   }
   const int base = sq.ctx - sq.n;
   const int tile_pf = base + t0 / a.G, tile_pl = base + (min(sq.rows, t0 + TR) - 1) / a.G;
-  const Span span = span_of(tile_pf, tile_pl, a.window, a.sinks);
+  const Span span = span_of<kChunk>(tile_pf, tile_pl, a.window, a.sinks);
   const int c0 = part * a.part_chunks, c1 = min(span.n, c0 + a.part_chunks);
   if (c0 >= c1) return;
   const int nc = c1 - c0;
@@ -579,14 +485,14 @@ window_tile_kernel(const WinArgs a) {
   }
 }
 
-// The merge of tiles in several parts: one thread per (row, 4 dims), 8 parts loaded at a time.
+// The merge of the tile kernel's tiles in several parts: one thread per (row, 4 dims).
 template <int D>
 constexpr int merge_rows() { return 1024 / D; }
 
 template <typename Tag, int D, bool kF32>
 __global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs a, int32_t groups,
                                                            int32_t tile_rows) {
-  constexpr int TPR = D / 4, kBatch = 8;
+  constexpr int TPR = D / 4;
   const int item = blockIdx.x / groups, group = blockIdx.x % groups;
   const int pair = item / a.tiles, tile = item % a.tiles;
   const int b = pair / a.KVH, kvh = pair % a.KVH;
@@ -595,111 +501,93 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs a, int3
   const int r = t0 + lr, d = 4 * (threadIdx.x % TPR);
   if (sq.bad || t0 >= sq.rows) return;
   const int base = sq.ctx - sq.n;
-  const Span span = span_of(base + t0 / a.G, base + (min(sq.rows, t0 + tile_rows) - 1) / a.G,
-                            a.window, a.sinks);
+  const Span span = span_of<kChunk>(base + t0 / a.G, base + (min(sq.rows, t0 + tile_rows) - 1) / a.G,
+                                    a.window, a.sinks);
   const int np = (span.n + a.part_chunks - 1) / a.part_chunks;
   if (np <= 1 || lr >= tile_rows || r >= sq.rows) return;
-  const int64_t row0 = ((int64_t(pair) * a.tiles + tile) * a.parts) * tile_rows + lr;
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  float M = -INFINITY, L = 0.f;
-  f32x4 A = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int p0 = 0; p0 < np; p0 += kBatch) {
-    f32x4 va[kBatch];
-    f32x2 ml[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      va[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      ml[i] = f32x2{-INFINITY, 0.f};
-      if (p0 + i < np) {
-        const int64_t row = row0 + int64_t(p0 + i) * tile_rows;
-        va[i] = *reinterpret_cast<const f32x4*>(a.ws_acc + row * D + d);
-        ml[i] = *reinterpret_cast<const f32x2*>(a.ws_ml + 2 * row);
-      }
-    }
-    float bm = M;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) bm = fmaxf(bm, ml[i][0]);
-    const float Mu = bm == -INFINITY ? 0.f : bm;
-    const float keep = dsp_weight(M - Mu);
-    L *= keep;
-    A *= keep;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const float x = dsp_weight(ml[i][0] - Mu);
-      L = fmaf(ml[i][1], x, L);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) A[e] = fmaf(va[i][e], x, A[e]);
-    }
-    M = bm;
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int qi = r / a.G;
-  const int64_t o = int64_t(sq.q0 + qi) * a.ost + int64_t(kvh * a.G + r - qi * a.G) * a.osh + d;
-  A *= inv;
-  if constexpr (kF32) {
-    float* p = static_cast<float*>(a.out) + o;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = A[j];
-  } else {
-    uint16_t* p = static_cast<uint16_t*>(a.out) + o;
-    const uint32_t lo = narrow2<Tag>(A[0], A[1]), hi = narrow2<Tag>(A[2], A[3]);
-    if (a.vec_out) {
-      *reinterpret_cast<dsp_u32x2*>(p) = dsp_u32x2{lo, hi};
-    } else {
-      p[0] = uint16_t(lo);
-      p[1] = uint16_t(lo >> 16);
-      p[2] = uint16_t(hi);
-      p[3] = uint16_t(hi >> 16);
-    }
-  }
+  const int64_t row = int64_t(item) * a.parts * tile_rows + lr;
+  merge_row<Tag, D, kF32>(a, sq.q0, row, row + tile_rows, tile_rows, np, r, kvh, d);
 }
 
 // ---- which launch a shape takes
-struct WinPlan {
-  bool tile;  // the tile kernel (else, with a cache in q's type, the general one)
-  int rows, tiles, parts, part_chunks;
-};
-
 bool quantised(int32_t format) { return format == DSP_KV_FP8 || format == DSP_KV_FP4; }
 
 WinPlan win_plan(int32_t B, int32_t KVH, int32_t G, int32_t D, int32_t max_q_len, int32_t max_ctx,
-                 int32_t window, int32_t sinks, int32_t format, int32_t dtype) {
+                 int32_t window, int32_t sinks, int32_t format, int32_t dtype, bool may_stream) {
   WinPlan p{};
   if (!(D == 64 || D == 128 || D == 256) || (dtype == DSP_F32 && !quantised(format))) return p;
   const int64_t rows = int64_t(max_q_len) * G;
-  p.rows = D > 128 || rows <= 128 || dtype == DSP_F32 ? 128 : 256;
-  const int64_t tiles = (rows + p.rows - 1) / p.rows, pairs = int64_t(B) * KVH;
+  p.stream = may_stream && rows <= 64;
+  p.rows = p.stream ? (rows <= 16 || D > 128 || dtype == DSP_F32 ? 16 : 32)
+                    : D > 128 || rows <= 128 || dtype == DSP_F32 ? 128 : 256;
+  const int size = p.stream ? kStreamChunk : kChunk;
+  const int64_t tiles = (rows + p.rows - 1) / p.rows;
   // chunks that a tile can have: its queries' windows side by side, anywhere in a chunk; the sinks'
-  int64_t chunks = (int64_t(max_ctx) + kChunk - 1) / kChunk;
+  int64_t chunks = (int64_t(max_ctx) + size - 1) / size;
   if (window > 0) {
     const int64_t queries = std::min<int64_t>(max_q_len, p.rows / G + 2);
-    chunks = std::min(chunks, (int64_t(window) + queries) / kChunk + 2 +
-                                  (int64_t(sinks) + kChunk - 1) / kChunk);
+    chunks = std::min(chunks, (int64_t(window) + queries) / size + 2 + (int64_t(sinks) + size - 1) / size);
   }
-  const int64_t slots = int64_t(dsp_detail::device_cus()) * (p.rows == 128 && D <= 128 ? 2 : 1);
-  const int64_t total = std::max<int64_t>(tiles * pairs, 1);
-  int64_t parts = total >= slots ? 1 : slots / total;
-  parts = std::max<int64_t>(1, std::min(parts, chunks / 2));
-  p.part_chunks = int((chunks + parts - 1) / parts);
-  p.parts = int((chunks + p.part_chunks - 1) / p.part_chunks);
+  const int64_t cus = dsp_detail::device_cus(), all = int64_t(B) * KVH;
+  int64_t workgroups;
+  if (p.stream) {
+    // In steps of 1.6 us, a wave's chunk of 128 dims for 16 rows: a round of whole tiles takes its start,
+    // 2.5, and the chunks of a split; equal runs their start, the scan and the merge, 10, and the
+    // chip's share.
+    const int waves = stream_block(D), most = dsp_detail::balanced_head_group(KVH);
+    const double step = (D > 128 ? 2.0 : D > 64 ? 1.0 : 0.7) * (p.rows > 16 ? 1.5 : 1.0);
+    double best = 10.0 + step * double(tiles * all * chunks) / double(cus * waves);
+    bool whole = false;
+    p.heads = most;
+    for (int h = 1; h <= std::min(most, waves); h *= 2) {
+      const int64_t rounds = (tiles * (all / h) + cus - 1) / cus, splits = waves / h;
+      const double cost = double(rounds) * (2.5 + step * double((chunks + splits - 1) / splits));
+      if (cost < best) {
+        best = cost;
+        whole = true;
+        p.heads = h;
+      }
+    }
+    const int splits = waves / p.heads;
+    p.start = splits;
+    p.least = 2 * splits + p.start;
+    const int64_t total = tiles * (all / p.heads), units = total * (chunks + p.start);
+    p.runs = whole ? 0 : int(std::min(cus, (units + p.least - 1) / p.least));
+    // 128 MiB of K and V, half of the last-level cache, behind which the next call finds little of its
+    // own: 1.1 GB of fp8 195 us (204 by ordinary loads), 134 MB 29.6 (30.5); 102 MB 35 (30).
+    const int64_t row = format == DSP_KV_FP8 ? D : format == DSP_KV_FP4 ? D / 2 : 2 * D;
+    p.once = all * chunks * size * 2 * row >= (int64_t(128) << 20);
+    workgroups = whole ? total + 8 * tiles : p.runs;
+    p.tile = units < (int64_t(1) << 31) && rows < (int64_t(1) << 30);
+  } else {
+    const int64_t slots = cus * (p.rows == 128 && D <= 128 ? 2 : 1);
+    const int64_t total = std::max<int64_t>(tiles * all, 1);
+    int64_t parts = total >= slots ? 1 : slots / total;
+    parts = std::max<int64_t>(1, std::min(parts, chunks / 2));
+    p.part_chunks = int((chunks + parts - 1) / parts);
+    p.parts = int((chunks + p.part_chunks - 1) / p.part_chunks);
+    workgroups = (all + 8) * tiles * p.parts;
+    p.tile = rows < (int64_t(1) << 30);
+  }
   p.tiles = int(tiles);
-  // (32 bits number the workgroups)
-  p.tile = rows < (int64_t(1) << 30) && (pairs + 8) * tiles * p.parts < (int64_t(1) << 31);
+  p.tile = p.tile && workgroups < (int64_t(1) << 31);  // (32 bits number the workgroups)
   return p;
 }
 
 size_t win_bytes(const WinPlan& p, int64_t pairs, int32_t D) {
-  return p.parts <= 1 ? 0
-                      : size_t(pairs) * p.tiles * p.parts * p.rows * (size_t(D) + 2) * sizeof(float);
+  if (!p.tile) return 0;
+  if (p.stream)
+    return size_t(p.runs) * (size_t(2) * p.heads * p.rows * (D + 2) + kDesc) * sizeof(float);
+  return p.parts <= 1 ? 0 : size_t(pairs) * p.tiles * p.parts * p.rows * (size_t(D) + 2) * sizeof(float);
 }
 
 template <typename Tag, int D, int kFmt, bool kF32>
 int launch_window(const WinPlan& p, const WinArgs& a, hipStream_t s) {
   const int64_t pairs = int64_t(a.B) * a.KVH, per = int64_t(p.tiles) * p.parts;
-  const int64_t grid = pairs >= 8 ? (pairs + 7) / 8 * 8 * per : (pairs * per + 7) / 8 * 8;
+  const unsigned grid = unsigned(pairs >= 8 ? (pairs + 7) / 8 * 8 * per : (pairs * per + 7) / 8 * 8);
   auto launch = [&](auto shape) {
     using S = decltype(shape);
-    window_tile_kernel<Tag, D, kFmt, kF32, S><<<unsigned(grid), 64 * S::NW, 0, s>>>(a);
+    window_tile_kernel<Tag, D, kFmt, kF32, S><<<grid, 64 * S::NW, 0, s>>>(a);
   };
   if constexpr (kF32 || D == 256) {
     launch(Shape<4, 2, 1>{});
@@ -711,8 +599,7 @@ int launch_window(const WinPlan& p, const WinArgs& a, hipStream_t s) {
   if (st != DSP_OK || p.parts <= 1) return st;
   const int64_t most = std::min<int64_t>(int64_t(a.max_q_len) * a.G, p.rows);
   const int groups = int((most + merge_rows<D>() - 1) / merge_rows<D>());
-  window_merge_kernel<Tag, D, kF32>
-      <<<unsigned(pairs * p.tiles * groups), 256, 0, s>>>(a, groups, p.rows);
+  window_merge_kernel<Tag, D, kF32><<<unsigned(pairs * p.tiles * groups), 256, 0, s>>>(a, groups, p.rows);
   return dsp_launch_status();
 }
 
@@ -751,10 +638,13 @@ extern "C" size_t dsp_paged_window_workspace_bytes(int32_t B, int32_t Hq, int32_
   if (B <= 0 || KVH <= 0 || Hq <= 0 || Hq % KVH != 0 || max_q_len <= 0 || max_ctx <= 0 ||
       window < 0 || sinks < 0)
     return 0;
-  const WinPlan p = win_plan(B, KVH, Hq / KVH, D, max_q_len, max_ctx, window, sinks, format, dtype);
-  const size_t tile = p.tile ? win_bytes(p, int64_t(B) * KVH, D) : 0;
+  size_t tile = 0;
+  for (bool stream : {false, true})
+    tile = std::max(tile, win_bytes(win_plan(B, KVH, Hq / KVH, D, max_q_len, max_ctx, window, sinks,
+                                             format, dtype, stream),
+                                    int64_t(B) * KVH, D));
   if (quantised(format)) return tile;
-  // (either launch's: which one a call takes goes by its strides too)
+  // (any launch's: which one a call takes goes by its strides too)
   return std::max(tile, dsp_detail::generic_workspace_bytes(
                             B, Hq, D, max_q_len, general_span(max_q_len, max_ctx, window, sinks),
                             general_partition(B, Hq, KVH, D, max_q_len, max_ctx, window, sinks)));
@@ -788,7 +678,15 @@ extern "C" int dsp_paged_window_attention(
   // (a window that reaches past every context is none)
   const bool all = window == 0 || window >= max_ctx;
   const int32_t win = all ? kWholeWindow : window, sink = all ? 0 : std::min(sinks, max_ctx);
-  const WinPlan p = win_plan(B, KVH, G, D, max_q_len, max_ctx, window, sinks, format, dtype);
+  const int64_t scale_bytes = D / dsp_quant::kGroup;
+  const bool scales_ok =
+      !quant || (scale_stride_slot >= 0 && scale_stride_slot < (int64_t(1) << 26) &&
+                 scale_stride_slot % scale_bytes == 0 && scale_stride_head % scale_bytes == 0 &&
+                 dsp_aligned(k_scale, scale_bytes) && dsp_aligned(v_scale, scale_bytes));
+  const bool rows16 = kv_stride_slot_bytes % 16 == 0 && kv_stride_head_bytes % 16 == 0 &&
+                      dsp_aligned(k_cache, 16) && dsp_aligned(v_cache, 16);
+  const WinPlan p = win_plan(B, KVH, G, D, max_q_len, max_ctx, window, sinks, format, dtype,
+                             rows16 && scales_ok);
   const int32_t row_align = quant ? (format == DSP_KV_FP8 ? 16 : 8) : 16;
   const int64_t q_align = dtype == DSP_F32 ? 1 : 8;
   const bool tile =
@@ -822,15 +720,21 @@ extern "C" int dsp_paged_window_attention(
   DSP_HOST_CHECK(workspace_bytes >= need && (need == 0 || workspace != nullptr), DSP_EWORKSPACE);
   DSP_HOST_CHECK(need == 0 || dsp_aligned(workspace, 16), DSP_EALIGN);
   float* ws = static_cast<float*>(workspace);
-  const int64_t part_rows = int64_t(B) * KVH * p.tiles * p.parts * p.rows;
+  const int64_t part_rows = p.stream ? int64_t(2) * p.runs * p.heads * p.rows
+                                     : int64_t(B) * KVH * p.tiles * p.parts * p.rows;
+  float* const ws_ml = ws + part_rows * D;
   const WinArgs a{q, q_stride_t, q_stride_h, static_cast<const char*>(k_cache),
                   static_cast<const char*>(v_cache), k_scale, v_scale,
                   uint32_t(num_slots / block_size), kv_stride_slot_bytes, kv_stride_head_bytes,
                   scale_stride_slot, scale_stride_head, block_table, bt_stride,
                   dsp_log2i(block_size), cu_q, ctx_lens, B, KVH, G, max_q_len, max_ctx, win, sink,
-                  scale * 1.4426950408889634f, p.tiles, p.parts, p.part_chunks, ws,
-                  p.parts > 1 ? ws + part_rows * D : nullptr, out, o_stride_t, o_stride_h,
+                  scale * 1.4426950408889634f, p.tiles, p.parts, p.part_chunks, p.heads, p.runs,
+                  p.least, p.start, (65536 + G - 1) / G, reinterpret_cast<int32_t*>(ws_ml + 2 * part_rows), ws, ws_ml, out, o_stride_t, o_stride_h,
                   o_stride_t % 4 == 0 && o_stride_h % 4 == 0 && dsp_aligned(out, 8), err_count};
+  if (p.stream)
+    return format == DSP_KV_FP8   ? stream_fp8(D, dtype, p, a, s)
+           : format == DSP_KV_FP4 ? stream_fp4(D, dtype, p, a, s)
+                                  : stream_plain(D, dtype, p, a, s);
   if (D == 64) return launch_format<64>(format, dtype, p, a, s);
   if (D == 128) return launch_format<128>(format, dtype, p, a, s);
   return launch_format<256>(format, dtype, p, a, s);

@@ -1,0 +1,7 @@
+// The stream kernel of window_stream.h over e4m3 caches.
+#include "window_stream.h"
+
+int dsp_window::stream_fp8(int32_t D, int32_t dtype, const WinPlan& p, const WinArgs& a,
+                           hipStream_t s) {
+  return stream_format<kFp8>(D, dtype, p, a, s);
+}

@@ -380,66 +380,84 @@ def window_workspace(batch, num_heads, num_kv_heads, head_dim, max_q_len, max_ct
     return torch.empty(need // 4 + 1, dtype=torch.float32, device=device) if need else None
 
 
-def _windowed(q, k_cache, v_cache, scales, fmt, block_table, cu_q, ctx_lens, kv_groups, window, sinks,
-              block_size, scale, max_q_len, max_ctx, out, err, workspace):
-    k_scale, v_scale = scales
-    _lib.one_gpu(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, ctx_lens, out, err, workspace)
-    if q.dim() != 3 or k_cache.dim() != 3 or v_cache.shape != k_cache.shape:
+def _windowed(q, k_cache, v_cache, k_scale, v_scale, fmt, block_table, cu_q, ctx_lens, kv_groups,
+              window, sinks, block_size, scale, max_q_len, max_ctx, out, err, workspace):
+    # (a decode step calls this once per layer: each attribute of a tensor is read once)
+    q_shape, k_shape, k_stride, v_stride = q.shape, k_cache.shape, k_cache.stride(), v_cache.stride()
+    if len(q_shape) != 3 or len(k_shape) != 3 or v_cache.shape != k_shape:
         raise ValueError(f"expected q (T, Hq, D) and caches (S, KVH, width); got {tuple(q.shape)}, "
                          f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
-    T, Hq, D = q.shape
-    S, KVH, width = k_cache.shape
+    T, Hq, D = q_shape
+    S, KVH, width = k_shape
     if width != (D // 2 if fmt == _lib.DSP_KV_FP4 else D) or Hq != KVH * kv_groups:
         raise ValueError(f"q has {Hq} heads of {D}, cache {KVH} heads of width {width}, kv_groups "
                          f"{kv_groups}")
-    if k_cache.stride() != v_cache.stride() or k_cache.stride(2) != 1:
+    if k_stride != v_stride or k_stride[2] != 1:
         raise ValueError("k_cache and v_cache need the same strides with head_dim contiguous")
-    window, sinks = int(window), int(sinks)
     if window < 0 or sinks < 0 or sinks and not window:
         raise ValueError(f"window {window} with {sinks} sinks: a window of 0 (the whole context) or "
                          "more, sinks beside a window only")
-    if q.stride(2) != 1:
+    q_stride = q.stride()
+    if q_stride[2] != 1:
         q = q.contiguous()
-    ctx_lens, block_table = _i32(ctx_lens), _i32(block_table)
-    B = ctx_lens.numel()
+        q_stride = q.stride()
+    ctx_lens, block_table, B = _i32(ctx_lens), _i32(block_table), ctx_lens.numel()
+    table = block_table.shape
     if cu_q is None:
         if T != B:
             raise ValueError(f"q has {T} rows for {B} sequences: without cu_q one query a sequence")
-        max_q_len = min(B, 1)
+        max_q_len, cu_ptr = min(B, 1), None
     else:
         cu_q = _i32(cu_q)
-    if (cu_q is not None and cu_q.numel() != B + 1 or block_table.dim() != 2
-            or block_table.shape[0] != B):
+        cu_ptr = cu_q.data_ptr()
+    if len(table) != 2 or table[0] != B or cu_q is not None and cu_q.numel() != B + 1:
         raise ValueError(f"cu_q has {None if cu_q is None else cu_q.numel()} entries, block_table shape "
                          f"{tuple(block_table.shape)} for {B} sequences")
     if max_q_len is None:
         max_q_len = int((cu_q[1:] - cu_q[:-1]).max().item()) if B else 0
+    cols = table[1]
     if max_ctx is None:
-        max_ctx = block_table.shape[1] * block_size
-    max_q_len, max_ctx = int(max_q_len), int(max_ctx)
-    if max_ctx > block_table.shape[1] * block_size:
-        raise ValueError(f"max_ctx {max_ctx} exceeds the table's {block_table.shape[1]} blocks")
-    scale = D ** -0.5 if scale is None else scale
-    out = torch.empty_like(q) if out is None else out
-    if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        max_ctx = cols * block_size
+    elif max_ctx > cols * block_size:
+        raise ValueError(f"max_ctx {max_ctx} exceeds the table's {cols} blocks")
+    if scale is None:
+        scale = D ** -0.5
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q_shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ValueError("out must have q's shape and dtype with head_dim contiguous")
+    o_stride = out.stride()
+    dev = _lib.same_gpu(q, k_cache, v_cache, block_table, ctx_lens, cu_q, k_scale, v_scale, out, err,
+                        workspace)
     if not (T and B and max_q_len):   # (rows behind the last sequence stay as they are)
         return out
     dtype, es = _lib.dtype_code(q.dtype), k_cache.element_size()
-    need = _window_ws_bytes(q.get_device(), B, Hq, KVH, D, max_q_len, max_ctx, window, sinks, fmt, dtype)
+    need = _window_ws_bytes(dev, B, Hq, KVH, D, max_q_len, max_ctx, window, sinks, fmt, dtype)
+    stream = _lib.stream_of(q)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        # (from torch's stream-ordered allocator, per call)
-        workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
-    with _lib.on_device(q):
-        _lib.check(_lib.calls().dsp_paged_window_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), S,
-            k_cache.stride(0) * es, k_cache.stride(1) * es, _lib.ptr(k_scale), _lib.ptr(v_scale),
-            0 if k_scale is None else k_scale.stride(0), 0 if k_scale is None else k_scale.stride(1),
-            fmt, block_table.data_ptr(), block_table.stride(0), block_size, _lib.ptr(cu_q),
-            ctx_lens.data_ptr(), B, Hq, KVH, D, float(scale), window, sinks, max_q_len, max_ctx,
-            _lib.ptr(workspace), need, out.data_ptr(), out.stride(0), out.stride(1), dtype,
-            _lib.ptr(err), _lib.stream_of(q)), "dsp_paged_window_attention")
+        # (large ones from torch's stream-ordered allocator, per call)
+        workspace = (_workspace(need, q.device, stream) if need <= _KEPT_BYTES
+                     else torch.empty(need // 4, dtype=torch.float32, device=q.device))
+    if k_scale is None:
+        ks_ptr = vs_ptr = None
+        s_slot = s_head = 0
+    else:
+        ks_ptr, vs_ptr = k_scale.data_ptr(), v_scale.data_ptr()
+        s_slot, s_head, _ = k_scale.stride()
+    args = (q.data_ptr(), q_stride[0], q_stride[1], k_cache.data_ptr(), v_cache.data_ptr(), S,
+            k_stride[0] * es, k_stride[1] * es, ks_ptr, vs_ptr, s_slot, s_head, fmt,
+            block_table.data_ptr(), block_table.stride(0), block_size, cu_ptr, ctx_lens.data_ptr(), B, Hq,
+            KVH, D, scale, window, sinks, max_q_len, max_ctx, workspace.data_ptr() if need else None, need,
+            out.data_ptr(), o_stride[0], o_stride[1], dtype, None if err is None else err.data_ptr(),
+            stream)
+    status = _lib.call_on(dev, _lib.calls().dsp_paged_window_attention, args)
+    if status:
+        _lib.check(status, "dsp_paged_window_attention")
     return out
+
+
+# workspaces of calls that bring none are kept, one per stream, up to so many bytes
+_KEPT_BYTES = 32 << 20
 
 
 def paged_window_attention(q, k_cache, v_cache, block_table, cu_q, ctx_lens, kv_groups, window=0,
@@ -463,10 +481,10 @@ def paged_window_attention(q, k_cache, v_cache, block_table, cu_q, ctx_lens, kv_
     err:         optional int32 device counter of bad lengths and block ids
     returns:     (sum q_len, num_heads, head_dim) in q's dtype
     """
-    if q.dtype not in _DTYPES or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    if not q.dtype == k_cache.dtype == v_cache.dtype or q.dtype not in _DTYPES:
         raise ValueError(f"q/k/v dtypes {q.dtype}/{k_cache.dtype}/{v_cache.dtype}: "
                          "the HIP kernels take bf16, fp16 or fp32, all the same")
-    return _windowed(q, k_cache, v_cache, (None, None), _lib.DSP_KV_PLAIN, block_table, cu_q, ctx_lens,
+    return _windowed(q, k_cache, v_cache, None, None, _lib.DSP_KV_PLAIN, block_table, cu_q, ctx_lens,
                      kv_groups, window, sinks, block_size, scale, max_q_len, max_ctx, out, err,
                      workspace)
 
@@ -479,22 +497,24 @@ def paged_quant_attention(q, k_cache, k_scale, v_cache, v_scale, block_table, cu
     v_scale (S, KVH, head_dim / 32) uint8.  q in bf16, fp16 or fp32, head_dim 64, 128 or 256; the
     cache's numbers count as `quant_gather` gives them in q's dtype; scale > 0.
     """
-    if q.dtype not in _DTYPES or any(t.dtype != torch.uint8 for t in (k_cache, k_scale, v_cache, v_scale)):
+    if (q.dtype not in _DTYPES
+            or not k_cache.dtype == v_cache.dtype == k_scale.dtype == v_scale.dtype == torch.uint8):
         raise ValueError(f"q {q.dtype}, codes {k_cache.dtype}/{v_cache.dtype}, scales {k_scale.dtype}/"
                          f"{v_scale.dtype}: q in bf16, fp16 or fp32, codes and scales in uint8")
-    D = q.shape[-1]
-    rows = k_cache.shape[:-1] + (D // 32,)
-    if D not in (64, 128, 256) or k_scale.shape != rows or v_scale.shape != rows:
+    D, codes, scales = q.shape[-1], k_cache.shape, k_scale.shape
+    if (D not in (64, 128, 256) or len(scales) != 3 or len(codes) != 3 or v_scale.shape != scales
+            or scales[0] != codes[0] or scales[1] != codes[1] or scales[2] * 32 != D):
         raise ValueError(f"scales {tuple(k_scale.shape)}, {tuple(v_scale.shape)} for codes "
                          f"{tuple(k_cache.shape)} and head_dim {D}: one for 32 elements, head_dim 64, "
                          "128 or 256")
-    if k_scale.stride() != v_scale.stride() or k_scale.stride(2) != 1:
+    strides = k_scale.stride()
+    if strides != v_scale.stride() or strides[2] != 1:
         raise ValueError("k_scale and v_scale need the same strides with a head's scales contiguous")
     if scale is not None and not 0 < scale < float("inf"):
         raise ValueError(f"scale {scale}: positive and finite over a quantised cache")
-    fmt = _lib.DSP_KV_FP4 if 2 * k_cache.shape[-1] == D else _lib.DSP_KV_FP8
-    return _windowed(q, k_cache, v_cache, (k_scale, v_scale), fmt, block_table, cu_q, ctx_lens,
-                     kv_groups, window, sinks, block_size, scale, max_q_len, max_ctx, out, err,
+    return _windowed(q, k_cache, v_cache, k_scale, v_scale,
+                     _lib.DSP_KV_FP4 if 2 * codes[2] == D else _lib.DSP_KV_FP8, block_table, cu_q,
+                     ctx_lens, kv_groups, window, sinks, block_size, scale, max_q_len, max_ctx, out, err,
                      workspace)
 
 

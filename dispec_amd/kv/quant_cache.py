@@ -31,27 +31,29 @@ def code_width(format: str, head_dim: int) -> int:
 def _pools(k_cache, k_scale, v_cache, v_scale):
     """(format, layers, slots, KVH, D, and code and scale strides of a layer and a slot) of pools
     (S, KVH, width) of one layer or (L, S, KVH, width) of all."""
-    shape, stride, scales = k_cache.shape, k_cache.stride(), k_scale.stride()
+    shape, stride, scales, s_stride = (k_cache.shape, k_cache.stride(), k_scale.shape,
+                                       k_scale.stride())
+    if not k_cache.dtype == k_scale.dtype == v_cache.dtype == v_scale.dtype == torch.uint8:
+        raise ValueError(f"codes and scales must be uint8, got {k_cache.dtype}, {k_scale.dtype}, "
+                         f"{v_cache.dtype}, {v_scale.dtype}")
     n = len(shape)
-    for t in (k_cache, k_scale, v_cache, v_scale):
-        if t.dtype != torch.uint8:
-            raise ValueError(f"codes and scales must be uint8, got {t.dtype}")
-    if n not in (3, 4) or v_cache.shape != shape or k_scale.shape != v_scale.shape:
+    if n not in (3, 4) or len(scales) != n or v_cache.shape != shape or v_scale.shape != scales:
         raise ValueError(f"expected codes (S, KVH, width) or (L, S, KVH, width) and scales alike for K "
-                         f"and V; got {tuple(shape)}, {tuple(v_cache.shape)}, {tuple(k_scale.shape)}, "
+                         f"and V; got {tuple(shape)}, {tuple(v_cache.shape)}, {tuple(scales)}, "
                          f"{tuple(v_scale.shape)}")
-    KVH, width = shape[-2:]
-    D = GROUP * k_scale.shape[-1]
-    if k_scale.shape[:-1] != shape[:-1] or width not in (D, D // 2):
-        raise ValueError(f"scales {tuple(k_scale.shape)} for codes {tuple(shape)}: one for {GROUP} "
-                         "elements of a byte or half a byte")
-    if (v_cache.stride() != stride or v_scale.stride() != scales or stride[-1] != 1
-            or stride[-2] != width and KVH > 1 or scales[-1] != 1
-            or scales[-2] != D // GROUP and KVH > 1):
+    S, KVH, width = shape[-3:]
+    groups = scales[-1]
+    D = GROUP * groups
+    if scales[-2] != KVH or scales[-3] != S or scales[0] != shape[0] or width != D and 2 * width != D:
+        raise ValueError(f"scales {tuple(scales)} for codes {tuple(shape)}: one for {GROUP} elements of "
+                         "a byte or half a byte")
+    if (v_cache.stride() != stride or v_scale.stride() != s_stride or stride[-1] != 1
+            or s_stride[-1] != 1 or (stride[-2] != width or s_stride[-2] != groups) and KVH > 1):
         raise ValueError("codes and scales need the same strides for K and V with contiguous rows")
     fmt = _lib.DSP_KV_FP8 if width == D else _lib.DSP_KV_FP4
-    layers, layer, scale_layer = (1, 0, 0) if n == 3 else (shape[0], stride[0], scales[0])
-    return fmt, layers, shape[-3], KVH, D, (layer, stride[-3], scale_layer, scales[-3])
+    if n == 3:
+        return fmt, 1, S, KVH, D, (0, stride[0], 0, s_stride[0])
+    return fmt, shape[0], S, KVH, D, (stride[0], stride[1], s_stride[0], s_stride[1])
 
 
 def quant_append(k_cache, k_scale, v_cache, v_scale, slots, k, v, err=None) -> None:
@@ -70,30 +72,37 @@ def quant_append(k_cache, k_scale, v_cache, v_scale, slots, k, v, err=None) -> N
     are first clamped to +-61440 ("fp8") or +-49152 ("fp4"), so that they read back finite.  A group
     with an infinity or NaN reads back as NaN.
     """
-    _lib.one_gpu(k_cache, k_scale, v_cache, v_scale, slots, k, v, err)
     fmt, L, S, KVH, D, strides = _pools(k_cache, k_scale, v_cache, v_scale)
-    T = slots.numel()
-    rows = ((L,) if k_cache.dim() == 4 else ()) + (T, KVH, D)
-    if k.shape != rows or v.shape != rows:
-        raise ValueError(f"k, v have shapes {tuple(k.shape)}, {tuple(v.shape)}: expected {rows}")
-    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+    T, rows = slots.numel(), k.shape
+    n = len(rows)
+    if (n != k_cache.dim() or v.shape != rows or rows[-1] != D or rows[-2] != KVH or rows[-3] != T
+            or n == 4 and rows[0] != L):
+        raise ValueError(f"k, v have shapes {tuple(k.shape)}, {tuple(v.shape)}: expected "
+                         f"{((L,) if k_cache.dim() == 4 else ()) + (T, KVH, D)}")
+    dtype = k.dtype
+    if v.dtype != dtype or dtype not in _DTYPES:
         raise ValueError(f"k/v dtypes {k.dtype}/{v.dtype}: bf16, fp16 or fp32, both the same")
     if slots.dtype != torch.int64:
         raise ValueError(f"slots must be int64, got {slots.dtype}")
+    dev = _lib.same_gpu(k_cache, k_scale, v_cache, v_scale, slots, k, v, err)
     if not (T and L):
         return
-    if k.stride(-1) != 1:
-        k = k.contiguous()
-    if v.stride(-1) != 1:
-        v = v.contiguous()
-    slots = slots.contiguous()
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
     ks, vs = k.stride(), v.stride()
-    with _lib.on_device(k_cache):
-        _lib.check(_lib.calls().dsp_kv_append_quant(
-            k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), L, *strides,
-            S, k.data_ptr(), ks[0] if len(ks) == 4 else 0, ks[-3], ks[-2], v.data_ptr(),
-            vs[0] if len(vs) == 4 else 0, vs[-3], vs[-2], slots.data_ptr(), T, KVH, D, fmt,
-            _lib.dtype_code(k.dtype), _lib.ptr(err), _lib.stream_of(k_cache)), "dsp_kv_append_quant")
+    if ks[-1] != 1:
+        k = k.contiguous()
+        ks = k.stride()
+    if vs[-1] != 1:
+        v = v.contiguous()
+        vs = v.stride()
+    status = _lib.call_on(dev, _lib.calls().dsp_kv_append_quant, (
+        k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), L, *strides, S,
+        k.data_ptr(), ks[0] if n == 4 else 0, ks[-3], ks[-2], v.data_ptr(), vs[0] if n == 4 else 0,
+        vs[-3], vs[-2], slots.data_ptr(), T, KVH, D, fmt, _lib.dtype_code(dtype),
+        None if err is None else err.data_ptr(), _lib.stream_of(k_cache)))
+    if status:
+        _lib.check(status, "dsp_kv_append_quant")
 
 
 def quant_gather(k_cache, k_scale, v_cache, v_scale, slots, dtype=torch.bfloat16, err=None):
@@ -101,24 +110,25 @@ def quant_gather(k_cache, k_scale, v_cache, v_scale, slots, dtype=torch.bfloat16
     head_dim), or (L, T, KVH, head_dim) of pools of all layers, rounded to `dtype` (which loses
     nothing in bf16 and fp32, and in fp16 where the rows were written from fp16).  Arguments as for
     `quant_append`; a slot outside the pool leaves its rows undefined."""
-    _lib.one_gpu(k_cache, k_scale, v_cache, v_scale, slots, err)
     fmt, L, S, KVH, D, strides = _pools(k_cache, k_scale, v_cache, v_scale)
     if dtype not in _DTYPES:
         raise ValueError(f"values in bf16, fp16 or fp32, not {dtype}")
     if slots.dtype != torch.int64:
         raise ValueError(f"slots must be int64, got {slots.dtype}")
+    dev = _lib.same_gpu(k_cache, k_scale, v_cache, v_scale, slots, err)
     T = slots.numel()
-    rows = ((L,) if k_cache.dim() == 4 else ()) + (T, KVH, D)
-    k = torch.empty(rows, dtype=dtype, device=k_cache.device)
+    k = k_cache.new_empty((T, KVH, D) if k_cache.dim() == 3 else (L, T, KVH, D), dtype=dtype)
     v = torch.empty_like(k)
     if not (T and L):
         return k, v
-    slots = slots.contiguous()
-    with _lib.on_device(k_cache):
-        _lib.check(_lib.calls().dsp_kv_gather_quant(
-            k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), L, *strides,
-            S, slots.data_ptr(), T, KVH, D, fmt, k.data_ptr(), v.data_ptr(), _lib.dtype_code(dtype),
-            _lib.ptr(err), _lib.stream_of(k_cache)), "dsp_kv_gather_quant")
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
+    status = _lib.call_on(dev, _lib.calls().dsp_kv_gather_quant, (
+        k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), L, *strides, S,
+        slots.data_ptr(), T, KVH, D, fmt, k.data_ptr(), v.data_ptr(), _lib.dtype_code(dtype),
+        None if err is None else err.data_ptr(), _lib.stream_of(k_cache)))
+    if status:
+        _lib.check(status, "dsp_kv_gather_quant")
     return k, v
 
 

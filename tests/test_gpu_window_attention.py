@@ -80,15 +80,16 @@ def test_one_query_a_sequence_without_offsets(hip, D, dtype, fmt):
     ctx = [1, 17, 900, 64, 2000]
     for window, sinks in ((0, 0), (33, 2), (600, 4)):
         c = Case([1] * 5, ctx, 8, 2, D, dtype, window, sinks, seed=5, fmt=fmt)
-        got = c.call(cu=None)
-        c.check(got)
+        c.check(c.call(cu=None))
         # a sequence without a context: zeros, not counted; a bad one: zeros, counted
         err = torch.zeros(1, dtype=torch.int32, device=DEV)
         c.lens[0], c.lens[3] = 0, c.max_ctx + 1
         out = c.call(cu=None, err=err, out=torch.full_like(c.dq, 9.0))
         assert int(err) == 1 and not out[0].any() and not out[3].any()
+        # (the others' parts are cut elsewhere now: the same to rounding)
         keep = [1, 2, 4]
-        assert torch.equal(out[keep], got[keep])
+        o, A = c.reference()
+        c.check(out[keep], o[keep], A[keep])
 
 
 @pytest.mark.parametrize("fmt", [None, "fp8", "fp4"])
