@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from dispec_amd import _lib
+from dispec_amd.kv.paged_cache import PagedKVCache
 
 
 def _rms_weight(norm):
@@ -21,6 +22,28 @@ def _rms_weight(norm):
     if eps is None:
         raise ValueError(f"{type(norm).__name__}: no epsilon attribute (variance_epsilon / eps)")
     return norm.weight, float(eps)
+
+
+class ScratchRows:
+    """Rows that the prologue kernel appends to as to a cache layer's slots: for one stream at a
+    time, to be taken from before the next layer's come."""
+
+    def __init__(self, k: torch.Tensor):
+        self.key = torch.empty((1, *k.shape), dtype=k.dtype, device=k.device)
+        self.value = torch.empty_like(self.key)
+        self.slots = torch.arange(k.shape[0], device=k.device)
+        self._err = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._as_slots, self._after = PagedKVCache._as_slots, lambda: None
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+                 sin: torch.Tensor, q_norm=None, k_norm=None,
+                 rows: ScratchRows | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """`qk_norm_rope_append` without a cache: the normalised and rotated q and k (in `rows`, where it
+    is given), for a cache that takes its rows in another form (kv.quant_cache)."""
+    rows = ScratchRows(k) if rows is None else rows
+    q = qk_norm_rope_append(q, k, v, cos, sin, rows.slots, rows, 0, q_norm, k_norm)
+    return q, rows.key[0]
 
 
 def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,

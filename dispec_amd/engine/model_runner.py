@@ -18,6 +18,11 @@ the HF modules, unchanged.  What the backend replaces is the KV path inside `_at
                                         blocks (copy-on-write forks of one prompt,
                                         prefix-cache hits) the shared-prefix variant
                                         attends those blocks once for the whole batch
+  * a layer with a sliding window       -> dsp_paged_window_attention, decode and everything else
+    (the model's own, or the runner's   alike: the keys outside the window are not read
+    with its sinks)
+  * a quantised cache                   -> dsp_kv_append_quant after the prologue, and
+    (kv.quant_cache)                     dsp_paged_window_attention over the codes
   * a batch with drafted trees         -> dsp_paged_tree_attention, one launch for the whole
     (SeqMeta.parents)                   batch, each node with its ancestors (the reference
                                         drafts chains); the logits then go to verify_draft or
@@ -43,10 +48,12 @@ import torch.nn.functional as F
 from dispec_amd import _lib
 from dispec_amd.engine.hip_attn import (decode_workspace, mq_workspace,
                                        paged_decode_attention_blocks, paged_mq_attention,
-                                       paged_tree_attention, tree_mask, tree_workspace)
-from dispec_amd.engine.hip_prologue import qk_norm_rope_append
+                                       paged_quant_attention, paged_tree_attention,
+                                       paged_window_attention, tree_mask, tree_workspace)
+from dispec_amd.engine.hip_prologue import ScratchRows, qk_norm_rope, qk_norm_rope_append
 from dispec_amd.engine.hip_verify import MAX_TREE_NODES
 from dispec_amd.kv.paged_cache import PagedKVCache
+from dispec_amd.kv.quant_cache import QuantPagedKVCache
 
 
 @dataclass
@@ -81,6 +88,7 @@ class _Batch:
     balanced: bool = False   # short query blocks on the balanced split-K kernel
     seqs: tuple = ()         # the host SeqMeta list (attn_backend="native" walks it)
     tree_mask: torch.Tensor | None = None   # of a batch with drafted trees (see tree_mask)
+    rows: ScratchRows | None = None         # quantised caches: a layer's rotated k on its way there
 
 
 _BACKENDS = ("hip", "native")
@@ -105,7 +113,13 @@ class _FusedLayer:
 
 
 class ModelRunner:
-    def __init__(self, model, attn_backend: str = "hip", fuse: bool = False):
+    """window, sinks: a sliding window of so many tokens (0: none), with the first `sinks` tokens of a
+    sequence visible beside it, for the layers that have none of their own; layers that the model's
+    config calls "sliding_attention" have its sliding_window.  Blocks that hold no visible token may be
+    freed (their table entries are not read)."""
+
+    def __init__(self, model, attn_backend: str = "hip", fuse: bool = False, window: int = 0,
+                 sinks: int = 0):
         if attn_backend not in _BACKENDS:
             hint = (" (the Triton decode kernel is replaced by this package's HIP kernels: "
                     "use attn_backend='hip')" if attn_backend == "triton" else "")
@@ -125,9 +139,21 @@ class ModelRunner:
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.num_heads
         self.kv_groups = self.num_heads // self.num_kv_heads
         self.scale = 1.0 / self.head_dim ** 0.5
-        if "sliding_attention" in (getattr(cfg, "layer_types", None) or ()):
-            raise ValueError(f"{type(model).__name__} uses sliding-window attention layers, which "
-                             "the paged attention path does not implement")
+        if window < 0 or sinks < 0 or sinks and not window:
+            raise ValueError(f"window {window} with {sinks} sinks: sinks go with a window")
+        kinds = list(getattr(cfg, "layer_types", None) or ())
+        kinds += ["full_attention"] * (len(self.layers) - len(kinds))
+        unknown = set(kinds) - {"full_attention", "sliding_attention"}
+        if unknown:
+            raise ValueError(f"{type(model).__name__} uses {sorted(unknown)} layers, which the paged "
+                             "attention path does not implement")
+        own = getattr(cfg, "sliding_window", None)
+        if "sliding_attention" in kinds and not own:
+            raise ValueError(f"{type(model).__name__}: sliding_attention layers without a "
+                             "sliding_window")
+        # (window, sinks) of each layer; window 0: the whole context
+        self.windows = [(int(own), 0) if kind == "sliding_attention" else (int(window), int(sinks))
+                        for kind in kinds[:len(self.layers)]]
         first = self.layers[0].self_attn
         self.qk_norm = all(hasattr(first, n) for n in ("q_norm", "k_norm"))   # Qwen3
         # the MFMA attention kernels (and with them the balanced verify split and the shared
@@ -181,6 +207,10 @@ class ModelRunner:
         B = len(seq_meta)
         width = max(max((len(m.block_ids) for m in seq_meta), default=1), 1)
         trees = any(m.is_tree() for m in seq_meta)
+        quant = isinstance(cache, QuantPagedKVCache)
+        if trees and (quant or any(0 < w < width * cache.block_size for w, _ in self.windows)):
+            raise ValueError("drafted trees attend a cache in the model's type over the whole context: "
+                             "not a quantised one, and no sliding window")
         T = sum(m.q_len for m in seq_meta)
         end = 2 * B + 1 + B * width
         host = torch.zeros(end + (T if trees else 0), dtype=torch.int32)
@@ -207,11 +237,11 @@ class ModelRunner:
                     range(-1, m.q_len - 1) if m.parents is None else m.parents, dtype=torch.int32)
         dev = host.to(cache.key.device)                 # one H2D copy for all metadata
         decode = all(m.q_len == 1 for m in seq_meta)
-        shared = 0 if trees else self._shared_prefix(
+        shared = 0 if trees or quant else self._shared_prefix(
             seq_meta, host[2 * B + 1:end].view(B, width), cache.block_size)
         max_q_len = max(m.q_len for m in seq_meta)
         max_ctx = width * cache.block_size
-        balanced = (not decode and not shared and not trees and
+        balanced = (not decode and not shared and not trees and not quant and
                     self._prefer_balanced(seq_meta, max_q_len, max_ctx, cache.block_size))
         mask = (tree_mask(dev[end:], dev[B:2 * B + 1], max_q_len)
                 if trees and self.attn_backend == "hip" else None)
@@ -271,11 +301,28 @@ class ModelRunner:
         attn = layer.self_attn
         q, k, v = self._project_qkv(attn, x, layer_idx)
         # q_norm / k_norm (Qwen3), RoPE on q and k, and cache.write(k, v): one launch
-        q = qk_norm_rope_append(q, k, v, cos, sin, write_slots, cache, layer_idx,
-                                attn.q_norm if self.qk_norm else None,
-                                attn.k_norm if self.qk_norm else None)
+        norms = (attn.q_norm, attn.k_norm) if self.qk_norm else (None, None)
+        quant = isinstance(cache, QuantPagedKVCache)
+        if quant:
+            if batch.rows is None:
+                batch.rows = ScratchRows(k)
+            q, k = qk_norm_rope(q, k, v, cos, sin, *norms, rows=batch.rows)
+            cache.write(layer_idx, write_slots, k, v)
+        else:
+            q = qk_norm_rope_append(q, k, v, cos, sin, write_slots, cache, layer_idx, *norms)
+        window, sinks = self.windows[layer_idx]
+        if window >= batch.max_ctx:
+            window = sinks = 0
         if self.attn_backend == "native":
-            o = self._torch_attention(q, cache, layer_idx, batch.seqs)
+            o = self._torch_attention(q, cache, layer_idx, batch.seqs, window, sinks)
+        elif quant or window:
+            pools = (cache.layer(layer_idx) if quant
+                     else (cache.key[layer_idx], cache.value[layer_idx]))
+            attend = paged_quant_attention if quant else paged_window_attention
+            o = attend(q, *pools, batch.block_table, None if batch.decode else batch.cu_q,
+                       batch.ctx_lens, self.kv_groups, window=window, sinks=sinks,
+                       block_size=cache.block_size, scale=self.scale, max_q_len=batch.max_q_len,
+                       max_ctx=batch.max_ctx)
         elif batch.tree_mask is not None:
             o = paged_tree_attention(
                 q, cache.key[layer_idx], cache.value[layer_idx], batch.block_table, batch.cu_q,
@@ -296,7 +343,7 @@ class ModelRunner:
         return attn.o_proj(o.flatten(1))
 
     def _torch_attention(self, q: torch.Tensor, cache: PagedKVCache, layer_idx: int,
-                         seqs) -> torch.Tensor:
+                         seqs, window: int = 0, sinks: int = 0) -> torch.Tensor:
         """attn_backend="native": the reference's per-sequence attention
         (model_runner.py:160-185) -- the sequence's context rows gathered from the pool
         (the prologue has already appended this step's k and v, so a fresh prefill reads
@@ -312,6 +359,10 @@ class ModelRunner:
             keys, vals = cache.gather(layer_idx, cache.context_slots(m.block_ids, m.ctx_len))
             as_bhd = lambda t: t.float().transpose(0, 1).unsqueeze(0)  # noqa: E731
             seen = causal_lower_right(m.q_len, m.ctx_len)
+            if window:
+                key = torch.arange(m.ctx_len, device=q.device)
+                pos = key[m.ctx_len - m.q_len:, None]
+                seen = (key <= pos) & ((key > pos - window) | (key < sinks))
             if m.is_tree():
                 seen = torch.zeros(m.q_len, m.ctx_len, dtype=torch.bool)
                 seen[:, :m.ctx_len - m.q_len] = True
@@ -345,7 +396,8 @@ class ModelRunner:
         multi-query kernel, which reads those blocks once for the batch."""
         cos, sin = self.rope(positions)
         x = self.embed(token_ids)
-        if batch.workspace is None and self.attn_backend == "hip":
+        if (batch.workspace is None and self.attn_backend == "hip"
+                and not isinstance(cache, QuantPagedKVCache)):
             B = batch.ctx_lens.shape[0]
             if batch.tree_mask is not None:
                 batch.workspace = tree_workspace(B, self.num_heads, self.num_kv_heads,

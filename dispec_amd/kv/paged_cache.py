@@ -322,6 +322,15 @@ class PagedKVCache:
         shape = (self.num_layers, seq_len, self.num_kv_heads, self.head_dim)
         return kbuf.view(shape), vbuf.view(shape)
 
+    def export_into(self, block_ids: list[int], seq_len: int, k: torch.Tensor,
+                    v: torch.Tensor) -> None:
+        """`export_contiguous` into given contiguous (num_layers, seq_len, H, D) tensors."""
+        self._check_blocks(block_ids, seq_len)
+        table = self.block_table([block_ids])
+        cu = torch.tensor([0, seq_len], dtype=torch.long).to(self.key.device)
+        flat = (self.num_layers * seq_len, self.num_kv_heads, self.head_dim)
+        self.gather_into(table, cu, seq_len, k.view(flat), v.view(flat))
+
     def import_batch(self, tables: list[list[int]], k: torch.Tensor, v: torch.Tensor,
                      cu: list[int]) -> None:
         """Scatter flat buffers laid out as export_batch's into the given block tables."""

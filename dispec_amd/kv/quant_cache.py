@@ -105,20 +105,29 @@ def quant_append(k_cache, k_scale, v_cache, v_scale, slots, k, v, err=None) -> N
         _lib.check(status, "dsp_kv_append_quant")
 
 
-def quant_gather(k_cache, k_scale, v_cache, v_scale, slots, dtype=torch.bfloat16, err=None):
+def quant_gather(k_cache, k_scale, v_cache, v_scale, slots, dtype=torch.bfloat16, err=None, out=None):
     """The values (k, v) that slots of a quantised pool hold (dsp_kv_gather_quant): each (T, KVH,
     head_dim), or (L, T, KVH, head_dim) of pools of all layers, rounded to `dtype` (which loses
     nothing in bf16 and fp32, and in fp16 where the rows were written from fp16).  Arguments as for
-    `quant_append`; a slot outside the pool leaves its rows undefined."""
+    `quant_append`; a slot outside the pool leaves its rows as they were (undefined without `out`).
+    out: optional pair of contiguous tensors of that shape and type to write."""
     fmt, L, S, KVH, D, strides = _pools(k_cache, k_scale, v_cache, v_scale)
     if dtype not in _DTYPES:
         raise ValueError(f"values in bf16, fp16 or fp32, not {dtype}")
     if slots.dtype != torch.int64:
         raise ValueError(f"slots must be int64, got {slots.dtype}")
-    dev = _lib.same_gpu(k_cache, k_scale, v_cache, v_scale, slots, err)
     T = slots.numel()
-    k = k_cache.new_empty((T, KVH, D) if k_cache.dim() == 3 else (L, T, KVH, D), dtype=dtype)
-    v = torch.empty_like(k)
+    rows = (T, KVH, D) if k_cache.dim() == 3 else (L, T, KVH, D)
+    if out is None:
+        k = k_cache.new_empty(rows, dtype=dtype)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
+        for t in out:
+            if t.shape != rows or t.dtype != dtype or not t.is_contiguous():
+                raise ValueError(f"out must be two contiguous tensors {rows} of {dtype}; got "
+                                 f"{tuple(t.shape)} {t.dtype}")
+    dev = _lib.same_gpu(k_cache, k_scale, v_cache, v_scale, slots, k, v, err)
     if not (T and L):
         return k, v
     if not slots.is_contiguous():
@@ -222,10 +231,15 @@ class QuantPagedKVCache(PagedKVCache):
                 else torch.empty(shape, dtype=self.dtype, device=self.key.device) for i in (0, 1)]
         return flat[0], flat[1], cu
 
-    def _read(self, block_ids, n):
-        kv = quant_gather(*self._all(), self._slots_of([block_ids], [n]), self.dtype, err=self._err)
+    def _read(self, block_ids, n, out=None):
+        kv = quant_gather(*self._all(), self._slots_of([block_ids], [n]), self.dtype, err=self._err,
+                          out=out)
         self._after()
         return kv
+
+    def export_into(self, block_ids, seq_len, k, v) -> None:
+        self._check_blocks(block_ids, seq_len)
+        self._read(block_ids, seq_len, (k, v))
 
     def import_batch(self, tables, k, v, cu) -> None:
         """Quantise flat buffers laid out as export_batch's into the given block tables."""

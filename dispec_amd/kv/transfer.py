@@ -465,6 +465,10 @@ class CrossModelKVMap:
                              f"{cache.head_dim}")
         if cache.dtype != torch.bfloat16:
             raise ValueError("map_into fills bf16 caches")
+        if cache.key.dtype != cache.dtype:   # a quantised cache: the rows are quantised as they come
+            keys, values = self.map(k, v, source_rope, target_rope, use_residual)
+            cache.import_contiguous(block_ids, keys, values)
+            return
         cache._check_blocks(block_ids, T)
         table = cache._upload_tables([block_ids], [])[0]
         kv = H * D

@@ -196,14 +196,10 @@ class HipIpcTransport(Transport):
         launch over all layers) and return it as a payload ready for `send`."""
         L, T = cache.num_layers, len(tokens)
         shape = (L, T, cache.num_kv_heads, cache.head_dim)
-        nbytes = L * T * cache.row_bytes
+        nbytes = L * T * cache.num_kv_heads * cache.head_dim * cache.dtype.itemsize
         kmem, vmem = alloc_region(nbytes), alloc_region(nbytes)
         k, v = kmem.tensor(cache.dtype, shape), vmem.tensor(cache.dtype, shape)
-        cache._check_blocks(block_ids, T)
-        table = cache.block_table([block_ids])
-        cu = torch.tensor([0, T], dtype=torch.long).to(cache.key.device)
-        flat = (L * T, cache.num_kv_heads, cache.head_dim)
-        cache.gather_into(table, cu, T, k.view(flat), v.view(flat))
+        cache.export_into(block_ids, T, k, v)
         cache.check_errors()
         self._exported[k.data_ptr()] = kmem
         self._exported[v.data_ptr()] = vmem
