@@ -193,6 +193,42 @@ def calls() -> _Calls:
     return _CALLS
 
 
+_TORCH_CALLS = None
+
+
+def torch_calls():
+    """dispec_amd._torchcall (csrc/torchcall.cpp), bound to the library: calls that take tensors and
+    return None where they leave the call to their Python wrapper.  None where it is not built."""
+    global _TORCH_CALLS
+    if _TORCH_CALLS is None:
+        try:
+            from dispec_amd import _torchcall
+        except ImportError:
+            _TORCH_CALLS = False
+            return None
+        handle = lib()
+        _torchcall.bind(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in (
+            "dsp_paged_window_attention", "dsp_paged_window_workspace_bytes", "dsp_kv_append_quant",
+            "dsp_kv_gather_quant")))
+        _TORCH_CALLS = _torchcall
+    return _TORCH_CALLS or None
+
+
+def current_stream(t) -> int | None:
+    """hipStream_t of torch's current stream where t is on the current device; None elsewhere."""
+    global _current_device, _raw_stream
+    if _current_device is None or _raw_stream is None:
+        import torch
+        _current_device = torch.cuda.current_device
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda i: torch.cuda.current_stream(i).cuda_stream)
+    index = t.get_device()
+    return _raw_stream(index) if index >= 0 and index == _current_device() else None
+
+
+_raw_stream = None
+
+
 def error_string(status: int) -> str:
     return lib().dsp_error_string(status).decode()
 

@@ -2,7 +2,8 @@
 
 Every source is compiled to an object in dispec_amd/_build/ (in parallel), then linked
 into dispec_amd/libdispec_hip.so in-tree, where the loader looks for it, and the fast
-binding csrc/fastcall.c into the dispec_amd._fastcall module.  Run as
+bindings csrc/fastcall.c and csrc/torchcall.cpp into the dispec_amd._fastcall and _torchcall
+modules.  Run as
 `python -m dispec_amd.build`.
 """
 
@@ -78,16 +79,44 @@ def _build_fastcall(verbose: bool) -> Path:
     return out
 
 
+def _build_torchcall(verbose: bool) -> Path:
+    """csrc/torchcall.cpp -> the CPython module dispec_amd._torchcall (g++ against torch's headers;
+    host code only)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    out = PKG / ("_torchcall" + sysconfig.get_config_var("EXT_SUFFIX"))
+    tmp = out.with_name(out.name + ".tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    for path in [sysconfig.get_paths()["include"], *include_paths()]:
+        cmd += ["-isystem", path]
+    for path in library_paths():
+        cmd += ["-L", path]
+    cmd += [str(CSRC / "torchcall.cpp"), "-o", str(tmp), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on torchcall.cpp:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, out)
+    return out
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile every csrc/*.hip into libdispec_hip.so (the product library) and
-    csrc/fastcall.c into the dispec_amd._fastcall module.  Returns the library path."""
+    """Compile every csrc/*.hip into libdispec_hip.so (the product library), csrc/fastcall.c into the
+    dispec_amd._fastcall module and csrc/torchcall.cpp into dispec_amd._torchcall.  Returns the
+    library path."""
     sources = sorted(CSRC.glob("*.hip"))
     if not sources:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     OBJ_DIR.mkdir(exist_ok=True)
     jobs = jobs or min(len(sources), max(1, (os.cpu_count() or 2)))
     with ThreadPoolExecutor(max_workers=jobs) as pool:
+        bound = pool.submit(_build_torchcall, verbose)
         objs = list(pool.map(lambda s: _compile(s, verbose), sources))
+        bound.result()
     _build_fastcall(verbose)
     return _link(objs, LIB, verbose)
 

@@ -382,7 +382,6 @@ def window_workspace(batch, num_heads, num_kv_heads, head_dim, max_q_len, max_ct
 
 def _windowed(q, k_cache, v_cache, k_scale, v_scale, fmt, block_table, cu_q, ctx_lens, kv_groups,
               window, sinks, block_size, scale, max_q_len, max_ctx, out, err, workspace):
-    # (a decode step calls this once per layer: each attribute of a tensor is read once)
     q_shape, k_shape, k_stride, v_stride = q.shape, k_cache.shape, k_cache.stride(), v_cache.stride()
     if len(q_shape) != 3 or len(k_shape) != 3 or v_cache.shape != k_shape:
         raise ValueError(f"expected q (T, Hq, D) and caches (S, KVH, width); got {tuple(q.shape)}, "
@@ -481,6 +480,13 @@ def paged_window_attention(q, k_cache, v_cache, block_table, cu_q, ctx_lens, kv_
     err:         optional int32 device counter of bad lengths and block ids
     returns:     (sum q_len, num_heads, head_dim) in q's dtype
     """
+    fast, stream = _lib.torch_calls(), _lib.current_stream(q)
+    if fast is not None and stream is not None:
+        got = fast.window(q, k_cache, None, v_cache, None, block_table, cu_q, ctx_lens, kv_groups,
+                          window, sinks, block_size, scale, max_q_len, max_ctx, out, err, workspace,
+                          stream)
+        if got is not None:
+            return got
     if not q.dtype == k_cache.dtype == v_cache.dtype or q.dtype not in _DTYPES:
         raise ValueError(f"q/k/v dtypes {q.dtype}/{k_cache.dtype}/{v_cache.dtype}: "
                          "the HIP kernels take bf16, fp16 or fp32, all the same")
@@ -497,6 +503,13 @@ def paged_quant_attention(q, k_cache, k_scale, v_cache, v_scale, block_table, cu
     v_scale (S, KVH, head_dim / 32) uint8.  q in bf16, fp16 or fp32, head_dim 64, 128 or 256; the
     cache's numbers count as `quant_gather` gives them in q's dtype; scale > 0.
     """
+    fast, stream = _lib.torch_calls(), _lib.current_stream(q)
+    if fast is not None and stream is not None:
+        got = fast.window(q, k_cache, k_scale, v_cache, v_scale, block_table, cu_q, ctx_lens, kv_groups,
+                          window, sinks, block_size, scale, max_q_len, max_ctx, out, err, workspace,
+                          stream)
+        if got is not None:
+            return got
     if (q.dtype not in _DTYPES
             or not k_cache.dtype == v_cache.dtype == k_scale.dtype == v_scale.dtype == torch.uint8):
         raise ValueError(f"q {q.dtype}, codes {k_cache.dtype}/{v_cache.dtype}, scales {k_scale.dtype}/"

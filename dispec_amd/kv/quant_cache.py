@@ -72,6 +72,10 @@ def quant_append(k_cache, k_scale, v_cache, v_scale, slots, k, v, err=None) -> N
     are first clamped to +-61440 ("fp8") or +-49152 ("fp4"), so that they read back finite.  A group
     with an infinity or NaN reads back as NaN.
     """
+    fast, stream = _lib.torch_calls(), _lib.current_stream(k_cache)
+    if fast is not None and stream is not None and fast.append(
+            k_cache, k_scale, v_cache, v_scale, slots, k, v, err, stream):
+        return
     fmt, L, S, KVH, D, strides = _pools(k_cache, k_scale, v_cache, v_scale)
     T, rows = slots.numel(), k.shape
     n = len(rows)
@@ -111,6 +115,11 @@ def quant_gather(k_cache, k_scale, v_cache, v_scale, slots, dtype=torch.bfloat16
     nothing in bf16 and fp32, and in fp16 where the rows were written from fp16).  Arguments as for
     `quant_append`; a slot outside the pool leaves its rows as they were (undefined without `out`).
     out: optional pair of contiguous tensors of that shape and type to write."""
+    fast, stream = _lib.torch_calls(), _lib.current_stream(k_cache)
+    if fast is not None and stream is not None and out is None:
+        got = fast.gather(k_cache, k_scale, v_cache, v_scale, slots, dtype, err, stream)
+        if got is not None:
+            return got
     fmt, L, S, KVH, D, strides = _pools(k_cache, k_scale, v_cache, v_scale)
     if dtype not in _DTYPES:
         raise ValueError(f"values in bf16, fp16 or fp32, not {dtype}")
