@@ -198,6 +198,10 @@ int stream_plain(int32_t D, int32_t dtype, const WinPlan& p, const WinArgs& a, h
 int stream_fp8(int32_t D, int32_t dtype, const WinPlan& p, const WinArgs& a, hipStream_t s);
 int stream_fp4(int32_t D, int32_t dtype, const WinPlan& p, const WinArgs& a, hipStream_t s);
 
+// Tiles of 256 rows (window_prefill.hip): q in 16 bits, D 64 or 128.
+int wide_tiles(int D, int fmt, bool f16, unsigned grid, const WinArgs& a, hipStream_t s);
+
+constexpr int kChunk = 64;  // keys per chunk of the tile kernels
 // Chunks of the stream kernel, in keys, and waves of its workgroups: one workgroup fills a CU.
 constexpr int kStreamChunk = 32;
 constexpr int stream_block(int D) { return D > 128 ? 4 : 8; }

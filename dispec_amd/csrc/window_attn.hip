@@ -15,32 +15,14 @@ using namespace dsp_window;
 
 namespace {
 
-constexpr int kChunk = 64;           // keys per chunk
-template <int kNW, int kBufs, int kOcc>
-struct Shape {
-  static constexpr int NW = kNW, TR = 32 * kNW, NB = kBufs, OCC = kOcc;
-};
-
-// Waits until at most n stages' loads (kLoads each) of this wave are out, n <= kMost.
-template <int kMost, int kLoads>
-__device__ __forceinline__ void wait_stages(int n) {
-  if constexpr (kMost > 0) {
-    if (n >= kMost) {
-      __builtin_amdgcn_s_waitcnt(dsp_waitcnt_vm<kMost * kLoads>());
-      return;
-    }
-    wait_stages<kMost - 1, kLoads>(n);
-  } else {
-    __builtin_amdgcn_s_waitcnt(dsp_waitcnt_vm<0>());
-  }
-}
+constexpr int NW = 4, TR = 32 * NW;  // waves and rows of a tile
+constexpr int NB = 2;                // chunks in LDS
 
 // kF32: q and out in fp32 over a quantised cache.  An element times its scale is exact in bf16, and
 // q and the probabilities enter the products as three bf16 operands each, all 24 bits.
-template <typename Tag, int D, int kFmt, bool kF32, typename S>
-__global__ __launch_bounds__(64 * S::NW) __attribute__((amdgpu_waves_per_eu(S::OCC))) void
-window_tile_kernel(const WinArgs a) {
-  constexpr int NW = S::NW, TR = S::TR, NB = S::NB;
+template <typename Tag, int D, int kFmt, bool kF32>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(kF32 || D == 256 ? 1 : 2)))
+void window_tile_kernel(const WinArgs a) {
   constexpr int NKS = D / 16, NDT = D / 32;   // 16-dim steps of K Q^T, 32-dim tiles of V^T P^T
   constexpr int CPR = D / 8, ROWB = 2 * D;    // 16-byte pieces and bytes of a row in LDS
   constexpr int SLAB = kChunk * ROWB;
@@ -298,7 +280,7 @@ window_tile_kernel(const WinArgs a) {
     const int buf = c % NB, t = key_of(c);
     if constexpr (kFmt == kNone) {
       __builtin_amdgcn_sched_barrier(0);
-      wait_stages<NB - 2, 2 * LPW>(min(nc - 1 - c, NB - 2));
+      __builtin_amdgcn_s_waitcnt(dsp_waitcnt_vm<0>());
     }
     const bool tile_edge = !sees_all(t, tile_pf, tile_pl);
     char* const my_v = &lds[buf][1][wave * LPW * 1024];  // the V rows this wave loaded
@@ -518,6 +500,8 @@ WinPlan win_plan(int32_t B, int32_t KVH, int32_t G, int32_t D, int32_t max_q_len
   if (!(D == 64 || D == 128 || D == 256) || (dtype == DSP_F32 && !quantised(format))) return p;
   const int64_t rows = int64_t(max_q_len) * G;
   p.stream = may_stream && rows <= 64;
+  // Tiles of 256 rows where a sequence has more than half of one and its registers suffice
+  // (window_prefill.hip); of 128 they pass K and V through LDS twice as often.
   p.rows = p.stream ? (rows <= 16 || D > 128 || dtype == DSP_F32 ? 16 : 32)
                     : D > 128 || rows <= 128 || dtype == DSP_F32 ? 128 : 256;
   const int size = p.stream ? kStreamChunk : kChunk;
@@ -556,7 +540,7 @@ WinPlan win_plan(int32_t B, int32_t KVH, int32_t G, int32_t D, int32_t max_q_len
     // 128 MiB of K and V, half of the last-level cache, behind which the next call finds little of its
     // own: 1.1 GB of fp8 195 us (204 by ordinary loads), 134 MB 29.6 (30.5); 102 MB 35 (30).
     const int64_t row = format == DSP_KV_FP8 ? D : format == DSP_KV_FP4 ? D / 2 : 2 * D;
-    p.once = all * chunks * size * 2 * row >= (int64_t(128) << 20);
+    p.once = double(all) * double(chunks * size * 2 * row) >= double(128 << 20);
     workgroups = whole ? total + 8 * tiles : p.runs;
     p.tile = units < (int64_t(1) << 31) && rows < (int64_t(1) << 30);
   } else {
@@ -571,6 +555,8 @@ WinPlan win_plan(int32_t B, int32_t KVH, int32_t G, int32_t D, int32_t max_q_len
   }
   p.tiles = int(tiles);
   p.tile = p.tile && workgroups < (int64_t(1) << 31);  // (32 bits number the workgroups)
+  if (p.stream && !p.tile)
+    return win_plan(B, KVH, G, D, max_q_len, max_ctx, window, sinks, format, dtype, false);
   return p;
 }
 
@@ -585,17 +571,13 @@ template <typename Tag, int D, int kFmt, bool kF32>
 int launch_window(const WinPlan& p, const WinArgs& a, hipStream_t s) {
   const int64_t pairs = int64_t(a.B) * a.KVH, per = int64_t(p.tiles) * p.parts;
   const unsigned grid = unsigned(pairs >= 8 ? (pairs + 7) / 8 * 8 * per : (pairs * per + 7) / 8 * 8);
-  auto launch = [&](auto shape) {
-    using S = decltype(shape);
-    window_tile_kernel<Tag, D, kFmt, kF32, S><<<grid, 64 * S::NW, 0, s>>>(a);
-  };
-  if constexpr (kF32 || D == 256) {
-    launch(Shape<4, 2, 1>{});
+  int st;
+  if (p.rows == 256) {
+    st = wide_tiles(D, kFmt, std::is_same<Tag, F16Tag>::value, grid, a, s);
   } else {
-    if (p.rows == 256) launch(Shape<8, kFmt == kNone ? 4 : 2, 2>{});
-    else launch(Shape<4, 2, 2>{});
+    window_tile_kernel<Tag, D, kFmt, kF32><<<grid, 64 * NW, 0, s>>>(a);
+    st = dsp_launch_status();
   }
-  const int st = dsp_launch_status();
   if (st != DSP_OK || p.parts <= 1) return st;
   const int64_t most = std::min<int64_t>(int64_t(a.max_q_len) * a.G, p.rows);
   const int groups = int((most + merge_rows<D>() - 1) / merge_rows<D>());
@@ -729,7 +711,8 @@ extern "C" int dsp_paged_window_attention(
                   scale_stride_slot, scale_stride_head, block_table, bt_stride,
                   dsp_log2i(block_size), cu_q, ctx_lens, B, KVH, G, max_q_len, max_ctx, win, sink,
                   scale * 1.4426950408889634f, p.tiles, p.parts, p.part_chunks, p.heads, p.runs,
-                  p.least, p.start, (65536 + G - 1) / G, reinterpret_cast<int32_t*>(ws_ml + 2 * part_rows), ws, ws_ml, out, o_stride_t, o_stride_h,
+                  p.least, p.start, (65536 + G - 1) / G,
+                  reinterpret_cast<int32_t*>(ws_ml + 2 * part_rows), ws, ws_ml, out, o_stride_t, o_stride_h,
                   o_stride_t % 4 == 0 && o_stride_h % 4 == 0 && dsp_aligned(out, 8), err_count};
   if (p.stream)
     return format == DSP_KV_FP8   ? stream_fp8(D, dtype, p, a, s)
