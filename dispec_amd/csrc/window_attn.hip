@@ -617,9 +617,10 @@ extern "C" size_t dsp_paged_window_workspace_bytes(int32_t B, int32_t Hq, int32_
                                                    int32_t max_q_len, int32_t max_ctx,
                                                    int32_t window, int32_t sinks, int32_t format,
                                                    int32_t dtype) {
-  if (B <= 0 || KVH <= 0 || Hq <= 0 || Hq % KVH != 0 || max_q_len <= 0 || max_ctx <= 0 ||
+  if (B <= 0 || KVH <= 0 || Hq <= 0 || Hq % KVH != 0 || max_q_len <= 0 || max_ctx < 0 ||
       window < 0 || sinks < 0)
     return 0;
+  max_ctx = std::max(max_ctx, 1);  // (as the launch is planned)
   size_t tile = 0;
   for (bool stream : {false, true})
     tile = std::max(tile, win_bytes(win_plan(B, KVH, Hq / KVH, D, max_q_len, max_ctx, window, sinks,
@@ -657,6 +658,7 @@ extern "C" int dsp_paged_window_attention(
   const int64_t es = dtype == DSP_F32 ? 4 : 2;
   DSP_HOST_CHECK(dsp_aligned(q, es) && dsp_aligned(out, es), DSP_EALIGN);
   const int G = Hq / KVH;
+  const int32_t plan_ctx = std::max(max_ctx, 1);  // (no context at all: as for one token)
   // (a window that reaches past every context is none)
   const bool all = window == 0 || window >= max_ctx;
   const int32_t win = all ? kWholeWindow : window, sink = all ? 0 : std::min(sinks, max_ctx);
@@ -667,7 +669,7 @@ extern "C" int dsp_paged_window_attention(
                  dsp_aligned(k_scale, scale_bytes) && dsp_aligned(v_scale, scale_bytes));
   const bool rows16 = kv_stride_slot_bytes % 16 == 0 && kv_stride_head_bytes % 16 == 0 &&
                       dsp_aligned(k_cache, 16) && dsp_aligned(v_cache, 16);
-  const WinPlan p = win_plan(B, KVH, G, D, max_q_len, max_ctx, window, sinks, format, dtype,
+  const WinPlan p = win_plan(B, KVH, G, D, max_q_len, plan_ctx, window, sinks, format, dtype,
                              rows16 && scales_ok);
   const int32_t row_align = quant ? (format == DSP_KV_FP8 ? 16 : 8) : 16;
   const int64_t q_align = dtype == DSP_F32 ? 1 : 8;
@@ -686,16 +688,16 @@ extern "C" int dsp_paged_window_attention(
     DSP_HOST_CHECK(dsp_aligned(k_cache, es) && dsp_aligned(v_cache, es) &&
                        kv_stride_slot_bytes % es == 0 && kv_stride_head_bytes % es == 0,
                    DSP_EALIGN);
-    const int32_t P = general_partition(B, Hq, KVH, D, max_q_len, max_ctx, window, sinks);
+    const int32_t P = general_partition(B, Hq, KVH, D, max_q_len, plan_ctx, window, sinks);
     const size_t need = dsp_detail::generic_workspace_bytes(
-        B, Hq, D, max_q_len, general_span(max_q_len, max_ctx, window, sinks), P);
+        B, Hq, D, max_q_len, general_span(max_q_len, plan_ctx, window, sinks), P);
     DSP_HOST_CHECK(workspace_bytes >= need && (need == 0 || workspace != nullptr), DSP_EWORKSPACE);
     DSP_HOST_CHECK(need == 0 || dsp_aligned(workspace, 16), DSP_EALIGN);
     return dsp_detail::generic_window_attention(
         q, q_stride_t, q_stride_h, k_cache, v_cache, num_slots, kv_stride_slot_bytes / es,
         kv_stride_head_bytes / es, block_table, bt_stride, dsp_log2i(block_size), cu_q, ctx_lens, B,
         Hq, KVH, D, scale, win, sink, max_q_len, max_ctx,
-        general_span(max_q_len, max_ctx, window, sinks), P, workspace, out, o_stride_t, o_stride_h,
+        general_span(max_q_len, plan_ctx, window, sinks), P, workspace, out, o_stride_t, o_stride_h,
         dtype, err_count, s);
   }
   const size_t need = win_bytes(p, int64_t(B) * KVH, D);
