@@ -30,6 +30,9 @@ void window_tile_kernel(const WinArgs a) {
   constexpr int LPW = SLAB / 1024 / NW;       // KiB a wave loads of a slab
   constexpr int RPI = 1024 / ROWB;            // rows per LDS DMA
   constexpr int kTerms = kF32 ? 3 : 1;
+  // fp32 of 256 dims: q alone is 192 registers, and operands that the compiler reads ahead push more of
+  // them into memory (24 x 32 rows of 4 KV heads over 4000 fp8 tokens: 398 us, 792 with them)
+  constexpr bool kCrowded = kF32 && D == 256;
   static_assert(RPW <= 16 && LPW >= 1 && LPW * RPI == RPW, "a wave's rows lie in one block");
   static_assert(!kF32 || (kFmt != kNone && std::is_same<Tag, Bf16Tag>::value), "exact in bf16");
   __shared__ __attribute__((aligned(1024))) char lds[NB][2][SLAB];
@@ -338,16 +341,18 @@ void window_tile_kernel(const WinArgs a) {
     // ---- scores S^T (keys x rows): sc[x][j] is key t + 32 x + 8 (j / 4) + 4 hl + j % 4 of row col
     f32x16 sc[2];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int j = 0; j < 16; ++j) sc[x][j] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) {
+    for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if constexpr (kCrowded) __builtin_amdgcn_sched_barrier(0);
         const dsp_u32x4 k = read_k(buf, x, ks);
 #pragma unroll
         for (int i = kTerms - 1; i >= 0; --i) sc[x] = mfma32x32<Tag>(k, qop[i][ks], sc[x]);
       }
-    }
     const bool edge = !sees_all(t, pf, pl);
     if (edge) {
 #pragma unroll
@@ -413,6 +418,7 @@ void window_tile_kernel(const WinArgs a) {
       }
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) {
+        if constexpr (kCrowded) __builtin_amdgcn_sched_barrier(0);
         const dsp_u32x4 v = read_v(buf, ps, dt);
 #pragma unroll
         for (int i = kTerms - 1; i >= 0; --i) acc[dt] = mfma32x32<Tag>(v, pop[i], acc[dt]);
