@@ -8,7 +8,9 @@
 // that the format has below fp16's end (61440, 49152): what is read back is finite in fp16.
 //
 // A thread takes units of 8 elements; a group's maximum is that of four neighbouring lanes (two quad
-// permutes).  Bound by memory: each row is read once and written once.
+// permutes).  Bound by memory: each row is read once and written once.  2050 tokens of 36 layers in and
+// out, 760 MB, 149 us (88 and 69 of kernels); 4096 out, 915 MB, 169; both at the rate of a large copy,
+// 5.2 TB/s.  32 rows of one layer: 3 us a kernel, 5 with the call.
 #include <algorithm>
 
 #include "dsp_common.h"

@@ -239,7 +239,8 @@ window_wide_kernel(const WinArgs a) {
   };
 
   // chunks seen0 .. seen1 - 1 of the piece: those of the window that all rows of the tile see whole
-  const int seen0 = max(span.sink, (max(tile_pl - a.window, -1) + kChunk) / kChunk - span.first + span.sink) - c0;
+  const int seen0 =
+      max(span.sink, (max(tile_pl - a.window, -1) + kChunk) / kChunk - span.first + span.sink) - c0;
   const int seen1 = (tile_pf + 1) / kChunk - span.first + span.sink - c0;
   // whether rows at positions f .. l, of the tile's, see all keys of chunk c
   auto sees_all = [&](int c, int f, int l) {
