@@ -1,4 +1,5 @@
-// What the kernels of dsp_paged_window_attention share (window_attn.hip, window_stream.h).
+// What the kernels of dsp_paged_window_attention share (window_attn.hip, window_prefill.hip,
+// window_stream.h).
 #pragma once
 
 #include <float.h>
