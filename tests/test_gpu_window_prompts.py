@@ -93,3 +93,47 @@ def test_infinities(hip, D, dtype, window, sinks, holes):
         want = keep.clone()
         want[torch.from_numpy(c.see[0][:, key]).nonzero()[:, 0].to(DEV), 2:4, d] = x
         assert torch.equal(torch.nan_to_num(got, 1e4, 2e4, 3e4), torch.nan_to_num(want, 1e4, 2e4, 3e4)), key
+
+
+@pytest.mark.parametrize("fmt", [None, "fp8"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (260, 20)])
+def test_graph_of_two_calls_beside_eager_ones(hip, fmt, window, sinks):
+    """Two captured calls of one graph, replayed on other lengths while eager calls run on a second
+    stream; their workspaces are their own."""
+    c = Case([150, 3], [1700, 900], 4, 2, 128, BF16, window, sinks, seed=8, fmt=fmt, hole=0)
+    ctx = c.lens.clone()
+    c.call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        one, two = c.call(), c.call(scale=0.25)
+    side = torch.cuda.Stream()
+    for step in range(4):
+        c.lens.copy_(ctx - 40 * step)
+        want = c.call(), c.call(scale=0.25)
+        one.fill_(3.0)
+        side.wait_stream(torch.cuda.current_stream())
+        g.replay()
+        with torch.cuda.stream(side):
+            beside = [c.call() for _ in range(3)]
+        torch.cuda.current_stream().wait_stream(side)
+        for got in (one, *beside):
+            assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want[0])), step
+        assert torch.equal(torch.nan_to_num(two), torch.nan_to_num(want[1])), step
+
+
+@pytest.mark.parametrize("fmt", [None, "fp4"])
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, F16)])
+def test_strides_and_rows_behind(hip, D, dtype, fmt):
+    """q and out as parts of wider rows, heads between others; rows of no sequence stay."""
+    c = Case([150, 0, 140], [400, 5, 333], 6, 2, D, dtype, 100, 7, seed=9, fmt=fmt)
+    want = c.call()
+    c.check(want, *_reference(c))
+    q = torch.full((295, 8, 2 * D), float("nan"), dtype=dtype, device=DEV)
+    q[:290, 1:7, D:] = c.dq
+    out = torch.full((295, 7, D + 8), 5.0, dtype=dtype, device=DEV)
+    got = c.call(q=q[:, 1:7, D:], out=out[:, 1:, :D])
+    assert got.data_ptr() == out[:, 1:].data_ptr()
+    assert torch.equal(got[:290], want)
+    out[:290, 1:, :D] = 5.0
+    assert (out == 5).all()
