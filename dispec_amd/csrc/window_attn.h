@@ -19,6 +19,19 @@ using dsp_quant::kFp4;
 using dsp_quant::kFp8;
 using dsp_quant::kNone;
 
+// The 16-bit operands that hold a probability where q has 16 bits.
+template <int D>
+constexpr int prob_terms() {
+  return D > 128 ? 3 : 1;
+}
+// By how much, in powers of two, a score may exceed the running maximum before it moves.  (fp16 in three
+// operands: by little, so that a row's largest probability is 2^13 or more, and fp16's end, 2^-24, below
+// 2^-37 of it: less than half of fp32's last bit for 4096 keys in a row)
+template <typename Tag, int kTerms>
+constexpr float lag() {
+  return std::is_same<Tag, F16Tag>::value && kTerms == 3 ? 2.f : 8.f;
+}
+
 constexpr int kWholeWindow = 1 << 30;  // a window that no context reaches the end of
 
 struct WinArgs {

@@ -11,7 +11,7 @@
 // the window; of a block none of whose keys is seen neither id nor rows are read.  Two workgroups a CU at
 // 64 and 128 dims: a chunk is loaded while the one before it is used, and one workgroup multiplies while
 // another is at its barrier.  24 x 32 queries of 16 heads over 4 KV heads, 4000 tokens: under a window of
-// 2048 29 us (64 dims), 41 (128), 80 (256); the whole context in fp8 42, 56, 147: bound by the chain of
+// 2048 29 us (64 dims), 39 (128), 101 (256); the whole context in fp8 42, 55, 180: bound by the chain of
 // chunks that a workgroup has (a load, a barrier, products and exponentials one after the other).
 #include "window_attn.h"
 
@@ -24,6 +24,9 @@ constexpr int NB = 2;                // chunks in LDS
 
 // kF32: q and out in fp32 over a quantised cache.  An element times its scale is exact in bf16, and
 // q and the probabilities enter the products as three bf16 operands each, all 24 bits.
+// 16-bit q: a probability is three operands (pack8), all 24 bits, where heads have 256 dims, as in all
+// other attention of theirs (the two batches above 101 and 180 us, 77 and 135 with one operand); one,
+// rounded once, at 64 and 128 dims, as in the multi-query tiles there: half the products.
 template <typename Tag, int D, int kFmt, bool kF32>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(kF32 || D == 256 ? 1 : 2)))
 void window_tile_kernel(const WinArgs a) {
@@ -33,7 +36,8 @@ void window_tile_kernel(const WinArgs a) {
   constexpr int RPW = kChunk / NW;            // rows a wave loads of a chunk, in one block
   constexpr int LPW = SLAB / 1024 / NW;       // KiB a wave loads of a slab
   constexpr int RPI = 1024 / ROWB;            // rows per LDS DMA
-  constexpr int kTerms = kF32 ? 3 : 1;
+  constexpr int kTerms = kF32 ? 3 : 1;                        // operands of q
+  constexpr int kPTerms = kF32 ? 3 : prob_terms<D>();         // ... of a probability
   // fp32 of 256 dims: q alone is 192 registers, and operands that the compiler reads ahead push more of
   // them into memory (24 x 32 rows of 4 KV heads over 4000 fp8 tokens: 398 us, 792 with them)
   constexpr bool kCrowded = kF32 && D == 256;
@@ -258,13 +262,13 @@ void window_tile_kernel(const WinArgs a) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[dt][j] = 0.f;
   // What m holds is the running maximum (base 2) less kRef: fp16 probabilities go up to 2^15 and end
-  // at 2^-31 of a row's largest.  It moves when a score exceeds it by kLag more.
+  // at 2^-31 of a row's largest (three operands: 2^-37).  It moves when a score exceeds it by kLag more.
   constexpr bool kF16 = std::is_same<Tag, F16Tag>::value;
-  constexpr float kLag = 8.f, kRef = kF16 ? 7.f : 0.f;
+  constexpr float kLag = lag<Tag, kPTerms>(), kRef = kF16 ? 15.f - kLag : 0.f;
   // In a chunk that every row sees whole a probability is kept above 0, so that an infinity in V
-  // meets a positive factor.
+  // meets a positive factor (three operands: pack8 keeps those of what is not below kLeastP).
   constexpr uint32_t kLeast = kF16 ? 0x00010001u : 0x00800080u;
-  constexpr float kLeastP = 0x1p-126f;
+  constexpr float kLeastP = kF16 ? 0x1p-24f : 0x1p-126f;
 
   // which keys of half x of the chunk at key t this lane's row sees (bit i: key t + 32 x + 4 hl + i)
   auto window_bits = [&](int t, int x) {
@@ -406,8 +410,8 @@ void window_tile_kernel(const WinArgs a) {
     // ---- O^T += V^T P^T, 16 keys a step: step ps takes registers 8 (ps % 2) .. of half ps / 2
 #pragma unroll
     for (int ps = 0; ps < 4; ++ps) {
-      dsp_u32x4 pop[kTerms];
-      if constexpr (kTerms == 1) {
+      dsp_u32x4 pop[kPTerms];
+      if constexpr (kPTerms == 1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           pop[0][i] = not_below(narrow2<Tag>(sc[ps >> 1][8 * (ps & 1) + 2 * i],
@@ -418,14 +422,14 @@ void window_tile_kernel(const WinArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           p[i] = fmaxf(sc[ps >> 1][8 * (ps & 1) + i], edge || bad ? 0.f : kLeastP);
-        pack8<Tag, kTerms>(p, pop);
+        pack8<Tag, kPTerms>(p, pop);
       }
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) {
         if constexpr (kCrowded) __builtin_amdgcn_sched_barrier(0);
         const dsp_u32x4 v = read_v(buf, ps, dt);
 #pragma unroll
-        for (int i = kTerms - 1; i >= 0; --i) acc[dt] = mfma32x32<Tag>(v, pop[i], acc[dt]);
+        for (int i = kPTerms - 1; i >= 0; --i) acc[dt] = mfma32x32<Tag>(v, pop[i], acc[dt]);
       }
     }
   }

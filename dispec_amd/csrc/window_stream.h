@@ -31,7 +31,8 @@ __global__ __launch_bounds__(64 * stream_block(D)) __attribute__((
 window_stream_kernel(const WinArgs a) {
   constexpr int NW = stream_block(D), TR = 16 * kRG;
   constexpr int NKK = D / 32, NT = D / 16, ROWB = 2 * D, SLAB = kStreamChunk * ROWB;
-  constexpr int kTerms = kF32 ? 3 : 1;
+  constexpr int kTerms = kF32 ? 3 : 1;                 // operands of q
+  constexpr int kPTerms = kF32 ? 3 : prob_terms<D>();  // ... of a probability (as in the tile kernel)
   constexpr bool kF16 = std::is_same<Tag, F16Tag>::value;
   // K: of a key's row a lane takes the pieces grp + 4 i; V: 64 pieces at a time
   constexpr int kKB = kFmt == kNone ? D / 2 : dsp_quant::bytes<kFmt>(D / 4);  // bytes of a lane's dims
@@ -368,9 +369,9 @@ window_stream_kernel(const WinArgs a) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) acc[g][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    constexpr float kLag = 8.f, kRef = kF16 ? 7.f : 0.f;  // (as in the tile kernel)
+    constexpr float kLag = lag<Tag, kPTerms>(), kRef = kF16 ? 15.f - kLag : 0.f;  // (as in the tile kernel)
     constexpr uint32_t kLeast = kF16 ? 0x00010001u : 0x00800080u;
-    constexpr float kLeastP = 0x1p-126f;
+    constexpr float kLeastP = kF16 ? 0x1p-24f : 0x1p-126f;
     // which keys of half h of the chunk at key t row group g's row sees (bit j: key t + 16 h + 4 grp + j)
     auto window_bits = [&](int g, int t, int h) {
       const int k = t + 16 * h + 4 * grp;
@@ -471,7 +472,7 @@ window_stream_kernel(const WinArgs a) {
           wave_lds_fence();
         }
       }
-      dsp_u32x4 pop[kRG][kTerms];
+      dsp_u32x4 pop[kRG][kPTerms];
 #pragma unroll
       for (int g = 0; g < kRG; ++g) {
         float top = -INFINITY;
@@ -499,14 +500,14 @@ window_stream_kernel(const WinArgs a) {
           p[i] = dsp_exp2(fmaf(sc[g][i >> 2][i & 3], a.scale_log2, neg_m));
           lpart[g] += p[i];
         }
-        if constexpr (kTerms == 1) {
+        if constexpr (kPTerms == 1) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             pop[g][0][i] = not_below(narrow2<Tag>(p[2 * i], p[2 * i + 1]), edge || bad_now ? 0u : kLeast);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) p[i] = fmaxf(p[i], edge || bad_now ? 0.f : kLeastP);
-          pack8<Tag, kTerms>(p, pop[g]);
+          pack8<Tag, kPTerms>(p, pop[g]);
         }
       }
 #pragma unroll
@@ -515,7 +516,7 @@ window_stream_kernel(const WinArgs a) {
 #pragma unroll
         for (int g = 0; g < kRG; ++g)
 #pragma unroll
-          for (int x = kTerms - 1; x >= 0; --x) acc[g][nt] = mfma32<Tag>(v, pop[g][x], acc[g][nt]);
+          for (int x = kPTerms - 1; x >= 0; --x) acc[g][nt] = mfma32<Tag>(v, pop[g][x], acc[g][nt]);
       }
     }
 #pragma unroll

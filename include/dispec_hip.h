@@ -424,7 +424,7 @@ int dsp_kv_gather_quant(const void* k_pool, const void* k_scale, const void* v_p
  * alignment, blocks of >= 16 tokens, num_slots a multiple of them, scale > 0 (else DSP_EUNSUPPORTED);
  * its numbers count as dsp_kv_gather_quant gives them.  Infinities and NaN of a key's V reach the rows
  * that see the key and no others.  Probabilities: fp32, but one 16-bit operand (rounded once; fp16 ends
- * at 2^-31 of a row's largest) where q has 16 bits and D is 64, 128 or 256. */
+ * at 2^-31 of a row's largest) where q has 16 bits and D is 64 or 128. */
 size_t dsp_paged_window_workspace_bytes(int32_t B, int32_t Hq, int32_t KVH, int32_t D,
                                         int32_t max_q_len, int32_t max_ctx, int32_t window,
                                         int32_t sinks, int32_t format, int32_t dtype);
