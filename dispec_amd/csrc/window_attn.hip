@@ -676,7 +676,8 @@ extern "C" int dsp_paged_window_attention(
   // (a window that reaches past every context is none)
   const bool all = window == 0 || window >= max_ctx;
   const int32_t win = all ? kWholeWindow : window, sink = all ? 0 : std::min(sinks, max_ctx);
-  const int64_t scale_bytes = D / dsp_quant::kGroup;
+  DSP_HOST_CHECK(!quant || D == 64 || D == 128 || D == 256, DSP_EUNSUPPORTED);
+  const int64_t scale_bytes = D / dsp_quant::kGroup;  // (of a quantised cache: of a head's scales)
   const bool scales_ok =
       !quant || (scale_stride_slot >= 0 && scale_stride_slot < (int64_t(1) << 26) &&
                  scale_stride_slot % scale_bytes == 0 && scale_stride_head % scale_bytes == 0 &&
