@@ -678,9 +678,11 @@ extern "C" int dsp_paged_window_attention(
   const int32_t win = all ? kWholeWindow : window, sink = all ? 0 : std::min(sinks, max_ctx);
   DSP_HOST_CHECK(!quant || D == 64 || D == 128 || D == 256, DSP_EUNSUPPORTED);
   const int64_t scale_bytes = D / dsp_quant::kGroup;  // (of a quantised cache: of a head's scales)
+  // (the kernels address the rows of a block in 32 bits, as those of codes)
+  DSP_HOST_CHECK(!quant || (scale_stride_slot >= 0 && scale_stride_slot < (int64_t(1) << 26)),
+                 DSP_EUNSUPPORTED);
   const bool scales_ok =
-      !quant || (scale_stride_slot >= 0 && scale_stride_slot < (int64_t(1) << 26) &&
-                 scale_stride_slot % scale_bytes == 0 && scale_stride_head % scale_bytes == 0 &&
+      !quant || (scale_stride_slot % scale_bytes == 0 && scale_stride_head % scale_bytes == 0 &&
                  dsp_aligned(k_scale, scale_bytes) && dsp_aligned(v_scale, scale_bytes));
   const bool rows16 = kv_stride_slot_bytes % 16 == 0 && kv_stride_head_bytes % 16 == 0 &&
                       dsp_aligned(k_cache, 16) && dsp_aligned(v_cache, 16);

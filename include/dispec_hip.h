@@ -421,7 +421,8 @@ int dsp_kv_gather_quant(const void* k_pool, const void* k_scale, const void* v_p
  * cu_q and ctx 0: zeros, not counted); keys of block ids outside the cache are counted and skipped.
  * DSP_KV_PLAIN: dtype DSP_BF16, DSP_F16 or DSP_F32, of q, cache and out, D a power of two from 8 to 256,
  * any G.  A quantised cache: q and out of `dtype`, D 64, 128 or 256, rows of 16 (FP8) or 8 (FP4) bytes
- * alignment, blocks of >= 16 tokens, num_slots a multiple of them, scale > 0 (else DSP_EUNSUPPORTED);
+ * alignment, slot strides of codes and scales from 0 to 2^26 - 1, blocks of >= 16 tokens, num_slots a
+ * multiple of them, scale > 0 (else DSP_EUNSUPPORTED);
  * its numbers count as dsp_kv_gather_quant gives them.  Infinities and NaN of a key's V reach the rows
  * that see the key and no others.  Probabilities: fp32, but one 16-bit operand (rounded once; fp16 ends
  * at 2^-31 of a row's largest) where q has 16 bits and D is 64 or 128. */
