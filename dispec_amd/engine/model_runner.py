@@ -347,8 +347,9 @@ class ModelRunner:
         """attn_backend="native": the reference's per-sequence attention
         (model_runner.py:160-185) -- the sequence's context rows gathered from the pool
         (the prologue has already appended this step's k and v, so a fresh prefill reads
-        back exactly the rows it projected), then torch SDPA with the bottom-right causal
-        mask (a drafted tree's nodes: their ancestors) and grouped KV heads.  SDPA runs in
+        back exactly the rows it projected; under a window those that a query sees), then
+        torch SDPA with the bottom-right causal mask (a drafted tree's nodes: their
+        ancestors; the window and the sinks) and grouped KV heads.  SDPA runs in
         float32: torch's bf16 batched matmul on the transposed key operand SDPA forms is
         avoided on this platform; the output is rounded to the model dtype."""
         from torch.nn.attention.bias import causal_lower_right
@@ -356,13 +357,18 @@ class ModelRunner:
         end = 0
         for m in seqs:
             start, end = end, end + m.q_len
-            keys, vals = cache.gather(layer_idx, cache.context_slots(m.block_ids, m.ctx_len))
             as_bhd = lambda t: t.float().transpose(0, 1).unsqueeze(0)  # noqa: E731
-            seen = causal_lower_right(m.q_len, m.ctx_len)
             if window:
+                # the keys that some query sees: the others' blocks may be freed or another's by now
                 key = torch.arange(m.ctx_len, device=q.device)
                 pos = key[m.ctx_len - m.q_len:, None]
+                key = key[(key < sinks) | (key > m.ctx_len - m.q_len - window)]
                 seen = (key <= pos) & ((key > pos - window) | (key < sinks))
+                slots = cache.slots_for_positions(m.block_ids, key)
+            else:
+                seen = causal_lower_right(m.q_len, m.ctx_len)
+                slots = cache.context_slots(m.block_ids, m.ctx_len)
+            keys, vals = cache.gather(layer_idx, slots)
             if m.is_tree():
                 seen = torch.zeros(m.q_len, m.ctx_len, dtype=torch.bool)
                 seen[:, :m.ctx_len - m.q_len] = True
