@@ -8,12 +8,14 @@
 // device is the current one come from the wrapper.  The library's entry points are called through the
 // addresses that dispec_amd._lib hands to bind(), as in fastcall.c.  Built with g++ (no device code).
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <exception>
 #include <limits>
 
 #include "../../include/dispec_hip.h"
@@ -253,7 +255,8 @@ PyObject* gather(PyObject* const* a) {
   return both;
 }
 
-// No C++ exception leaves a binding: what torch throws becomes a RuntimeError.
+// No C++ exception leaves a binding: what torch throws becomes the Python exception that torch makes of it
+// (of a failed allocation an OutOfMemoryError).
 template <PyObject* (*F)(PyObject* const*), int kArgs>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != kArgs) {
@@ -264,8 +267,8 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return F(args);
   } catch (const Slow&) {
     Py_RETURN_NONE;
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
 }
