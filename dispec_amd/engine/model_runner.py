@@ -92,6 +92,9 @@ class _Batch:
 
 
 _BACKENDS = ("hip", "native")
+# families (config.model_type) whose sliding layers are their full ones with a window.  Others' go with parts
+# that the runner does not have: capped scores, learned sinks, norms or a RoPE of their own.
+_SLIDING_FAMILIES = ("qwen2", "qwen3")
 
 
 def _compute_dtype(model) -> torch.dtype:
@@ -114,9 +117,10 @@ class _FusedLayer:
 
 class ModelRunner:
     """window, sinks: a sliding window of so many tokens (0: none), with the first `sinks` tokens of a
-    sequence visible beside it, for the layers that have none of their own; layers that the model's
-    config calls "sliding_attention" have its sliding_window.  Blocks that hold no visible token may be
-    freed (their table entries are not read)."""
+    sequence visible beside it, for the layers that have none of their own; layers that the config of a
+    model of `_SLIDING_FAMILIES` calls "sliding_attention" have its sliding_window.  Other families' sliding
+    layers, and layers of other kinds than sliding and full, are refused.  Blocks that hold no visible
+    token may be freed (their table entries are not read)."""
 
     def __init__(self, model, attn_backend: str = "hip", fuse: bool = False, window: int = 0,
                  sinks: int = 0):
@@ -147,6 +151,9 @@ class ModelRunner:
         if unknown:
             raise ValueError(f"{type(model).__name__} uses {sorted(unknown)} layers, which the paged "
                              "attention path does not implement")
+        if "sliding_attention" in kinds and getattr(cfg, "model_type", None) not in _SLIDING_FAMILIES:
+            raise ValueError(f"{type(model).__name__} uses sliding-window attention layers: the paged "
+                             f"attention path implements those of {_SLIDING_FAMILIES}")
         own = getattr(cfg, "sliding_window", None)
         if "sliding_attention" in kinds and not own:
             raise ValueError(f"{type(model).__name__}: sliding_attention layers without a "
