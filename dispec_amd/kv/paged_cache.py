@@ -116,6 +116,8 @@ def commit_path(key, value, block_table, cu_q, ctx_lens, path, num_accepted, blo
 
 
 class PagedKVCache:
+    format = None   # a quantised cache's (kv.quant_cache); None: numbers of `dtype`
+
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, num_kv_heads: int,
                  head_dim: int, dtype: torch.dtype = torch.bfloat16, device: str = "cuda"):
         self.num_layers = num_layers
@@ -399,6 +401,7 @@ class PagedKVCache:
     def copy_blocks_device(self, src: "PagedKVCache", src_ids: torch.Tensor,
                            dst_ids: torch.Tensor) -> None:
         """Block copy src -> self with int32 id arrays already on the GPU."""
+        self._same_format(src)
         _lib.check(_lib.lib().dsp_kv_copy_blocks(
             src.key.data_ptr(), src.value.data_ptr(), src.layer_bytes, src.num_blocks,
             self.key.data_ptr(), self.value.data_ptr(), self.layer_bytes, self.num_blocks,
@@ -408,6 +411,7 @@ class PagedKVCache:
     def copy_block_fanout_device(self, src: "PagedKVCache", src_block: int,
                                  dst_ids: torch.Tensor) -> None:
         """Block src_block of src copied into every block of dst_ids (int32, on the GPU)."""
+        self._same_format(src)
         _lib.check(_lib.lib().dsp_kv_copy_block_fanout(
             src.key.data_ptr(), src.value.data_ptr(), src.layer_bytes, src.num_blocks,
             self.key.data_ptr(), self.value.data_ptr(), self.layer_bytes, self.num_blocks,
@@ -423,8 +427,14 @@ class PagedKVCache:
         self._after()
 
     # -- block copies (copy-on-write, prefix-cache spill) ----------------------------------
+    def _same_format(self, src: "PagedKVCache") -> None:
+        if src.format != self.format:
+            raise ValueError(f"block copy from a {src.format or 'plain'} cache into a "
+                             f"{self.format or 'plain'} one: read and write rows instead")
+
     def copy_blocks_from(self, src: "PagedKVCache", src_ids: list[int], dst_ids: list[int]) -> None:
         """dst[l, block d] = src[l, block s] for every layer, K and V."""
+        self._same_format(src)
         if len(src_ids) != len(dst_ids):
             raise ValueError("src_ids and dst_ids differ in length")
         if (src.num_layers, src.block_bytes) != (self.num_layers, self.block_bytes):

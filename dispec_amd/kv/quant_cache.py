@@ -303,11 +303,6 @@ class QuantPagedKVCache(PagedKVCache):
             self.copy_blocks_device(src, ids[0], ids[1])
         self._after()
 
-    def _same_format(self, src) -> None:
-        if getattr(src, "format", None) != self.format:
-            raise ValueError(f"block copy from a {getattr(src, 'format', 'plain')} cache into a "
-                             f"{self.format} one: read and write rows instead")
-
     def commit_path(self, block_table, cu_q, ctx_lens, path, num_accepted) -> None:
         for k, v in ((self.key, self.value), (self.key_scale, self.value_scale)):
             commit_path(k, v, block_table, cu_q, ctx_lens, path, num_accepted,
