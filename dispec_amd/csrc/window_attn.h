@@ -25,8 +25,8 @@ constexpr int prob_terms() {
   return D > 128 ? 3 : 1;
 }
 // By how much, in powers of two, a score may exceed the running maximum before it moves.  (fp16 in three
-// operands: by little, so that a row's largest probability is 2^13 or more, and fp16's end, 2^-24, below
-// 2^-37 of it: less than half of fp32's last bit for 4096 keys in a row)
+// operands: by little, so that a row's largest probability is 2^13 or more and what pack8 keeps above 0
+// in the second and third, 2^-24 each, is 2^-36 of it: fp32's last bit after 4096 such keys)
 template <typename Tag, int kTerms>
 constexpr float lag() {
   return std::is_same<Tag, F16Tag>::value && kTerms == 3 ? 2.f : 8.f;

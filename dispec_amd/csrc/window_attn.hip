@@ -262,7 +262,7 @@ void window_tile_kernel(const WinArgs a) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[dt][j] = 0.f;
   // What m holds is the running maximum (base 2) less kRef: fp16 probabilities go up to 2^15 and end
-  // at 2^-31 of a row's largest (three operands: 2^-37).  It moves when a score exceeds it by kLag more.
+  // at 2^-31 of a row's largest (three operands: 2^-36).  It moves when a score exceeds it by kLag more.
   constexpr bool kF16 = std::is_same<Tag, F16Tag>::value;
   constexpr float kLag = lag<Tag, kPTerms>(), kRef = kF16 ? 15.f - kLag : 0.f;
   // In a chunk that every row sees whole a probability is kept above 0, so that an infinity in V

@@ -171,3 +171,53 @@ def test_infinities_under_several_operands(hip, dtype, q_lens, spread):
         want = keep.clone()
         want[torch.from_numpy(c.see[0][:, key]).nonzero()[:, 0].to("cuda"), 2:4, d] = x
         assert torch.equal(torch.nan_to_num(got, 1e4, 2e4, 3e4), torch.nan_to_num(want, 1e4, 2e4, 3e4)), key
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n", [6, 40, 150])
+@pytest.mark.parametrize("size,step", [(10, 1), (20, 8), (24, 8), (25, 4), (25, 8), (26, 8), (27, 16),
+                                       (28, 32)])
+@pytest.mark.parametrize("scale", [math.log(2.0), 1.0])
+def test_large_scores(hip, dtype, D, n, size, step, scale):
+    """Scores of 2^size and, from key 40 or 170 on, `step` more (both exact in fp32; a later one
+    exceeds the first by a step of fp32 or a few): no operand overflows, and the weights are 1 and
+    e^(scale step), whose exponent is off by a rounding of it and of log2(e) scale, 2^-23 of it
+    each at most."""
+    for turn in (40, 170):
+        c = Case([n], [300], 4, 2, D, dtype, seed=size)
+        c.dk.zero_()
+        c.dq.zero_()
+        first, second = (torch.from_numpy(s).to(c.dk.device)
+                         for s in (c.slots[0][:turn], c.slots[0][turn:]))
+        c.dq[:, :, 0], c.dq[:, :, 1] = 2.0 ** (size // 2), 1
+        c.dk[:, :, 0] = 2.0 ** (size - size // 2)
+        c.dk[second, :, 1] = step
+        c.dv[first], c.dv[second] = 1.0, 0.0
+        got = c.call(scale=scale).double().cpu()
+        total = torch.from_numpy(c.see[0].sum(1)).double()[:, None, None]
+        ones = total.clamp_max(turn)
+        # of the first keys, whose value is 1
+        share = ones / (ones + (total - ones) * math.exp(scale * step))
+        half = torch.finfo(dtype).eps / 2
+        bound = share * (2 * half * (1 + half) + 2.0 ** -21 * step + 300 * 2.0 ** -24)
+        if dtype == F16:
+            # the running maximum is a multiple of fp32's step at that size, up to half of one above
+            # what it stands for, and the end of fp16 as much nearer
+            unit = 2.0 ** (math.floor(math.log2(2.0 ** size * scale * math.log2(math.e))) - 23)
+            bound = bound + 2.0 ** -25
+            if D < 256:
+                bound = bound + ones * 2.0 ** (-31 + unit / 2) / total
+            else:
+                # Three operands: the second and third are kept above 0, 2^-24 each, so a p is held
+                # 2^-23 too large at most.  A row's largest p is 2^13 at first; with the running maximum
+                # rounded to a step it is 2^(13 - unit / 2) to 2^(13 + unit / 2), and where that exceeds
+                # 2^15 the maximum moves one step up: more than 2^(15 - unit).  The row sum, without
+                # these 2^-23, is as many of the largest p as there are later keys (or all).
+                largest = min(13 - unit / 2, 15 - unit)
+                many = torch.where(total > ones, total - ones, total)
+                bound = bound + ones * 2.0 ** (-23 - largest) / many
+        err = (got - share).abs()
+        assert bool(torch.isfinite(got).all()), turn
+        assert bool((err <= bound).all()), (turn, float((err / bound).max()))
