@@ -106,10 +106,12 @@ class HipGraphDecoder:
         host[ctx_off + B: tab_off] = torch.arange(B + 1, dtype=torch.int32)   # cu_q: one row each
         dev = torch.zeros(n, dtype=torch.int32, device=dev_)
         i64 = dev[:6 * B].view(torch.int64)
+        workspace = (decode_workspace(B, self.r.num_heads, self.r.num_kv_heads, self.r.head_dim,
+                                      W * bs, dev_)
+                     if self.r._shares_workspace(self.cache, W * bs) else None)
         meta = _Batch(block_table=dev[tab_off:].view(B, W), ctx_lens=dev[ctx_off:ctx_off + B],
                       cu_q=dev[ctx_off + B:tab_off], max_q_len=1, max_ctx=W * bs, decode=True,
-                      workspace=decode_workspace(B, self.r.num_heads, self.r.num_kv_heads,
-                                                 self.r.head_dim, W * bs, dev_))
+                      workspace=workspace)
         return _Graph(B, W, host, dev, i64[:B], i64[B:2 * B], i64[2 * B:], meta,
                       torch.cuda.Event())
 

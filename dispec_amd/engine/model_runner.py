@@ -391,6 +391,12 @@ class ModelRunner:
             out[start:end] = o[0].transpose(0, 1)
         return out
 
+    def _shares_workspace(self, cache: PagedKVCache, max_ctx: int) -> bool:
+        """Whether some layer runs one of the launches that take the batch's workspace (windowed and
+        quantised attention bring their own)."""
+        return (self.attn_backend == "hip" and not isinstance(cache, QuantPagedKVCache)
+                and any(not 0 < w < max_ctx for w, _ in self.windows))
+
     @torch.inference_mode()
     def forward(self, token_ids: torch.Tensor, positions: torch.Tensor,
                 write_slots: torch.Tensor, seq_meta: list[SeqMeta],
@@ -409,8 +415,7 @@ class ModelRunner:
         multi-query kernel, which reads those blocks once for the batch."""
         cos, sin = self.rope(positions)
         x = self.embed(token_ids)
-        if (batch.workspace is None and self.attn_backend == "hip"
-                and not isinstance(cache, QuantPagedKVCache)):
+        if batch.workspace is None and self._shares_workspace(cache, batch.max_ctx):
             B = batch.ctx_lens.shape[0]
             if batch.tree_mask is not None:
                 batch.workspace = tree_workspace(B, self.num_heads, self.num_kv_heads,
