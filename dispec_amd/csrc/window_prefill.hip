@@ -13,11 +13,15 @@
 // barrier that ends the last phase before its use.
 //
 // Four prompts' chunks of 2048 tokens over 8192, 32 query heads over 8 of 128 dims, a window of 4096
-// (5.5e11 operations): 645 us a call in a tight loop, 738 by the tile kernel on the same card; 545, 1010
-// TFLOP/s, among other work (8192^3 products through the library: 1064).  Four chunks of 512 over 3000 to
-// 4608 fp8 tokens: 177 us (190).  In the tight loop a chunk takes 4300 cycles, of which the products of
-// both groups are 2050: a product phase is 1250 (its 128 KB of operands pass LDS in 1020), the vector work
-// beside it 1500 (512 of them the exponentials), and a wave's four loads hold it for 400.
+// (5.5e11 operations): 645 us a call in a tight loop, 738 by the tile kernel on the same card; 545 to 575,
+// 1010 to 957 TFLOP/s, among other work (8192^3 products through the library: 1064 and 1152 on two cards).
+// Four chunks of 512 over 3247 to 4608 fp8 tokens: 190 us, over 3766 each, as many keys, 148: a workgroup
+// takes one tile, and the longest context decides; over bf16 154 and 133, so that widening is a tenth.
+// A probability is one 16-bit operand, rounded once (at these head dims the multi-query tiles hold it so;
+// a second one is half as many products again): 2.3e-3 from 64 bits in bf16, 1.7e-3 of it the output's own
+// rounding.  In the tight loop a chunk takes 4300 cycles, of which the products of both groups are 2050: a
+// product phase is 1250 (its 128 KB of operands pass LDS in 1020), the vector work beside it 1500 (512 of
+// them the exponentials), and a wave's four loads hold it for 400.
 #include "window_attn.h"
 
 namespace dsp_window {

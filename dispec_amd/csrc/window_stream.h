@@ -14,8 +14,10 @@
 // Bound by HBM where there is much to read: 16 contexts of 32768 fp8 tokens (1.1 GB) 196 us, 5.8 TB/s, of
 // which the merge is 4.7; 32 tokens under a window of 1024, 131 MB, 28 us; small calls by the chain of
 // lengths, block ids and first keys, 4 us, and 1.6 us a chunk: 48 over up to 2048 fp4 tokens 17 us, 24
-// verifies of 1 to 9 under a window of 512 14.  Slower: two chunks ahead in registers (37, 214 and 19 us
-// for 29, 194 and 18), four waves a workgroup and three a SIMD (33, 204, 19).
+// verifies of 1 to 9 under a window of 512 14.  16-bit q: probabilities as in the tile kernel, one operand at
+// 64 and 128 dims, three at 256 (32 tokens under a window of 2048, 8 KV heads of 256: 96 us, 95 with one).
+// Slower: two chunks ahead in registers (37, 214 and 19 us for 29, 194 and 18), four waves a workgroup and
+// three a SIMD (33, 204, 19).
 #pragma once
 
 #include "window_attn.h"
